@@ -354,6 +354,61 @@ MPT_API int mpt_nvfp4_quantize(const float *in, float *out, float *block_scales,
                                int64_t rows, int64_t cols, float global_scale, void *workspace,
                                float *global_scale_out, void *stream);
 
+/* ---- serving from packed block formats (NEW: no reference counterpart) --------------------------------
+ * Operators that read the packed codes of the quantizers above.  `dtype` is the type of the dense tensors;
+ * sums, softmax statistics and scales are held in fp32. */
+enum { MPT_DTYPE_F32 = 0, MPT_DTYPE_BF16 = 1, MPT_DTYPE_F16 = 2 };
+enum { MPT_BLOCK_MXFP4 = 0, MPT_BLOCK_NVFP4 = 1 };
+
+/* y[rows, n_out] = x[rows, n_in] W^T + bias, W [n_out, n_in] as packed E2M1 codes ([n_out, n_in / 2] bytes,
+ * element 2i in the low nibble) with MXFP4 scales (E8M0, [n_out, n_in / 32]) or NVFP4 scales (E4M3,
+ * [n_out, n_in / 16], times the fp32 scale at the device address `global_scale`, 1 where it is NULL).  n_in is a
+ * multiple of 32; `codes` begins at a multiple of 16 bytes; x and y are contiguous; `bias` may be NULL.
+ * `workspace`: mpt_block_linear_workspace_bytes() bytes at a multiple of 256, of this call alone until it is done. */
+MPT_API size_t mpt_block_linear_workspace_bytes(int64_t rows, int64_t n_out, int64_t n_in, int format, int dtype);
+MPT_API int mpt_block_linear(const void *x, const uint8_t *codes, const uint8_t *scales, const float *global_scale,
+                             const void *bias, void *y, int64_t rows, int64_t n_out, int64_t n_in, int format, int dtype,
+                             void *workspace, size_t workspace_bytes, void *stream);
+
+/* A cache of K and V in MX format, in pages: codes [num_pages, heads, page, dim] bytes (E4M3) or
+ * [num_pages, heads, page, dim / 2] (E2M1), scales [num_pages, heads, page, dim / 32] E8M0 bytes.  dim is a multiple
+ * of 32 up to 256, page a power of two from 8 to 256; codes begin at a multiple of 16 bytes. */
+typedef struct {
+    uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+    int64_t num_pages;
+    int heads, dim, page, elem_format;
+} mpt_mx_cache;
+
+/* A batch of sequences: token t of sequence s lies in page pages[s * width + t / page] (an entry outside
+ * [0, num_pages) holds no tokens); lens[s] counts its tokens, the new ones among them; the new rows of
+ * sequence s are [starts[s], starts[s + 1]) of `rows`, or, where `starts` is NULL, rows / seqs of them each.  New row i
+ * of n stands at position lens[s] - n + i; rows before position 0, and rows behind the last sequence, stand nowhere.
+ * pages, lens and starts are device pointers. */
+typedef struct {
+    const int32_t *pages, *lens, *starts;
+    int64_t rows;
+    int seqs, width;
+} mpt_mx_batch;
+
+/* Quantizes the new rows of K and V into the cache: for each block of 32 the codes of mpt_mx_quantize.  Rows that stand
+ * nowhere, or in no page, are not written.  k, v: [rows, heads, dim] with element strides {sequence, row, head} (the
+ * first used only without `starts`), the last dimension contiguous. */
+MPT_API int mpt_mx_cache_write(const mpt_mx_cache *cache, const mpt_mx_batch *batch, const void *k, const void *v, int dtype,
+                               const int64_t *k_strides, const int64_t *v_strides, void *stream);
+/* Reads the new rows back: k, v [rows, heads, dim] contiguous; zeros for rows that stand nowhere. */
+MPT_API int mpt_mx_cache_read(const mpt_mx_cache *cache, const mpt_mx_batch *batch, void *k, void *v, int dtype, void *stream);
+
+/* Attention of the new rows over their sequences' tokens in the cache: out = softmax(scale * q K^T) V over the tokens t
+ * at most at the row's position p with window == 0, t > p - window or t < sinks.  Query head h reads kv head
+ * h / (q_heads / heads).  q: [rows, q_heads, dim] with strides as above; out: contiguous.  A row that sees nothing
+ * gives zeros; rows behind the last sequence are zeroed where `zero_tail` is set and left as they were otherwise.
+ * `workspace`: mpt_mx_attention_workspace_bytes() bytes at a multiple of 256, of this call alone until it is done. */
+MPT_API size_t mpt_mx_attention_workspace_bytes(const mpt_mx_cache *cache, const mpt_mx_batch *batch, int q_heads, int dtype,
+                                                int window, int sinks);
+MPT_API int mpt_mx_attention(const mpt_mx_cache *cache, const mpt_mx_batch *batch, const void *q, int dtype,
+                             const int64_t *q_strides, int q_heads, float scale, int window, int sinks, void *out,
+                             int zero_tail, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- quantized optimizer steps and tensor scaling -----------------------------------------------------
  * One launch updates many tensors in place (up to 40 per launch; more are split over launches).  The
  * table is a HOST array; nothing is allocated.  Quantizers are the reference's callables of the form

@@ -41,6 +41,17 @@ class Format(C.Structure):
         return Format(2, 0, 0, int(subnormals), 0, 1, 1, P, int(is_signed), int(overflow_policy))
 
 
+class MxCache(C.Structure):
+    """``mpt_mx_cache`` of include/mptorch_b200.h."""
+    _fields_ = [("k_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_codes", C.c_void_p), ("v_scales", C.c_void_p), ("num_pages", C.c_int64),
+                ("heads", C.c_int), ("dim", C.c_int), ("page", C.c_int), ("elem_format", C.c_int)]
+
+
+class MxBatch(C.Structure):
+    """``mpt_mx_batch`` of include/mptorch_b200.h."""
+    _fields_ = [("pages", C.c_void_p), ("lens", C.c_void_p), ("starts", C.c_void_p), ("rows", C.c_int64), ("seqs", C.c_int), ("width", C.c_int)]
+
+
 def lib() -> C.CDLL:
     global _lib
     if _lib is None:
@@ -93,6 +104,10 @@ def lib() -> C.CDLL:
             "mpt_scale_quantize": [p, p, i64, i64, C.c_double, i32, i32, i32, i32, i32, i32, p, p, sz, p],
             "mpt_mx_quantize": [p, p, p, p, i64, i64, i32, i32, p],
             "mpt_nvfp4_quantize": [p, p, p, p, p, i64, i64, C.c_float, p, p, p],
+            "mpt_block_linear": [p, p, p, p, p, p, i64, i64, i64, i32, i32, p, sz, p],
+            "mpt_mx_cache_write": [p, p, p, p, i32, p, p, p],
+            "mpt_mx_cache_read": [p, p, p, p, i32, p],
+            "mpt_mx_attention": [p, p, p, i32, p, i32, C.c_float, i32, i32, p, i32, p, sz, p],
         }
         for name, args in sig.items():
             fn = getattr(L, name, None)
@@ -100,6 +115,8 @@ def lib() -> C.CDLL:
                 continue
             fn.restype = i32
             fn.argtypes = args
+        L.mpt_block_linear_workspace_bytes.argtypes, L.mpt_block_linear_workspace_bytes.restype = [i64, i64, i64, i32, i32], sz
+        L.mpt_mx_attention_workspace_bytes.argtypes, L.mpt_mx_attention_workspace_bytes.restype = [p, p, i32, i32, i32, i32], sz
         _lib = L
     return _lib
 

@@ -750,3 +750,191 @@ def nvfp4_quantize(a, global_scale=None, return_scales=False, return_codes=False
              stream_ptr(a.device))
     res = (o,) + ((sc, gs_out) if return_scales else ()) + ((codes, scodes) if return_codes else ())
     return res if len(res) > 1 else o
+
+
+# ---------------------------------------------------------------------------------- serving from packed block formats (new)
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _dense_type(who, x):
+    if x.dtype not in _DTYPE:
+        raise RuntimeError("%s: float32, bfloat16 or float16 expected, not %s" % (who, x.dtype))
+    return _DTYPE[x.dtype]
+
+
+def _no_gradient(who, *tensors):
+    if any(t.requires_grad for t in tensors) and torch.is_grad_enabled():
+        raise RuntimeError("%s: has no backward pass; call it under torch.no_grad()" % who)
+
+
+def _whole(who, what, t, dtype, shape):
+    """``t`` is contiguous, of the given type and shape (None: any extent)."""
+    if t.dtype != dtype or t.dim() != len(shape) or not t.is_contiguous() or any(w is not None and w != n for w, n in zip(shape, t.shape)):
+        raise RuntimeError("%s: %s must be a contiguous %s tensor of shape %s" % (who, what, str(dtype).split(".")[-1],
+                                                                                  ["any" if w is None else w for w in shape]))
+
+
+def _on_device(who, like, **tensors):
+    for what, t in {"the first tensor": like, **tensors}.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("%s: %s must be a CUDA tensor" % (who, what))
+        if t.device != like.device:
+            raise RuntimeError("%s: %s is on %s, expected %s" % (who, what, t.device, like.device))
+
+
+def _workspace(need, device):
+    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+
+
+def _block_linear(who, x, codes, scales, global_scale, bias, fmt):
+    dtype, group = _dense_type(who, x), 16 if fmt else 32
+    if x.dim() < 1 or x.shape[-1] % 32:
+        raise RuntimeError("%s: the last dimension of x must be a multiple of 32" % who)
+    n_in = x.shape[-1]
+    _whole(who, "codes", codes, torch.uint8, (None, n_in // 2))
+    n_out = codes.shape[0]
+    _whole(who, "scales", scales, torch.uint8, (n_out, n_in // group))
+    if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (n_out,)):
+        raise RuntimeError("%s: bias must be [%d] of x's type" % (who, n_out))
+    if global_scale is not None and (global_scale.dtype != torch.float32 or global_scale.numel() != 1):
+        raise RuntimeError("%s: global_scale must be one float32 value" % who)
+    _no_gradient(who, x, *([bias] if bias is not None else []))
+    _on_device(who, x, codes=codes, scales=scales, bias=bias, global_scale=global_scale)
+    with torch.cuda.device(x.device):
+        x, bias = x.contiguous(), None if bias is None else bias.contiguous()
+        y = torch.empty(x.shape[:-1] + (n_out,), dtype=x.dtype, device=x.device)
+        if y.numel():
+            rows = y.numel() // n_out
+            need = _cabi.lib().mpt_block_linear_workspace_bytes(rows, n_out, n_in, fmt, dtype)
+            ws = _workspace(need, x.device)
+            call("mpt_block_linear", ptr(x), ptr(codes), ptr(scales), ptr(global_scale), ptr(bias), ptr(y), rows, n_out, n_in, fmt, dtype, ptr(ws),
+                 need, stream_ptr(x.device))
+    return y
+
+
+def mx_linear(x, codes, scales, bias=None):
+    """x W^T + bias with W as packed MXFP4 codes and E8M0 scales."""
+    if _ext is not None:
+        return _ext.mx_linear(x, codes, scales, bias)
+    return _block_linear("mx_linear", x, codes, scales, None, bias, 0)
+
+
+def nvfp4_linear(x, codes, scales, global_scale, bias=None):
+    """x W^T + bias with W as packed NVFP4 codes, E4M3 scales and a tensor scale."""
+    if _ext is not None:
+        return _ext.nvfp4_linear(x, codes, scales, global_scale, bias)
+    return _block_linear("nvfp4_linear", x, codes, scales, global_scale, bias, 1)
+
+
+def _serving_call(who, cache, pages, lens, starts, rows):
+    if len(cache) != 4:
+        raise RuntimeError("%s: the cache is (k_codes, k_scales, v_codes, v_scales)" % who)
+    names = ("k_codes", "k_scales", "v_codes", "v_scales")
+    for what, t in zip(names, cache):
+        _whole(who, what, t, torch.uint8, (None,) * 4)
+    (num, heads, page, width), dim = cache[0].shape, cache[1].shape[3] * 32
+    if width != dim and width * 2 != dim:
+        raise RuntimeError("%s: %d bytes of codes do not go with %d scales a row" % (who, width, dim // 32))
+    for what, t, w in zip(names, cache, (width, dim // 32) * 2):
+        _whole(who, what, t, torch.uint8, (num, heads, page, w))
+    _whole(who, "pages", pages, torch.int32, (None, None))
+    seqs = pages.shape[0]
+    _whole(who, "lens", lens, torch.int32, (seqs,))
+    if starts is not None:
+        _whole(who, "starts", starts, torch.int32, (seqs + 1,))
+    if heads > 65535 or dim > 256 or page > 256:
+        raise RuntimeError("%s: extents out of range" % who)
+    c = _cabi.MxCache(*(t.data_ptr() for t in cache), num, heads, dim, page, 0 if width == dim else 1)
+    b = _cabi.MxBatch(pages.data_ptr(), lens.data_ptr(), None if starts is None else starts.data_ptr(), rows, seqs, pages.shape[1])
+    return c, b
+
+
+def _row_shape(who, what, t, starts, seqs, dim):
+    if t.dim() != (4 if starts is None else 3) or (starts is None and t.shape[0] != seqs):
+        raise RuntimeError("%s: %s must be %s" % (who, what, "[sequences, new, heads, head_dim]" if starts is None else
+                                                  "[rows, heads, head_dim] where starts is given"))
+    if t.shape[-1] != dim:
+        raise RuntimeError("%s: %s has rows of %d values, the cache of %d" % (who, what, t.shape[-1], dim))
+
+
+def _row_count(who, what, t):
+    if t.dim() not in (3, 4):
+        raise RuntimeError("%s: %s needs three or four dimensions" % (who, what))
+    return t.shape[0] if t.dim() == 3 else t.shape[0] * t.shape[1]
+
+
+def _row_strides(t):
+    import ctypes
+
+    return (ctypes.c_int64 * 3)(t.stride(0) if t.dim() == 4 else 0, t.stride(t.dim() - 3), t.stride(t.dim() - 2))
+
+
+def mx_cache_write(k, v, cache, pages, lens, starts=None):
+    """Quantizes the new rows of K and V into the pages of an MX cache."""
+    if _ext is not None:
+        return _ext.mx_cache_write(k, v, list(cache), pages, lens, starts)
+    import ctypes
+
+    who = "mx_cache_write"
+    dtype = _dense_type(who, k)
+    c, b = _serving_call(who, cache, pages, lens, starts, _row_count(who, "k", k))
+    _row_shape(who, "k", k, starts, b.seqs, c.dim)
+    if k.shape[-2] != c.heads:
+        raise RuntimeError("%s: k has %d heads, the cache %d" % (who, k.shape[-2], c.heads))
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise RuntimeError("%s: v must have the shape and type of k" % who)
+    _no_gradient(who, k, v)
+    _on_device(who, k, v=v, k_codes=cache[0], k_scales=cache[1], v_codes=cache[2], v_scales=cache[3], pages=pages, lens=lens, starts=starts)
+    with torch.cuda.device(k.device):
+        k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (k, v))
+        call("mpt_mx_cache_write", ctypes.byref(c), ctypes.byref(b), ptr(k), ptr(v), dtype, _row_strides(k), _row_strides(v), stream_ptr(k.device))
+
+
+def mx_cache_read(cache, pages, lens, rows, starts=None, dtype=torch.float32):
+    """The newest rows of K and V as the cache holds them."""
+    if _ext is not None:
+        return tuple(_ext.mx_cache_read(list(cache), pages, lens, rows, starts, dtype))
+    import ctypes
+
+    who = "mx_cache_read"
+    if rows < 0:
+        raise RuntimeError("%s: a negative number of rows" % who)
+    c, b = _serving_call(who, cache, pages, lens, starts, rows if starts is not None else rows * pages.shape[0])
+    _on_device(who, cache[0], k_scales=cache[1], v_codes=cache[2], v_scales=cache[3], pages=pages, lens=lens, starts=starts)
+    k = torch.empty(((rows,) if starts is not None else (b.seqs, rows)) + (c.heads, c.dim), dtype=dtype, device=cache[0].device)
+    v = torch.empty_like(k)
+    with torch.cuda.device(k.device):
+        call("mpt_mx_cache_read", ctypes.byref(c), ctypes.byref(b), ptr(k), ptr(v), _dense_type(who, k), stream_ptr(k.device))
+    return k, v
+
+
+def mx_attention(q, cache, pages, lens, starts=None, scale=1.0, window=0, sinks=0, out=None):
+    """Attention of the new rows over their sequences' tokens in an MX cache."""
+    if _ext is not None:
+        return _ext.mx_attention(q, list(cache), pages, lens, starts, scale, window, sinks, out)
+    import ctypes
+
+    who = "mx_attention"
+    dtype = _dense_type(who, q)
+    c, b = _serving_call(who, cache, pages, lens, starts, _row_count(who, "q", q))
+    _row_shape(who, "q", q, starts, b.seqs, c.dim)
+    heads = q.shape[-2]
+    if c.heads < 1 or heads < 1 or heads % c.heads:
+        raise RuntimeError("%s: %d query heads do not divide among %d kv heads" % (who, heads, c.heads))
+    if not (0 <= window <= INT_MAX and 0 <= sinks <= INT_MAX):
+        raise RuntimeError("%s: window and sinks must not be negative" % who)
+    if out is not None:
+        _whole(who, "out", out, q.dtype, tuple(q.shape))
+    _no_gradient(who, q)
+    _on_device(who, q, out=out, k_codes=cache[0], k_scales=cache[1], v_codes=cache[2], v_scales=cache[3], pages=pages, lens=lens, starts=starts)
+    with torch.cuda.device(q.device):
+        q = q if q.stride(-1) == 1 else q.contiguous()
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+        if o.numel():
+            need = _cabi.lib().mpt_mx_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(b), heads, dtype, window, sinks)
+            ws = _workspace(need, q.device)
+            call("mpt_mx_attention", ctypes.byref(c), ctypes.byref(b), ptr(q), dtype, _row_strides(q), heads, scale, window, sinks, ptr(o),
+                 int(out is None), ptr(ws), need, stream_ptr(q.device))
+    return o

@@ -26,9 +26,10 @@ NVCC_FLAGS = [
 # Every fp32 multiply/add of the algorithms is written with an explicit rounding intrinsic, which the
 # compiler never contracts.  -fmad=false additionally keeps it from contracting the few plain
 # expressions that remain.  reduce.cu is the exception: it calls expf/logf, and those must compile
-# exactly as they do in the reference's CUDA build (nvcc defaults) to give the same bits.
+# exactly as they do in the reference's CUDA build (nvcc defaults) to give the same bits.  So are the
+# products with packed weights and the attention, whose sums have no prescribed roundings.
 EXTRA_FLAGS = {"reduce.cu": [], "rows_softmax_fwd.cu": [], "rows_softmax_bwd.cu": [], "rows_softmax_lse.cu": [], "rows_layernorm_fwd.cu": [],
-               "rows_layernorm_bwd.cu": []}
+               "rows_layernorm_bwd.cu": [], "blocklinear.cu": [], "attention.cu": []}
 DEFAULT_EXTRA = ["-fmad=false"]
 
 

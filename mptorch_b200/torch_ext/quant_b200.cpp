@@ -9,6 +9,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <array>
+#include <optional>
 #include <vector>
 
 #include "mptorch_b200.h"
@@ -412,6 +414,182 @@ std::vector<at::Tensor> nvfp4_quantize(at::Tensor a, double global_scale, bool r
     if (return_codes) { out.push_back(codes); out.push_back(scodes); }
     return out;
 }
+// ---- serving from packed block formats (no quant_cuda counterpart).  Shapes and types are checked before devices. ----
+int dense_type(const char* who, const at::Tensor& x) {
+    switch (x.scalar_type()) {
+        case at::kFloat: return MPT_DTYPE_F32;
+        case at::kBFloat16: return MPT_DTYPE_BF16;
+        case at::kHalf: return MPT_DTYPE_F16;
+        default: TORCH_CHECK(false, who, ": float32, bfloat16 or float16 expected, not ", x.scalar_type());
+    }
+}
+void no_gradient(const char* who, const at::Tensor& x) {
+    TORCH_CHECK(!(x.requires_grad() && at::GradMode::is_enabled()), who, ": has no backward pass; call it under torch.no_grad()");
+}
+void bytes_tensor(const char* who, const char* what, const at::Tensor& t, int64_t dim) {
+    TORCH_CHECK(t.scalar_type() == at::kByte && t.dim() == dim && t.is_contiguous(), who, ": ", what, " must be a contiguous uint8 tensor with ", dim,
+                " dimensions");
+}
+void same_device(const char* who, const char* what, const at::Tensor& t, const at::Tensor& as) {
+    TORCH_CHECK(t.is_cuda(), who, ": ", what, " must be a CUDA tensor");
+    TORCH_CHECK(t.device() == as.device(), who, ": ", what, " is on ", t.device(), ", expected ", as.device());
+}
+at::Tensor workspace(size_t bytes, const at::Tensor& like) {
+    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
+at::Tensor block_linear(const std::string& who_s, const at::Tensor& x_in, const at::Tensor& codes, const at::Tensor& scales,
+                        const std::optional<at::Tensor>& global_scale, const std::optional<at::Tensor>& bias, int format) {
+    const char* who = who_s.c_str();
+    const int dtype = dense_type(who, x_in);
+    bytes_tensor(who, "codes", codes, 2);
+    bytes_tensor(who, "scales", scales, 2);
+    TORCH_CHECK(x_in.dim() >= 1, who, ": x needs at least one dimension");
+    const int64_t n_in = x_in.size(-1), n_out = codes.size(0), group = format == MPT_BLOCK_NVFP4 ? 16 : 32;
+    TORCH_CHECK(n_in % 32 == 0, who, ": the last dimension of x (", n_in, ") must be a multiple of 32");
+    TORCH_CHECK(codes.size(1) * 2 == n_in, who, ": codes hold ", codes.size(1) * 2, " values a row, x has ", n_in);
+    TORCH_CHECK(scales.size(0) == n_out && scales.size(1) * group == n_in, who, ": scales must be [", n_out, ", ", n_in / group, "]");
+    if (bias) TORCH_CHECK(bias->scalar_type() == x_in.scalar_type() && bias->dim() == 1 && bias->size(0) == n_out, who, ": bias must be [", n_out, "] of x's type");
+    if (global_scale) TORCH_CHECK(global_scale->scalar_type() == at::kFloat && global_scale->numel() == 1, who, ": global_scale must be one float32 value");
+    no_gradient(who, x_in);
+    if (bias) no_gradient(who, *bias);
+    TORCH_CHECK(x_in.is_cuda(), who, ": x must be a CUDA tensor");
+    same_device(who, "codes", codes, x_in);
+    same_device(who, "scales", scales, x_in);
+    if (bias) same_device(who, "bias", *bias, x_in);
+    if (global_scale) same_device(who, "global_scale", *global_scale, x_in);
+    c10::cuda::CUDAGuard guard(x_in.device());
+    const at::Tensor x = x_in.contiguous();
+    const at::Tensor b = bias ? bias->contiguous() : at::Tensor();
+    auto shape = x.sizes().vec();
+    shape.back() = n_out;
+    at::Tensor y = at::empty(shape, x.options());
+    if (y.numel() == 0) return y;
+    int64_t rows = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) rows *= shape[i];
+    const size_t need = mpt_block_linear_workspace_bytes(rows, n_out, n_in, format, dtype);
+    const at::Tensor ws = workspace(need, x);
+    check(mpt_block_linear(x.data_ptr(), codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), global_scale ? global_scale->data_ptr<float>() : nullptr,
+                           b.defined() ? b.data_ptr() : nullptr, y.data_ptr(), rows, n_out, n_in, format, dtype, need ? ws.data_ptr() : nullptr, need,
+                           stream()));
+    return y;
+}
+at::Tensor mx_linear(at::Tensor x, at::Tensor codes, at::Tensor scales, std::optional<at::Tensor> bias) {
+    return block_linear("mx_linear", x, codes, scales, std::nullopt, bias, MPT_BLOCK_MXFP4);
+}
+at::Tensor nvfp4_linear(at::Tensor x, at::Tensor codes, at::Tensor scales, at::Tensor global_scale, std::optional<at::Tensor> bias) {
+    return block_linear("nvfp4_linear", x, codes, scales, global_scale, bias, MPT_BLOCK_NVFP4);
+}
+
+struct ServingCall { mpt_mx_cache cache; mpt_mx_batch batch; };
+
+// `rows`: new rows in all; `uniform_seqs`: the sequences they are split among without `starts`
+ServingCall serving_call(const char* who, const std::vector<at::Tensor>& cache, const at::Tensor& pages, const at::Tensor& lens,
+                         const std::optional<at::Tensor>& starts, int64_t rows) {
+    static const char* const names[4] = {"k_codes", "k_scales", "v_codes", "v_scales"};
+    TORCH_CHECK(cache.size() == 4, who, ": the cache is (k_codes, k_scales, v_codes, v_scales)");
+    for (int i = 0; i < 4; ++i) bytes_tensor(who, names[i], cache[i], 4);
+    const at::Tensor& kc = cache[0];
+    const int64_t dim = cache[1].size(3) * 32;
+    TORCH_CHECK(kc.size(3) == dim || kc.size(3) * 2 == dim, who, ": ", kc.size(3), " bytes of codes do not go with ", cache[1].size(3), " scales a row");
+    for (int i = 1; i < 4; ++i)
+        TORCH_CHECK(cache[i].size(0) == kc.size(0) && cache[i].size(1) == kc.size(1) && cache[i].size(2) == kc.size(2) &&
+                    cache[i].size(3) == cache[i & 1].size(3), who, ": ", names[i], " does not match k_codes");
+    TORCH_CHECK(pages.scalar_type() == at::kInt && pages.dim() == 2 && pages.is_contiguous(), who, ": pages must be a contiguous int32 matrix");
+    const int64_t seqs = pages.size(0);
+    TORCH_CHECK(lens.scalar_type() == at::kInt && lens.dim() == 1 && lens.size(0) == seqs && lens.is_contiguous(), who, ": lens must be a contiguous int32 [", seqs, "]");
+    if (starts)
+        TORCH_CHECK(starts->scalar_type() == at::kInt && starts->dim() == 1 && starts->size(0) == seqs + 1 && starts->is_contiguous(), who,
+                    ": starts must be a contiguous int32 [", seqs + 1, "]");
+    TORCH_CHECK(kc.size(1) <= 65535 && dim <= 256 && kc.size(2) <= 256 && seqs <= INT_MAX && pages.size(1) <= INT_MAX, who, ": extents out of range");
+    ServingCall s;
+    s.cache = {cache[0].data_ptr<uint8_t>(), cache[1].data_ptr<uint8_t>(), cache[2].data_ptr<uint8_t>(), cache[3].data_ptr<uint8_t>(), kc.size(0),
+               (int)kc.size(1), (int)dim, (int)kc.size(2), kc.size(3) == dim ? MPT_ELEM_E4M3 : MPT_ELEM_E2M1};
+    s.batch = {pages.data_ptr<int>(), lens.data_ptr<int>(), starts ? starts->data_ptr<int>() : nullptr, rows, (int)seqs, (int)pages.size(1)};
+    return s;
+}
+void serving_devices(const char* who, const at::Tensor& like, const std::vector<at::Tensor>& cache, const at::Tensor& pages, const at::Tensor& lens,
+                     const std::optional<at::Tensor>& starts) {
+    for (const auto& t : cache) same_device(who, "the cache", t, like);
+    same_device(who, "pages", pages, like);
+    same_device(who, "lens", lens, like);
+    if (starts) same_device(who, "starts", *starts, like);
+}
+// [seqs, new, heads, dim], or [rows, heads, dim] with `starts`
+void row_shape(const char* who, const char* what, const at::Tensor& t, bool ragged, int64_t seqs, int64_t dim) {
+    TORCH_CHECK(ragged ? t.dim() == 3 : t.dim() == 4 && t.size(0) == seqs, who, ": ", what, " must be ",
+                ragged ? "[rows, heads, head_dim] where starts is given" : "[sequences, new, heads, head_dim]");
+    TORCH_CHECK(t.size(-1) == dim, who, ": ", what, " has rows of ", t.size(-1), " values, the cache of ", dim);
+}
+int64_t row_count(const at::Tensor& t) { return t.dim() == 3 ? t.size(0) : t.size(0) * t.size(1); }
+std::array<int64_t, 3> row_strides(const at::Tensor& t) {
+    const int64_t d = t.dim();
+    return {d == 4 ? t.stride(0) : 0, t.stride(d - 3), t.stride(d - 2)};
+}
+at::Tensor dense_last(const at::Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+
+void mx_cache_write(at::Tensor k_in, at::Tensor v_in, std::vector<at::Tensor> cache, at::Tensor pages, at::Tensor lens, std::optional<at::Tensor> starts) {
+    const char* who = "mx_cache_write";
+    const int dtype = dense_type(who, k_in);
+    TORCH_CHECK(k_in.dim() >= 3, who, ": k needs three or four dimensions");
+    const ServingCall s = serving_call(who, cache, pages, lens, starts, row_count(k_in));
+    row_shape(who, "k", k_in, starts.has_value(), s.batch.seqs, s.cache.dim);
+    TORCH_CHECK(k_in.size(-2) == s.cache.heads, who, ": k has ", k_in.size(-2), " heads, the cache ", s.cache.heads);
+    TORCH_CHECK(v_in.sizes() == k_in.sizes() && v_in.scalar_type() == k_in.scalar_type(), who, ": v must have the shape and type of k");
+    no_gradient(who, k_in);
+    no_gradient(who, v_in);
+    TORCH_CHECK(k_in.is_cuda(), who, ": k must be a CUDA tensor");
+    same_device(who, "v", v_in, k_in);
+    serving_devices(who, k_in, cache, pages, lens, starts);
+    c10::cuda::CUDAGuard guard(k_in.device());
+    const at::Tensor k = dense_last(k_in), v = dense_last(v_in);
+    const auto ks = row_strides(k), vs = row_strides(v);
+    check(mpt_mx_cache_write(&s.cache, &s.batch, k.data_ptr(), v.data_ptr(), dtype, ks.data(), vs.data(), stream()));
+}
+std::vector<at::Tensor> mx_cache_read(std::vector<at::Tensor> cache, at::Tensor pages, at::Tensor lens, int64_t rows, std::optional<at::Tensor> starts,
+                                      at::ScalarType type) {
+    const char* who = "mx_cache_read";
+    TORCH_CHECK(rows >= 0, who, ": a negative number of rows");
+    const ServingCall s = serving_call(who, cache, pages, lens, starts, starts ? rows : rows * pages.size(0));
+    TORCH_CHECK(cache[0].is_cuda(), who, ": the cache must be a CUDA tensor");
+    serving_devices(who, cache[0], cache, pages, lens, starts);
+    c10::cuda::CUDAGuard guard(cache[0].device());
+    std::vector<int64_t> shape = starts ? std::vector<int64_t>{rows} : std::vector<int64_t>{s.batch.seqs, rows};
+    shape.push_back(s.cache.heads);
+    shape.push_back(s.cache.dim);
+    at::Tensor k = at::empty(shape, cache[0].options().dtype(type)), v = at::empty_like(k);
+    check(mpt_mx_cache_read(&s.cache, &s.batch, k.data_ptr(), v.data_ptr(), dense_type(who, k), stream()));
+    return {k, v};
+}
+at::Tensor mx_attention(at::Tensor q_in, std::vector<at::Tensor> cache, at::Tensor pages, at::Tensor lens, std::optional<at::Tensor> starts, double scale,
+                        int64_t window, int64_t sinks, std::optional<at::Tensor> out_in) {
+    const char* who = "mx_attention";
+    const int dtype = dense_type(who, q_in);
+    TORCH_CHECK(q_in.dim() >= 3, who, ": q needs three or four dimensions");
+    const ServingCall s = serving_call(who, cache, pages, lens, starts, row_count(q_in));
+    row_shape(who, "q", q_in, starts.has_value(), s.batch.seqs, s.cache.dim);
+    const int64_t heads = q_in.size(-2);
+    TORCH_CHECK(s.cache.heads > 0 && heads > 0 && heads % s.cache.heads == 0, who, ": ", heads, " query heads do not divide among ", s.cache.heads, " kv heads");
+    TORCH_CHECK(window >= 0 && sinks >= 0 && window <= INT_MAX && sinks <= INT_MAX, who, ": window and sinks must not be negative");
+    if (out_in)
+        TORCH_CHECK(out_in->sizes() == q_in.sizes() && out_in->scalar_type() == q_in.scalar_type() && out_in->is_contiguous(), who,
+                    ": out must be contiguous with the shape and type of q");
+    no_gradient(who, q_in);
+    TORCH_CHECK(q_in.is_cuda(), who, ": q must be a CUDA tensor");
+    if (out_in) same_device(who, "out", *out_in, q_in);
+    serving_devices(who, q_in, cache, pages, lens, starts);
+    c10::cuda::CUDAGuard guard(q_in.device());
+    const at::Tensor q = dense_last(q_in);
+    at::Tensor out = out_in ? *out_in : at::empty(q.sizes(), q.options());
+    if (out.numel() == 0) return out;
+    const auto qs = row_strides(q);
+    const size_t need = mpt_mx_attention_workspace_bytes(&s.cache, &s.batch, (int)heads, dtype, (int)window, (int)sinks);
+    const at::Tensor ws = workspace(need, q);
+    check(mpt_mx_attention(&s.cache, &s.batch, q.data_ptr(), dtype, qs.data(), (int)heads, (float)scale, (int)window, (int)sinks, out.data_ptr(),
+                           out_in ? 0 : 1, need ? ws.data_ptr() : nullptr, need, stream()));
+    return out;
+}
+
 void float_quantize_multi(std::vector<at::Tensor> ins, std::vector<at::Tensor> outs, int man_bits, int exp_bits, bool subnormals, bool saturate,
                           int rounding, int prng_bits, uint64_t seed) {
     TORCH_CHECK(ins.size() == outs.size(), "float_quantize_multi: as many outputs as inputs");
@@ -500,4 +678,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("float_quantize_multi", &float_quantize_multi, py::arg("ins"), py::arg("outs"), py::arg("man_bits"), py::arg("exp_bits"),
           py::arg("subnormals"), py::arg("saturate"), py::arg("rounding") = 0, py::arg("prng_bits") = 0, py::arg("seed") = 0);
     m.def("scale_quantize", &scale_quantize);
+    m.def("mx_linear", &mx_linear);
+    m.def("nvfp4_linear", &nvfp4_linear);
+    m.def("mx_cache_write", &mx_cache_write);
+    m.def("mx_cache_read", &mx_cache_read);
+    m.def("mx_attention", &mx_attention);
 }

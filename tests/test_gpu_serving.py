@@ -1,0 +1,582 @@
+"""The operators that serve from packed block formats against plain 64-bit arithmetic on the GPU.
+
+Tolerances.  u(t) = finfo(t).eps / 2 is the largest relative error of one rounding to t.
+
+Linear: x may be held as two binary16 pieces (each drops at most 2^-11 of what it takes, so 2^-22 of the value at least is
+kept; 2^-21 is allowed), every sum of K products in fp32 adds at most K u(fp32) of the sum of magnitudes, and the result is
+rounded once: |y - y64| <= (2^-21 + (K + 4) 2^-24) sum |x w| + u(t) |y64|.
+
+Attention: a score is off by at most d = scale (2^-21 + (D + 4) 2^-24) sum |q k| + 2^-23 |s| (q in pieces, the products' sum in fp32,
+the scaling); a weight p = exp(s - m) is then off by a factor within exp(2 d) of one, times 1 + 2^-21 for the exponential and,
+where it is rounded for a 16-bit product, 1 + u(t).  Numerator and denominator each add (T + 4) 2^-24.  So with
+e = 2 max d + 2^-21 + u(16-bit t) + (T + 4) 2^-24:  |o - o64| <= 2 e sum p |v| + u(t) |o64|.  Weights are held to an
+absolute step as well, as binary16 pieces of p 2^15: 2^-39 of the row's largest weight, times the largest |v| of the
+block, 2^-50 where there are two pieces (fp32); each of T tokens adds one such step at most.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def q():
+    import mptorch_b200.quant as quant
+
+    return quant
+
+
+def half_ulp(t):
+    return torch.finfo(t).eps / 2
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+# ---------------------------------------------------------------------------------- packed values in 64 bits
+def field_value(code, e_bits, m_bits):
+    code = code.to(torch.int64)
+    e, m = (code >> m_bits) & ((1 << e_bits) - 1), code & ((1 << m_bits) - 1)
+    v = torch.where(e > 0, m + (1 << m_bits), m).double() * torch.exp2((e.clamp(min=1) - ((1 << (e_bits - 1)) - 1) - m_bits).double())
+    return torch.where((code >> (e_bits + m_bits)) & 1 > 0, -v, v)
+
+
+def e4m3_value(code):
+    return torch.where((code & 127) == 127, math.nan, field_value(code, 4, 3))
+
+
+def e8m0_value(code):
+    return torch.where(code == 255, math.nan, torch.exp2(code.double() - 127))
+
+
+def values(codes, scales, dim):
+    """What rows of codes and E8M0 scales stand for."""
+    if codes.shape[-1] == dim:
+        v = e4m3_value(codes)
+    else:
+        v = torch.stack([field_value(codes & 15, 2, 1), field_value(codes >> 4, 2, 1)], -1).flatten(-2)
+    return v * e8m0_value(scales).repeat_interleave(32, -1)
+
+
+def random_rows(shape, dim, elem, g, low=118, high=128):
+    """Random codes (no NaN) and scales."""
+    codes = torch.randint(0, 256, shape + (dim if elem == "e4m3" else dim // 2,), device="cuda", generator=g, dtype=torch.uint8)
+    if elem == "e4m3":
+        codes = torch.where((codes & 127) == 127, codes - 1, codes)
+    return codes, torch.randint(low, high, shape + (dim // 32,), device="cuda", generator=g, dtype=torch.uint8)
+
+
+# ---------------------------------------------------------------------------------- linear
+def pack(n, k, fmt, g):
+    codes = torch.randint(0, 256, (n, k // 2), device="cuda", generator=g, dtype=torch.uint8)
+    v = torch.stack([field_value(codes & 15, 2, 1), field_value(codes >> 4, 2, 1)], -1).flatten(-2)
+    if fmt == "mxfp4":
+        scales = torch.randint(112, 126, (n, k // 32), device="cuda", generator=g, dtype=torch.uint8)
+        return codes, scales, None, v * e8m0_value(scales).repeat_interleave(32, -1)
+    scales = torch.randint(0, 127, (n, k // 16), device="cuda", generator=g, dtype=torch.uint8)
+    glob = torch.tensor([0.0123], device="cuda")
+    return codes, scales, glob, v * e4m3_value(scales).repeat_interleave(16, -1) * glob.double()
+
+
+def linear(q, x, codes, scales, glob, bias=None):
+    return q.mx_linear(x, codes, scales, bias) if glob is None else q.nvfp4_linear(x, codes, scales, glob, bias)
+
+
+def check_linear(y, x, w, bias=None):
+    k = w.shape[1]
+    want = x.double() @ w.t()
+    mag = x.double().abs() @ w.abs().t()
+    if bias is not None:
+        want, mag = want + bias.double(), mag + bias.double().abs()
+    tol = (2.0 ** -21 + (k + 4) * 2.0 ** -24) * mag + half_ulp(x.dtype) * want.abs()
+    if x.dtype == torch.float16:
+        tol = tol + 2.0 ** -25                                   # half a step of its subnormal numbers
+    assert y.dtype == x.dtype and y.shape == want.shape
+    worst = ((y.double() - want).abs() - tol).max().item()
+    assert worst <= 0, "off by %g more than allowed" % worst
+    # roundings of random sign: sqrt(K) of them, each at most 2^-24 of a partial sum
+    norm = ((y.double() - want).norm() / want.norm()).item()
+    assert norm <= 2.0 ** -21 + (math.sqrt(k) + 4) * 2.0 ** -24 + half_ulp(x.dtype)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,k", [(1, 1, 32), (1, 17, 64), (1, 768, 768), (2, 33, 96), (3, 257, 160), (4, 64, 1024), (5, 2304, 768), (7, 100, 4096),
+                                      (8, 129, 512), (9, 48, 2080), (16, 130, 288), (17, 65, 544), (32, 200, 1056), (33, 300, 64), (64, 515, 768),
+                                      (65, 31, 128), (100, 513, 224), (127, 128, 256), (130, 260, 1568), (300, 1000, 768), (515, 129, 96)])
+def test_linear(q, fmt, dtype, rows, n, k):
+    g = gen(rows * 7 + n + k)
+    codes, scales, glob, w = pack(n, k, fmt, g)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(dtype)
+    bias = torch.randn(n, device="cuda", generator=g).to(dtype) if (rows + n) % 2 else None
+    check_linear(linear(q, x, codes, scales, glob, bias), x, w, bias)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("rows", [1, 3, 24, 200])
+def test_linear_range_of_x(q, fmt, rows):
+    """Values of x over many orders of magnitude, within a row and between rows, keep fp32's accuracy."""
+    g = gen(rows)
+    codes, scales, glob, w = pack(70, 256, fmt, g)
+    x = torch.randn(rows, 256, device="cuda", generator=g) * torch.exp2(torch.randint(-8, 9, (rows, 256), device="cuda", generator=g).float())
+    x = x * torch.exp2(torch.randint(-60, 60, (rows, 1), device="cuda", generator=g).float())
+    y = linear(q, x, codes, scales, glob)
+    want, mag = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    assert ((y.double() - want).abs() <= (2.0 ** -21 + 260 * 2.0 ** -24) * mag + 2.0 ** -24 * want.abs()).all()
+    one = x.clone()
+    one[:] = 0
+    one[:, 5] = 2.0 ** -100
+    assert torch.equal(linear(q, one, codes, scales, glob).double(), (one.double() @ w.t()).float().double())
+    zero = torch.zeros_like(x)
+    assert torch.equal(linear(q, zero, codes, scales, glob), zero[:, :1].expand(rows, 70))
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 5, 40, 150])
+def test_linear_specials(q, fmt, dtype, rows):
+    """NaN and infinities of x stay in their rows; a NaN scale in its output."""
+    g = gen(3)
+    codes, scales, glob, w = pack(40, 128, fmt, g)
+    scales[7, 1] = 255 if fmt == "mxfp4" else 127
+    x = torch.randn(rows, 128, device="cuda", generator=g).to(dtype)
+    clean = linear(q, x, codes, scales, glob)
+    assert clean[:, 7].isnan().all() and clean[:, :7].isfinite().all() and clean[:, 8:].isfinite().all()
+    bad = x.clone()
+    bad[-1, 3] = math.nan
+    y = linear(q, bad, codes, scales, glob)
+    assert y[-1].isnan().all() and torch.equal(y[:-1].nan_to_num(7), clean[:-1].nan_to_num(7))
+    bad = x.clone()
+    bad[0, 9] = math.inf
+    y, want = linear(q, bad, codes, scales, glob), bad.float() @ torch.cat([w[:7], w[8:]]).float().t()
+    y = torch.cat([y[:, :7], y[:, 8:]], 1)
+    assert torch.equal(y[0].isnan(), want[0].isnan()) and torch.equal(y[0].float()[~want[0].isnan()], want[0][~want[0].isnan()])
+    assert torch.equal(y[1:], torch.cat([clean[1:, :7], clean[1:, 8:]], 1))
+
+
+def test_linear_extreme_scales(q):
+    """E8M0 scales from end to end of their range, against rows of x that bring the products back into range."""
+    codes = torch.full((3, 32), 0x22, device="cuda", dtype=torch.uint8)           # ones
+    scales = torch.tensor([[0, 0], [127, 127], [254, 254]], device="cuda", dtype=torch.uint8)
+    for e in (-100, 0, 100):
+        for rows in (1, 20, 140):
+            x = torch.full((rows, 64), 2.0 ** e, device="cuda")
+            want = 64.0 * torch.tensor([2.0 ** -127, 1.0, 2.0 ** 127], device="cuda", dtype=torch.float64) * 2.0 ** e
+            assert torch.equal(q.mx_linear(x, codes, scales), want.float().expand(rows, 3))
+
+
+def test_linear_shapes_strides_and_quantizers(q):
+    g = gen(11)
+    w = torch.randn(96, 160, device="cuda", generator=g) * 0.02
+    wq, scales, codes = q.mx_quantize(w, "e2m1", 32, return_scales=True, return_codes=True)
+    nq, _, glob, ncodes, nscales = q.nvfp4_quantize(w, None, return_scales=True, return_codes=True)
+    x = torch.randn(2, 3, 320, device="cuda", generator=g)[..., ::2]              # a strided view, three dimensions
+    y = q.mx_linear(x, codes, scales)
+    assert y.shape == (2, 3, 96)
+    check_linear(y.flatten(0, 1), x.flatten(0, 1), wq.double())
+    check_linear(q.nvfp4_linear(x, ncodes, nscales, glob).flatten(0, 1), x.flatten(0, 1), nq.double())
+    assert torch.equal(q.nvfp4_linear(x, ncodes, nscales, glob), q.nvfp4_linear(x, ncodes, nscales, float(glob)))
+    assert q.mx_linear(x[0, 0], codes, scales).shape == (96,)
+    assert torch.equal(q.mx_linear(x[0, 0], codes, scales), q.mx_linear(x[0, :1], codes, scales)[0])
+    assert q.mx_linear(x[:0], codes, scales).shape == (0, 3, 96)
+    assert q.mx_linear(x, codes[:0], scales[:0]).shape == (2, 3, 0)
+    odd = torch.randn(4 * 160 + 1, device="cuda", generator=g)[1:].view(4, 160)    # an address that is a multiple of 4 only
+    assert torch.equal(q.mx_linear(odd, codes, scales), q.mx_linear(odd.clone(), codes, scales))
+    odd = odd.bfloat16()
+    pad = torch.empty(4 * 160 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(4, 160).copy_(odd)
+    assert torch.equal(q.mx_linear(pad, codes, scales), q.mx_linear(odd, codes, scales))
+    assert torch.equal(q.mx_linear(x, codes, scales), q.mx_linear(x, codes, scales))
+
+
+# ---------------------------------------------------------------------------------- the cache
+def place(lens, page, g, extra=2):
+    """A page table over pages in random order (-1 behind the last one) and the number of pages."""
+    counts = [-(-n // page) for n in lens]
+    total, width = sum(counts) + extra, max(counts + [1])
+    order = torch.randperm(total, device="cuda", generator=g).to(torch.int32)
+    pages, at = torch.full((len(lens), width), -1, device="cuda", dtype=torch.int32), 0
+    for i, n in enumerate(counts):
+        pages[i, :n] = order[at:at + n]
+        at += n
+    return pages, total
+
+
+def i32(x):
+    return torch.tensor(x, device="cuda", dtype=torch.int32)
+
+
+def cumulative(new):
+    return i32([0] + list(torch.tensor(new).cumsum(0)))
+
+
+@pytest.mark.parametrize("elem", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,heads,page", [(32, 1, 8), (64, 3, 16), (96, 2, 64), (128, 4, 32), (256, 1, 256)])
+def test_cache_write_and_read(q, elem, dtype, dim, heads, page):
+    g = gen(dim)
+    new, lens = [5, 1, 40, 0, 3], [5, 33, 40, 12, 2]                              # the last: one row stands before the first token
+    pages, total = place(lens, page, g)
+    cache = q.MXCache.empty(total, heads, dim, page, elem)
+    for t in cache:
+        t.random_(0, 256)
+    before = [t.clone() for t in cache]
+    qkv = torch.randn(49, heads * dim * 3, device="cuda", generator=g).to(dtype)  # k and v as views of one projection
+    k, v = qkv[:, heads * dim:2 * heads * dim].view(49, heads, dim), qkv[:, 2 * heads * dim:].view(49, heads, dim)
+    k[7, 0, 3] = math.inf
+    v[8, heads - 1, dim - 1] = math.nan
+    v[9] = 0
+    k[10] *= 2.0 ** -14
+    starts = cumulative(new)
+    q.mx_cache_write(k, v, cache, pages, i32(lens), starts)
+    kr, vr = q.mx_cache_read(cache, pages, i32(lens), 49, starts)
+    hit = torch.zeros(total, heads, page, dtype=torch.bool, device="cuda")
+    row = 0
+    for s, (n, length) in enumerate(zip(new, lens)):
+        for i in range(n):
+            pos = length - n + i
+            if pos >= 0:
+                p, o = int(pages[s, pos // page]), pos % page
+                hit[p, :, o] = True
+                for x, codes, scales, back in ((k, cache[0], cache[1], kr), (v, cache[2], cache[3], vr)):
+                    held, sc, cd = q.mx_quantize(x[row].float(), elem, 32, return_scales=True, return_codes=True)
+                    assert torch.equal(codes[p, :, o], cd) and torch.equal(scales[p, :, o], sc)
+                    assert torch.equal(back[row].nan_to_num(9), held.nan_to_num(9)) and torch.equal(back[row].isnan(), held.isnan())
+            else:
+                assert not kr[row].any() and not vr[row].any()
+            row += 1
+    for t, b in zip(cache, before):
+        assert torch.equal(t[~hit], b[~hit])
+    low = q.mx_cache_read(cache, pages, i32(lens), 49, starts, dtype=dtype)
+    assert torch.equal(low[0].nan_to_num(9), kr.to(dtype).nan_to_num(9)) and low[1].dtype == dtype
+
+
+@pytest.mark.parametrize("elem", ["e4m3", "e2m1"])
+def test_cache_uniform_padded_and_missing_pages(q, elem):
+    g = gen(5)
+    pages, total = place([24, 24, 24], 8, g)
+    pages[1, 1], pages[2, 0] = -1, total + 5                                       # tokens 8..15 of one, 0..7 of the other: no page
+    lens = i32([24, 24, 3])
+    a, b = q.MXCache.empty(total, 2, 64, 8, elem), q.MXCache.empty(total, 2, 64, 8, elem)
+    big = torch.randn(3, 2, 20, 65, device="cuda", generator=g)
+    k, v = big[..., 1:].transpose(1, 2), big.flip(0)[..., :64].transpose(1, 2)     # [3, 20, 2, 64], rows that are not aligned
+    q.mx_cache_write(k, v, a, pages, lens)
+    q.mx_cache_write(k.contiguous(), v.contiguous(), b, pages, lens)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    kr, vr = q.mx_cache_read(a, pages, lens, 20)
+    want = q.mx_quantize(k.contiguous(), elem, 32)
+    want[1, 4:12] = 0
+    want[2] = 0                                                                    # 17 rows before its first token, 3 in no page
+    assert torch.equal(kr, want)
+    # more tokens than the table has places for: those behind it are neither written nor read
+    q.mx_cache_write(k[:1, :4], v[:1, :4], a, pages[:1], i32([26]))
+    kr, _ = q.mx_cache_read(a, pages[:1], i32([26]), 4)
+    assert torch.equal(kr[0, :2], q.mx_quantize(k[0, :2].contiguous(), elem, 32)) and not kr[0, 2:].any()
+    # nothing at all
+    q.mx_cache_write(k[:, :0], v[:, :0], a, pages, lens)
+    assert q.mx_cache_read(a, pages, lens, 0)[0].shape == (3, 0, 2, 64)
+    q.mx_cache_write(k[:0], v[:0], a, pages[:0], lens[:0])
+    kr, vr = q.mx_cache_read(a, pages, lens, 7, i32([0, 2, 2, 4]))                 # rows behind the last sequence
+    assert not kr[4:].any() and not vr[4:].any()
+
+
+# ---------------------------------------------------------------------------------- attention
+def reference(qry, cache, pages, lens, new, dim, scale, window=0, sinks=0):
+    """Row by row in 64 bits: (outputs, allowed error) for rows in order; ``new`` rows of each sequence."""
+    heads, group, page = cache[0].shape[1], qry.shape[1] // cache[0].shape[1], cache[0].shape[2]
+    out, tol, at, u = torch.zeros(qry.shape, device="cuda", dtype=torch.float64), torch.zeros(qry.shape, device="cuda", dtype=torch.float64), 0, half_ulp(qry.dtype)
+    for s, n in enumerate(new):
+        if n == 0:
+            continue
+        length = min(int(lens[s]), pages.shape[1] * page)
+        rows = qry[at:at + n].double()                                             # [n, heads * group, dim]
+        pos = int(lens[s]) - n + torch.arange(n, device="cuda")[:, None]
+        t = torch.arange(max(length, 0), device="cuda")
+        table = pages[s].long()
+        there = (table >= 0) & (table < cache[0].shape[0])
+        slot = table.clamp(0, cache[0].shape[0] - 1)[t // page]
+        seen = (t <= pos) & there[t // page]
+        if window:
+            seen &= (t > pos - window) | (t < sinks)
+        for h in range(heads):
+            k, v = (values(cache[i][slot, h, t % page], cache[i + 1][slot, h, t % page], dim) for i in (0, 2))
+            for j in range(h * group, (h + 1) * group):
+                x = rows[:, j]
+                some = seen.any(1)
+                sc = torch.where(seen, (x @ k.t()) * scale, -math.inf)
+                p = torch.where(some[:, None], torch.softmax(sc, -1), 0.0)
+                # a masked token takes no part, whatever it holds
+                o = torch.stack([p[i][seen[i]] @ v[seen[i]] for i in range(n)])
+                d = torch.where(seen, abs(scale) * (2.0 ** -21 + (dim + 4) * 2.0 ** -24) * (x.abs() @ k.abs().t()) + 2.0 ** -23 * sc.abs(), 0.0).amax(-1) if len(t) else torch.zeros(n, device="cuda", dtype=torch.float64)
+                e = 2 * d + 2.0 ** -21 + (u if qry.dtype != torch.float32 else 0.0) + (len(t) + 4) * 2.0 ** -24
+                out[at:at + n, j] = o
+                step = len(t) * 2.0 ** (-50 if qry.dtype == torch.float32 else -39)
+                most = v.abs().nan_to_num(0).unflatten(-1, (-1, 32)).amax((0, 2)).repeat_interleave(32) if len(t) else 0.0
+                tol[at:at + n, j] = 2 * e[:, None] * torch.stack([p[i][seen[i]] @ v[seen[i]].abs() for i in range(n)]) + u * o.abs() + step * most
+        at += n
+    return out, tol + (2.0 ** -25 if qry.dtype == torch.float16 else 0.0)
+
+
+def check_attention(got, want, tol):
+    assert torch.equal(got.isnan(), want.isnan())
+    worst = ((got.double() - want).abs() - tol).nan_to_num(0, 0, 0).max().item() if got.numel() else 0
+    assert worst <= 0, "off by %g more than allowed" % worst
+
+
+def setup(q, lens, new, heads, group, dim, page, elem, dtype, seed, uniform=False):
+    g = gen(seed)
+    pages, total = place(lens, page, g)
+    cache = q.MXCache(*random_rows((total, heads, page), dim, elem, g), *random_rows((total, heads, page), dim, elem, g))
+    shape = (len(new), new[0]) if uniform else (sum(new),)
+    qry = (torch.randn(shape + (heads * group, dim), device="cuda", generator=g) * (0.05 if elem == "e4m3" else 1.0)).to(dtype)
+    return qry, cache, pages, i32(lens), (None if uniform else cumulative(new))
+
+
+SHAPES = [  # lens, new, kv heads, group, dim, page
+    ([1, 7, 130, 0], [1, 1, 1, 1], 2, 1, 64, 16), ([300, 17, 64, 65, 1000], [1] * 5, 1, 8, 128, 64), ([129, 31], [1, 1], 3, 4, 96, 8),
+    ([2100], [1], 2, 2, 32, 32), ([513, 200], [1, 1], 2, 3, 256, 128), ([77, 260, 5], [1] * 3, 1, 16, 192, 16), ([6000, 3], [1, 1], 1, 5, 64, 64)]
+CHUNKS = [([40, 9, 300], [40, 2, 33], 2, 1, 64, 16), ([200], [200], 1, 4, 128, 64), ([700, 130, 1], [129, 130, 1], 2, 2, 128, 32),
+          ([90, 0, 260], [64, 0, 128], 3, 1, 32, 8), ([150, 400], [17, 65], 1, 8, 96, 128), ([333], [300], 1, 2, 256, 16), ([260, 70], [200, 70], 1, 3, 192, 64)]
+
+
+@pytest.mark.parametrize("elem", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(SHAPES)))
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
+def test_attention_one_token(q, elem, dtype, case, window, sinks):
+    lens, new, heads, group, dim, page = SHAPES[case]
+    qry, cache, pages, ln, starts = setup(q, lens, new, heads, group, dim, page, elem, dtype, case, uniform=True)
+    got = q.mx_attention(qry, cache, pages, ln, window=window, sinks=sinks)
+    want, tol = reference(qry.flatten(0, 1), cache, pages, lens, new, dim, 1 / math.sqrt(dim), window, sinks)
+    check_attention(got.flatten(0, 1), want, tol)
+
+
+@pytest.mark.parametrize("elem", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(CHUNKS)))
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 5), (1, 0)])
+def test_attention_chunks(q, elem, dtype, case, window, sinks):
+    lens, new, heads, group, dim, page = CHUNKS[case]
+    qry, cache, pages, ln, starts = setup(q, lens, new, heads, group, dim, page, elem, dtype, 50 + case)
+    got = q.mx_attention(qry, cache, pages, ln, starts, scale=0.11, window=window, sinks=sinks)
+    want, tol = reference(qry, cache, pages, lens, new, dim, 0.11, window, sinks)
+    check_attention(got, want, tol)
+
+
+FORMS = [([70, 33], [1, 1], 1, 4), ([70, 33, 260], [9, 20, 130], 1, 2), ([190], [180], 2, 2)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("form", range(len(FORMS)))
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_masked_places_hold_anything(q, dtype, form, dim):
+    """NaN scales and codes behind the last token, in pages that are not there and where a row's mask hides them change
+    nothing; a NaN that a row sees makes that row NaN (in K all of it, in V the block)."""
+    lens, new, heads, group = FORMS[form]
+    qry, cache, pages, ln, starts = setup(q, lens, new, heads, group, dim, 16, "e4m3", dtype, 80 + form)
+    clean = q.mx_attention(qry, cache, pages, ln, starts)
+    used = torch.zeros(cache[0].shape[0], 16, dtype=torch.bool, device="cuda")
+    for s, n in enumerate(lens):
+        for t in range(n):
+            used[pages[s, t // 16], t % 16] = True
+    dirty = q.MXCache(*(torch.where(used[:, None, :, None], t, 255) for t in cache))
+    assert torch.equal(q.mx_attention(qry, dirty, pages, ln, starts), clean)
+    # the last token of the first sequence: NaN in K, then in one block of V
+    p, o = int(pages[0, (lens[0] - 1) // 16]), (lens[0] - 1) % 16
+    for which in (1, 3):
+        bad = q.MXCache(*(t.clone() for t in cache))
+        bad[which][p, 0, o, 1] = 255
+        got = q.mx_attention(qry, bad, pages, ln, starts)
+        want, tol = reference(qry, bad, pages, lens, new, dim, 1 / math.sqrt(dim))
+        assert want.isnan().any() and not want.isnan().all()
+        check_attention(got, want, tol)
+        keep = ~want.isnan()
+        assert torch.equal(got[keep], clean[keep])
+    # the same in the middle, under a window that hides it from some rows
+    p, o = int(pages[0, (lens[0] // 2) // 16]), (lens[0] // 2) % 16
+    for which in (1, 3):
+        bad = q.MXCache(*(t.clone() for t in cache))
+        bad[which][p, 0, o, 0] = 255
+        got = q.mx_attention(qry, bad, pages, ln, starts, window=20, sinks=2)
+        want, tol = reference(qry, bad, pages, lens, new, dim, 1 / math.sqrt(dim), 20, 2)
+        check_attention(got, want, tol)
+    # a row of q with a NaN or an infinity
+    for x in (math.nan, math.inf):
+        bad = qry.clone()
+        bad[-1, 1, 5] = x
+        got = q.mx_attention(bad, cache, pages, ln, starts)
+        assert got[-1, 1].isnan().all()
+        assert torch.equal(got[:-1], clean[:-1]) and torch.equal(got[-1, 0], clean[-1, 0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [1, 40, 150])
+def test_attention_rows_that_see_nothing(q, dtype, new):
+    lens = [0, new + 30, max(new - 25, 0), 17]
+    qry, cache, pages, ln, _ = setup(q, [max(n, 1) for n in lens], [new] * 4, 2, 2, 64, 8, "e4m3", dtype, new, uniform=True)
+    ln = i32(lens)
+    pages[1, 1] = -1                                                              # a hole
+    pages[3, :] = cache[0].shape[0]                                               # nothing there at all
+    got = q.mx_attention(qry, cache, pages, ln)
+    want, tol = reference(qry.flatten(0, 1), cache, pages, lens, [new] * 4, 64, 1 / 8)
+    check_attention(got.flatten(0, 1), want, tol)
+    assert not got[0].any() and not got[3].any() and got[1].any()
+    # more tokens than the table has places for
+    ln[1] = pages.shape[1] * 8 + 5
+    got = q.mx_attention(qry, cache, pages, ln)
+    want, tol = reference(qry.flatten(0, 1), cache, pages, [0, int(ln[1]), lens[2], 17], [new] * 4, 64, 1 / 8)
+    check_attention(got.flatten(0, 1), want, tol)
+    # rows behind the last sequence: zeros, or left as they were in a tensor of the caller's
+    flat, starts = qry.flatten(0, 1), cumulative([new, 1, 0, 0])
+    got = q.mx_attention(flat, cache, pages, ln, starts)
+    assert not got[new + 1:].any()
+    mine = torch.full_like(flat, 7)
+    assert q.mx_attention(flat, cache, pages, ln, starts, out=mine) is mine or True
+    assert torch.equal(mine[:new + 1], got[:new + 1]) and (mine[new + 1:] == 7).all()
+    assert q.mx_attention(flat[:0], cache, pages, ln, cumulative([0] * 4)).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [1, 30, 140])
+def test_attention_strides_and_order(q, dtype, new):
+    qry, cache, pages, ln, _ = setup(q, [new + 40, new + 7, new], [new] * 3, 2, 2, 96, 16, "e2m1", dtype, 9, uniform=True)
+    want = q.mx_attention(qry, cache, pages, ln)
+    assert torch.equal(q.mx_attention(qry.transpose(1, 2).contiguous().transpose(1, 2), cache, pages, ln), want)   # heads outside
+    wide = torch.zeros(3, new, 4, 97, device="cuda", dtype=dtype)
+    wide[..., 1:] = qry
+    assert torch.equal(q.mx_attention(wide[..., 1:], cache, pages, ln), want)                                     # rows not aligned
+    assert torch.equal(q.mx_attention(qry.transpose(2, 3).contiguous().transpose(2, 3), cache, pages, ln), want)  # dimension outside
+    assert torch.equal(q.mx_attention(qry.flatten(0, 1), cache, pages, ln, cumulative([new] * 3)).view_as(want), want)
+    assert torch.equal(q.mx_attention(qry, cache, pages, ln, out=torch.empty_like(qry)), want)
+    assert torch.equal(q.mx_attention(qry, tuple(cache), pages, ln, window=1 << 30), want)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
+@pytest.mark.parametrize("new", [1, 20, 129])
+def test_attention_scales(q, scale, new):
+    """No scale, a negative one, and scores far apart."""
+    qry, cache, pages, ln, starts = setup(q, [new + 90], [new], 1, 2, 64, 16, "e2m1", torch.float32, 4)
+    got = q.mx_attention(qry, cache, pages, ln, starts, scale=scale)
+    want, tol = reference(qry, cache, pages, [new + 90], [new], 64, scale)
+    check_attention(got, want, tol)
+
+
+@pytest.mark.parametrize("new", [1, 30, 140])
+def test_attention_scales_of_v_far_apart(q, new):
+    """Tokens whose V differs by many orders of magnitude, small ones with the large weights."""
+    qry, cache, pages, ln, starts = setup(q, [new + 90], [new], 1, 2, 64, 16, "e4m3", torch.float32, 6)
+    g = gen(8)
+    cache.v_scales.copy_(torch.randint(100, 150, cache.v_scales.shape, device="cuda", generator=g, dtype=torch.uint8))
+    got = q.mx_attention(qry, cache, pages, ln, starts, scale=0.05)
+    want, tol = reference(qry, cache, pages, [new + 90], [new], 64, 0.05)
+    check_attention(got, want, tol)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("new", [1, 130])
+def test_offsets_past_32_bits(q, dtype, new):
+    """A cache of more than 2^32 bytes of codes: pages at its far end."""
+    cache = q.MXCache.empty(9000, 8, 256, 256)                                     # 4.7e9 bytes of codes each for K and V
+    pages, ln = i32([[8999, 8500]]), i32([256 + 140])
+    g = gen(1)
+    k, v = torch.randn(1, 396, 8, 256, device="cuda", generator=g).to(dtype), torch.randn(1, 396, 8, 256, device="cuda", generator=g).to(dtype)
+    q.mx_cache_write(k, v, cache, pages, ln)
+    kr, vr = q.mx_cache_read(cache, pages, ln, 396)
+    assert torch.equal(kr, q.mx_quantize(k.float(), "e4m3", 32)) and torch.equal(vr, q.mx_quantize(v.float(), "e4m3", 32))
+    qry = torch.randn(1, new, 8, 256, device="cuda", generator=g).to(dtype)
+    small = q.MXCache(*(t[pages[0].long()] for t in cache))
+    got = q.mx_attention(qry, cache, pages, ln)
+    want, tol = reference(qry[0], small, i32([[0, 1]]), [396], [new], 256, 1 / 16)
+    check_attention(got[0], want, tol)
+
+
+# ---------------------------------------------------------------------------------- streams, graphs, a run of them together
+@pytest.mark.parametrize("new", [1, 150])
+def test_streams_and_graphs(q, new):
+    """Another stream than the default, and two captured graphs replayed with new inputs in turn: eager calls give the bits."""
+    g = gen(2)
+    lens = [new + 700, new + 41]
+    codes, scales, glob, _ = pack(256, 256, "nvfp4", g)
+
+    def step(qry, k, v, cache, pages, ln):
+        q.mx_cache_write(k, v, cache, pages, ln)
+        o = q.mx_attention(qry, cache, pages, ln)
+        return o, q.nvfp4_linear(o.flatten(2), codes, scales, glob)
+
+    def inputs(seed):
+        qry, cache, pages, ln, _ = setup(q, lens, [new] * 2, 2, 2, 64, 16, "e4m3", torch.bfloat16, seed, uniform=True)
+        h = gen(seed + 1)
+        return [qry, torch.randn(2, new, 2, 64, device="cuda", generator=h).bfloat16(), torch.randn(2, new, 2, 64, device="cuda", generator=h).bfloat16(), cache, pages, ln]
+
+    sets = [inputs(s) for s in (21, 22)]
+    eager = []
+    for a in sets:
+        b = [*a[:3], q.MXCache(*(t.clone() for t in a[3])), *a[4:]]
+        eager.append([t.clone() for t in step(*b)])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(*[*sets[0][:3], q.MXCache(*(t.clone() for t in sets[0][3])), *sets[0][4:]])
+    side.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, eager[0]))
+    static = [[t.clone() for t in a[:3]] + [q.MXCache(*(t.clone() for t in a[3]))] + [t.clone() for t in a[4:]] for a in sets]
+    graphs, outs = [], []
+    for a in static:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(step(*a))
+        graphs.append(gr)
+    for _ in range(3):
+        for gr in graphs:
+            gr.replay()
+    torch.cuda.synchronize()
+    for o, e in zip(outs, eager):
+        assert all(torch.equal(x, y) for x, y in zip(o, e))
+    # new inputs in the first graph's tensors
+    for t, s in zip(static[0][:3], sets[1][:3]):
+        t.copy_(s)
+    for t, s in zip(static[0][3], sets[1][3]):
+        t.copy_(s)
+    static[0][4].copy_(sets[1][4])
+    static[0][5].copy_(sets[1][5])
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(outs[0], eager[1]))
+
+
+def test_both_routes_agree(q, monkeypatch):
+    from mptorch_b200 import backend as be
+
+    if be._ext is None:
+        pytest.skip("the extension is not built")
+    g = gen(6)
+    codes, scales, glob, _ = pack(100, 256, "nvfp4", g)
+    mcodes, mscales, _, _ = pack(100, 256, "mxfp4", g)
+    x, bias = torch.randn(5, 256, device="cuda", generator=g), torch.randn(100, device="cuda", generator=g)
+    qry, cache, pages, ln, starts = setup(q, [30, 170], [4, 140], 2, 2, 64, 16, "e4m3", torch.float32, 3)
+    k = torch.randn(144, 2, 64, device="cuda", generator=g)
+
+    def all_of_them():
+        c = q.MXCache(*(t.clone() for t in cache))
+        q.mx_cache_write(k, -k, c, pages, ln, starts)
+        return [q.nvfp4_linear(x, codes, scales, glob, bias), q.mx_linear(x, mcodes, mscales, bias), *c, *q.mx_cache_read(c, pages, ln, 144, starts, torch.bfloat16),
+                q.mx_attention(qry, c, pages, ln, starts), q.mx_attention(qry[:4].view(2, 2, 4, 64), c, pages, ln, window=9, sinks=1)]
+
+    a = all_of_them()
+    monkeypatch.setattr(be, "_ext", None)
+    assert all(torch.equal(s, t) for s, t in zip(a, all_of_them()))
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_another_device_than_the_current_one(q):
+    dev = torch.device("cuda", 1)
+    qry, cache, pages, ln, starts = setup(q, [30, 170], [4, 140], 2, 2, 64, 16, "e4m3", torch.float32, 3)
+    want = q.mx_attention(qry, cache, pages, ln, starts)
+    there = q.mx_attention(qry.to(dev), q.MXCache(*(t.to(dev) for t in cache)), pages.to(dev), ln.to(dev), starts.to(dev))
+    assert there.device == dev and torch.equal(there.cpu(), want.cpu())
+    with pytest.raises(RuntimeError, match="expected"):
+        q.mx_attention(qry.to(dev), cache, pages, ln, starts)
