@@ -10,8 +10,11 @@ Attention: a score is off by at most d = scale (2^-21 + (D + 4) 2^-24) sum |q k|
 the scaling); a weight p = exp(s - m) is then off by a factor within exp(2 d) of one, times 1 + 2^-21 for the exponential and,
 where it is rounded for a 16-bit product, 1 + u(t).  Numerator and denominator each add (T + 4) 2^-24.  So with
 e = 2 max d + 2^-21 + u(16-bit t) + (T + 4) 2^-24:  |o - o64| <= 2 e sum p |v| + u(t) |o64|.  Weights are held to an
-absolute step as well, as binary16 pieces of p 2^15: 2^-39 of the row's largest weight, times the largest |v| of the
-block, 2^-50 where there are two pieces (fp32); each of T tokens adds one such step at most.
+absolute step as well.  They are binary16 values w = p 2^15, times the scale of V relative to the largest 2^E of a group of tokens:
+below 2^-14 binary16 has a step of 2^-24, so a rounding moves w 2^(e - E) by up to 2^-25, which is 2^-40 of the row's largest
+weight times 2^E, and two such roundings (of w and of the product) 2^-39, times the largest |v| of the block, for each of T tokens.
+Where p is held in two pieces the same holds: the scale of V multiplies each piece by itself, so that what the first one's
+rounding drops is not in the second.
 """
 import math
 
@@ -314,7 +317,7 @@ def reference(qry, cache, pages, lens, new, dim, scale, window=0, sinks=0):
                 d = torch.where(seen, abs(scale) * (2.0 ** -21 + (dim + 4) * 2.0 ** -24) * (x.abs() @ k.abs().t()) + 2.0 ** -23 * sc.abs(), 0.0).amax(-1) if len(t) else torch.zeros(n, device="cuda", dtype=torch.float64)
                 e = 2 * d + 2.0 ** -21 + (u if qry.dtype != torch.float32 else 0.0) + (len(t) + 4) * 2.0 ** -24
                 out[at:at + n, j] = o
-                step = len(t) * 2.0 ** (-50 if qry.dtype == torch.float32 else -39)
+                step = len(t) * 2.0 ** -39
                 most = v.abs().nan_to_num(0).unflatten(-1, (-1, 32)).amax((0, 2)).repeat_interleave(32) if len(t) else 0.0
                 tol[at:at + n, j] = 2 * e[:, None] * torch.stack([p[i][seen[i]] @ v[seen[i]].abs() for i in range(n)]) + u * o.abs() + step * most
         at += n
