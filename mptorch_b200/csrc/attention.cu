@@ -8,19 +8,25 @@
 //   s[t, r] = sum_b 2^e[t,b] sum_{d in b} c_k[t,d] q[r,d]        o[d, r] = sum_t c_v[t,d] (2^e[t,b(d)] p[t,r])
 // Codes are exact in binary16, so both inner sums run on m16n8k16 tensor-core products of codes as they are (one conversion per two
 // elements) with fp32 sums: K as the 16 x 16 operand and q^T as the 16 x 8 one, then V^T and p^T.  The scale of K multiplies a
-// block's partial sums; the scale of V multiplies p, relative to the largest of 32 tokens, and what was taken out multiplies the
-// partial sums.  q is scaled by a power of two to a largest value in [2^14, 2^15) and held as binary16: bfloat16 and float16 in
+// block's partial sums; the scale of V multiplies p, relative to the block's largest so far (which moves like the running maximum
+// of the softmax), and that is put back at the end.  q is scaled by a power of two to a largest value in [2^14, 2^15) and held as binary16: bfloat16 and float16 in
 // one piece, exact unless a value is 2^-29 of the row's largest or less; float32 in two columns, the second 2^11 times what the
 // first leaves (22 bits).  p 2^15 is rounded to binary16 (11 bits) in one piece, for float32 in two.  The running maximum is
 // moved only when a tile exceeds it.
 //
 // Measured figures stand at the launch rule below.
+#include <atomic>
+
 #include "attention.cuh"
 
 namespace mpt {
 namespace {
 
-constexpr int kWarps = 4, kTok = 32;
+#ifndef MPT_ATT_WARPS
+#define MPT_ATT_WARPS 4
+#define MPT_ATT_LEAST 8
+#endif
+constexpr int kWarps = MPT_ATT_WARPS, kTok = 32, kLeast = MPT_ATT_LEAST;
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(live ? 16 : 0));
@@ -31,6 +37,10 @@ __device__ __forceinline__ void cp8(uint32_t dst, const void* src, bool live) {
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -44,58 +54,130 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t half_power(int down) {   // 2^-down as binary16, zero below 2^-24
     return down < 15 ? (uint32_t)(15 - down) << 10 : (down < 25 ? 1u << (24 - down) : 0u);
 }
-__device__ __forceinline__ bool has_ff(uint32_t w) {     // some byte of w is 0xFF
-    const uint32_t x = ~w;
-    return ((x - 0x01010101u) & ~x & 0x80808080u) != 0u;
-}
 
 // Bytes of a token in shared memory.  A warp's reads meet no bank twice when eight K rows of four words (E2M1), four K rows of
 // four double words (E4M3) and four V rows two apart fall into different quarters of the banks.
 struct Layout {
-    int k_pitch, v_pitch, scales, stage, q_pitch;
-    __host__ __device__ Layout(int dim, bool fp4) {
+    int k_pitch, v_pitch, scales, half, q_pitch, expand;      // expand: K's scales as floats, V's as pairs of binary16 powers
+    constexpr __host__ __device__ Layout(int dim, bool fp4)
+        : k_pitch(0), v_pitch(0), scales(0), half(0), q_pitch(0), expand(0) {
         const int nb = dim / 32, row = fp4 ? dim / 2 : dim, odd16 = ((row / 16) | 1) * 16;
         k_pitch = fp4 ? odd16 : ((row / 32) | 1) * 32;
         v_pitch = odd16;
-        scales = kTok * (k_pitch + v_pitch);
-        stage = (scales + 2 * kTok * nb + 16 + 15) / 16 * 16;
+        scales = kTok * (k_pitch > v_pitch ? k_pitch : v_pitch);
+        half = scales + kTok * nb;             // K or V of 32 tokens
         q_pitch = (nb | 1) * 64;
+        expand = nb * kTok * 4 + kTok / 2 * ((nb + 3) & ~3) * 4 * 2;
     }
 };
-__host__ __device__ __forceinline__ int smem_bytes(int dim, bool fp4, int nt, int stages) {
+__host__ __device__ __forceinline__ int smem_bytes(int dim, bool fp4, int nt) {
     const Layout l(dim, fp4);
-    const int ring = kWarps * stages * l.stage, cols = 8 * nt;
+    const int ring = kWarps * (3 * l.half + l.expand), cols = 8 * nt;
     const int merge = kWarps * cols * (dim + 4) * 4;
     return cols * l.q_pitch + (ring > merge ? ring : merge);
 }
 
-template <int NBT, bool FP4, int PIECES, int NT, int STAGES>
-__global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const AttentionParams p) {
+// How the work is shared out.  A sequence's row tiles have `pieces` pieces of 32 tokens each (as many as its last one, or what a
+// window leaves; one at least, so that rows that see nothing are written); all pieces of all (sequence, kv head, row tile) in that
+// order are cut into equal runs, one for each CTA.  A row tile that lies in one run is finished there; of one that is cut each
+// CTA leaves its sums in a slot, which mx_attention_join_kernel joins.
+struct Work { int tiles, pieces; };            // of a sequence, for each kv head
+
+__device__ __forceinline__ Work work_of(const AttentionParams& p, int seq) {
+    Work w;
+    w.tiles = (int)(((int64_t)rows_of(p.c, seq).y * p.group + p.tile_rows - 1) / p.tile_rows);
+    const int end = min(__ldg(p.c.lens + seq), p.c.capacity());
+    int most = (end + kTok - 1) / kTok;
+    if (p.window > 0) most = (int)min((int64_t)most, ((int64_t)p.sinks + kTok - 1) / kTok + ((int64_t)p.window + p.tile_rows + kTok - 1) / kTok + 1);
+    w.pieces = max(most, 1);
+    return w;
+}
+
+// A place in the run of all pieces.
+struct Place { int seq, item, piece; Work w; };
+
+// Finds where run `run` begins (`place` means nothing behind the last one); `per`: pieces of a run; returns the number of all pieces.  Called by whole blocks of 128 threads; `sm` has room for 8 words.
+__device__ __forceinline__ int64_t find_place(const AttentionParams& p, int run, int64_t& per, Place& place, int64_t* sm) {
+    const int each = (p.c.seqs + blockDim.x - 1) / blockDim.x, s0 = min((int)threadIdx.x * each, p.c.seqs), s1 = min(s0 + each, p.c.seqs);
+    int64_t mine = 0;
+    for (int s = s0; s < s1; ++s) {
+        const Work w = work_of(p, s);
+        mine += (int64_t)w.tiles * w.pieces;
+    }
+    mine *= p.c.heads;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) sm[warp] = upto;
+    __syncthreads();
+    int64_t before = 0, total = 0;
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) {
+        if (w < warp) before += sm[w];
+        total += sm[w];
+    }
+    upto += before;
+    per = max((total + p.runs - 1) / p.runs, (int64_t)p.least);
+    const int64_t at = run * per;
+    Place* out = reinterpret_cast<Place*>(sm + 4);
+    if (at >= upto - mine && at < upto) {
+        int64_t rest = at - (upto - mine);
+        for (int s = s0; s < s1; ++s) {
+            const Work w = work_of(p, s);
+            const int64_t all = (int64_t)w.tiles * w.pieces * p.c.heads;
+            if (rest < all) {
+                *out = Place{s, (int)(rest / w.pieces), (int)(rest % w.pieces), w};
+                break;
+            }
+            rest -= all;
+        }
+    }
+    __syncthreads();
+    place = *out;
+    return total;
+}
+
+template <int NB, bool FP4, int PIECES, int NT>
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 && NB <= 4 ? 4 : NB * NT <= 8 ? 3 : 2) mx_attention_rows_kernel(const AttentionParams p) {
     constexpr int kCols = 8 * NT, kRows = kCols / PIECES, kMine = PIECES == 1 ? 2 * NT : NT;   // columns and rows of the CTA; rows that a lane holds
     extern __shared__ __align__(16) uint8_t smem[];
     const CacheView& c = p.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, tig = lane & 3;
-    const int dim = c.dim, nb = dim >> 5, head = blockIdx.y, split = blockIdx.z;
-    const Layout lay(dim, FP4);
-    if (split == 0 && head == 0) zero_outside(p);
-    int seq, tile;
-    if (!find_tile(p, blockIdx.x, seq, tile)) return;
+    constexpr int dim = 32 * NB, nb = NB;
+    constexpr Layout lay(dim, FP4);
+    __shared__ int64_t place_sm[9];
+    __shared__ float row_mul[kRows];
+    zero_outside(p);
+    Place at;
+    int64_t per;
+    const int64_t total = find_place(p, blockIdx.x, per, at, place_sm);
+    int64_t left = min(per, total - blockIdx.x * per);
+    bool begins = true;                         // the segment stands at the beginning of this CTA's run
+    while (left > 0) {
+    const int seq = at.seq, head = at.item / at.w.tiles, tile = at.item - head * at.w.tiles;
+    const int take = (int)min((int64_t)(at.w.pieces - at.piece), left);
     const int2 own = rows_of(c, seq);
     const int first = tile * kRows, count = min(kRows, own.y * p.group - first);
-    if (count <= 0) return;
     const int len = __ldg(c.lens + seq), pos0 = len - own.y;
     const TokenTiles<kTok> tt(p, pos0 + first / p.group, pos0 + (first + count - 1) / p.group);
-    // parts of at least two tiles a warp
-    const int parts = max(1, min(p.splits, tt.tiles / (2 * kWarps)));
-    if (split >= parts) return;
-    const int j_lo = (int)((int64_t)tt.tiles * split / parts), j_hi = (int)((int64_t)tt.tiles * (split + 1) / parts);
+    const bool finished = take == at.w.pieces;
+    const int j_lo = min(at.piece, tt.tiles), j_hi = min(at.piece + take, tt.tiles);
 
     uint8_t* q_sm = smem;
-    uint8_t* ring = smem + kCols * lay.q_pitch + warp * STAGES * lay.stage;
+    uint8_t* ring = smem + kCols * lay.q_pitch + warp * (3 * lay.half + lay.expand);
+    float* k_scale = reinterpret_cast<float*>(ring + 3 * lay.half);                       // [block][token]
+    uint32_t* v_scale = reinterpret_cast<uint32_t*>(k_scale + nb * kTok);                       // [pair of tokens][block, of four]
+    constexpr int nb4 = (nb + 3) & ~3;
+    uint32_t* v_scale2 = v_scale + kTok / 2 * nb4;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
 
     // ---- the warp's ring
-    const int row_bytes = FP4 ? dim >> 1 : dim, chunks = row_bytes >> 4, inv = 65536 / chunks + 1;
+    constexpr int row_bytes = FP4 ? dim / 2 : dim, chunks = row_bytes / 16, put_step = 32 / chunks;
+    const int in_page = (1 << c.page_shift) - 1;
+    const int put_tok = lane / chunks, put_ch = lane - put_tok * chunks;        // this lane's token and piece of 16 bytes
     auto page_of = [&](int j) -> int {          // the page of this lane's token of tile j; -1: none
         if (j >= j_hi) return -1;
         const int t = tt.start(j) + lane, slot = t >> c.page_shift;
@@ -103,47 +185,51 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
         const int page = __ldg(c.pages + (int64_t)seq * c.width + slot);
         return page >= 0 && page < c.num_pages ? page : -1;
     };
-    auto issue = [&](int j, int stage, int page) {
+    // K (or V) of the 32 tokens of tile j into place `slot` of the ring
+    auto issue = [&](const uint8_t* codes, const uint8_t* scales, int pitch, int j, int slot, int page) {
         if (j < j_hi) {
-            const uint32_t at = ring_at + stage * lay.stage;
-            const int t0 = tt.start(j), in_page = (1 << c.page_shift) - 1;
-            for (int i = 0; i < chunks; ++i) {
-                const int idx = i * 32 + lane, tok = (idx * inv) >> 16, ch = idx - tok * chunks;
-                const int pg = __shfl_sync(0xFFFFFFFFu, page, tok);
-                const int64_t row = (((int64_t)max(pg, 0) * c.heads + head) << c.page_shift) + ((t0 + tok) & in_page);
-                const int64_t off = row * row_bytes + ch * 16;
-                cp16(at + tok * lay.k_pitch + ch * 16, c.k_codes + (pg >= 0 ? off : 0), pg >= 0);
-                cp16(at + kTok * lay.k_pitch + tok * lay.v_pitch + ch * 16, c.v_codes + (pg >= 0 ? off : 0), pg >= 0);
+            const uint32_t at = ring_at + slot * lay.half, to = at + put_tok * pitch + put_ch * 16;
+            const int t0 = tt.start(j);
+            const unsigned live = __ballot_sync(0xFFFFFFFFu, page >= 0);
+            if (live == 0xFFFFFFFFu && c.page_shift >= 5) {                    // 32 rows that lie together
+                const int64_t row = (((int64_t)page * c.heads + head) << c.page_shift) + (t0 & in_page) + put_tok;
+                const uint8_t* src = codes + row * row_bytes + put_ch * 16;
+                if (put_tok < put_step) {
+#pragma unroll
+                    for (int base = 0; base < kTok; base += put_step)
+                        if (base + put_step <= kTok || base + put_tok < kTok) cp16(to + base * pitch, src + base * row_bytes, true);
+                }
+            } else {
+                const int64_t mine = (((int64_t)max(page, 0) * c.heads + head) << c.page_shift) + ((t0 + lane) & in_page);
+                for (int base = 0; base < kTok; base += put_step) {
+                    const int tok = min(base + put_tok, kTok - 1);
+                    const int64_t row = __shfl_sync(0xFFFFFFFFu, mine, tok);
+                    const bool on = (live >> tok) & 1u;
+                    if (put_tok < put_step && base + put_tok < kTok) cp16(to + base * pitch, codes + (on ? row * row_bytes + put_ch * 16 : 0), on);
+                }
             }
             const int grp = lane / nb, pg = __shfl_sync(0xFFFFFFFFu, page, min(grp, 3) * 8);
             if (grp < 4) {                      // eight tokens' scales lie together, whatever the page size
                 const int64_t row = (((int64_t)max(pg, 0) * c.heads + head) << c.page_shift) + ((t0 + grp * 8) & in_page);
-                const int64_t off = pg >= 0 ? row * nb + (lane - grp * nb) * 8 : 0;
-                cp8(at + lay.scales + lane * 8, c.k_scales + off, pg >= 0);
-                cp8(at + lay.scales + kTok * nb + lane * 8, c.v_scales + off, pg >= 0);
+                cp8(at + lay.scales + lane * 8, scales + (pg >= 0 ? row * nb + (lane - grp * nb) * 8 : 0), pg >= 0);
             }
-            const unsigned there = __ballot_sync(0xFFFFFFFFu, page >= 0);
-            if (lane == 0) *reinterpret_cast<uint32_t*>(ring + stage * lay.stage + lay.scales + 2 * kTok * nb) = there;
         }
         asm volatile("cp.async.commit_group;\n" ::);
     };
-    int j_put = j_lo + warp, page_put = page_of(j_put);
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-        issue(j_put, s, page_put);
-        j_put += kWarps;
-        page_put = page_of(j_put);
-    }
+    int page_put = page_of(j_lo + warp);
+    unsigned there = __ballot_sync(0xFFFFFFFFu, page_put >= 0);               // which tokens of the tile there are
+    issue(c.k_codes, c.k_scales, lay.k_pitch, j_lo + warp, 0, page_put);
+    issue(c.v_codes, c.v_scales, lay.v_pitch, j_lo + warp, 1, page_put);
+    page_put = page_of(j_lo + warp + kWarps);
 
     // ---- q: scaled by a power of two, as binary16 columns; one warp takes a row at a time
-    __shared__ float row_mul[kRows];
     for (int r = warp; r < kRows; r += kWarps) {
         const int rr = first + r, i = rr / p.group;
-        float x[NBT], top = 0.f;
+        float x[NB], top = 0.f;
 #pragma unroll
-        for (int b = 0; b < NBT; ++b) {
+        for (int b = 0; b < NB; ++b) {
             x[b] = 0.f;
-            if (b < nb && r < count) {
+            if (r < count) {
                 const int64_t off = c.starts == nullptr ? seq * p.q_seq + i * p.q_row : (own.x + i) * p.q_row;
                 x[b] = load_value(p.q, p.dtype, off + (head * p.group + rr - i * p.group) * p.q_head + b * 32 + lane);
                 const float a = fabsf(x[b]);
@@ -155,8 +241,8 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
         const float up = __uint_as_float((uint32_t)(127 + e) << 23);
         if (lane == 0) row_mul[r] = p.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
-        for (int b = 0; b < NBT; ++b) {
-            if (b < nb) {
+        for (int b = 0; b < NB; ++b) {
+            {
                 const float v = x[b] * up;
                 const __half hi = __float2half_rn(v);
                 __half* to = reinterpret_cast<__half*>(q_sm + r * PIECES * lay.q_pitch) + b * 32 + lane;
@@ -184,9 +270,9 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
         poison[r] = 0u;
     }
     const int low_pos = pos0 + first / p.group, high_pos = pos0 + (first + count - 1) / p.group;
-    float o[NBT][2][NT][4];
+    float o[NB][2][NT][4];
 #pragma unroll
-    for (int b = 0; b < NBT; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -194,52 +280,22 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[b][j][n][i] = 0.f;
 
-    int stage = 0;
-    for (int j = j_lo + warp; j < j_hi; j += kWarps) {
-        {
-            int put = stage + STAGES - 1;
-            if (put >= STAGES) put -= STAGES;
-            issue(j_put, put, page_put);
-            j_put += kWarps;
-            page_put = page_of(j_put);
-        }
-        asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 1));
-        __syncwarp();
-        uint8_t* k_sm = ring + stage * lay.stage;
-        uint8_t* v_sm = k_sm + kTok * lay.k_pitch;
-        const uint8_t* ks = k_sm + lay.scales;
-        const uint8_t* vs = ks + kTok * nb;
-        const uint32_t there = *reinterpret_cast<const uint32_t*>(vs + kTok * nb);
-        const int t0 = tt.start(j);
-
-        // a block scale of 0xFF: what the tokens' rows of K and V hold there is NaN
-        uint32_t k_nan = 0u;
-        bool ff = false;
-        if (lane < 4 * nb) {
-            const uint2 a = reinterpret_cast<const uint2*>(ks)[lane], b = reinterpret_cast<const uint2*>(vs)[lane];
-            ff = has_ff(a.x) || has_ff(a.y) || has_ff(b.x) || has_ff(b.y);
-        }
-        if (__any_sync(0xFFFFFFFFu, ff)) {
-            bool bad_k = false;
-            uint32_t bad_v = 0u;
-            if ((there >> lane) & 1u)
-                for (int b = 0; b < nb; ++b) {
-                    bad_k |= ks[lane * nb + b] == 255;
-                    if (vs[lane * nb + b] == 255) {
-                        bad_v |= 1u << b;
-                        for (int i = 0; i < (FP4 ? 4 : 8); ++i) reinterpret_cast<uint32_t*>(v_sm + lane * lay.v_pitch)[b * (FP4 ? 4 : 8) + i] = 0u;
-                    }
-                }
-            k_nan = __ballot_sync(0xFFFFFFFFu, bad_k);
-            for (uint32_t some = __ballot_sync(0xFFFFFFFFu, bad_v != 0u); some; some &= some - 1) {
-                const int t = __ffs(some) - 1;
-                const uint32_t blocks = __shfl_sync(0xFFFFFFFFu, bad_v, t);
+    int v_top[NB];                            // the exponent that the sums of a block are relative to, the largest so far
 #pragma unroll
-                for (int r = 0; r < kMine; ++r)
-                    if (sees(p, pos[r], t0 + t)) poison[r] |= blocks;
-            }
-            __syncwarp();
-        }
+    for (int b = 0; b < NB; ++b) v_top[b] = 0;
+    // The ring has three places: while K of a tile is used, V of it and K of the warp's next tile are on the way.
+    int slot = 0;
+    for (int j = j_lo + warp; j < j_hi; j += kWarps) {
+        const int slot_v = slot == 2 ? 0 : slot + 1, slot_k = slot_v == 2 ? 0 : slot_v + 1;
+        issue(c.k_codes, c.k_scales, lay.k_pitch, j + kWarps, slot_k, page_put);
+        asm volatile("cp.async.wait_group 2;\n" ::);
+        __syncwarp();
+        const uint8_t* k_sm = ring + slot * lay.half;
+        uint8_t* v_sm = ring + slot_v * lay.half;
+        const int t0 = tt.start(j);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) k_scale[b * kTok + lane] = e8m0_value(k_sm[lay.scales + lane * nb + b]);
+        __syncwarp();
 
         // ---- scores
         float s[2][NT][4];
@@ -250,8 +306,8 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[mt][n][i] = 0.f;
 #pragma unroll
-        for (int b = 0; b < NBT; ++b) {
-            if (b < nb) {
+        for (int b = 0; b < NB; ++b) {
+            {
                 uint4 qb[NT];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) qb[n] = *reinterpret_cast<const uint4*>(q_sm + (n * 8 + g) * lay.q_pitch + b * 64 + tig * 16);
@@ -267,13 +323,11 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
                         e4m3x4_to_half(x.x, a[0], a[1]); e4m3x4_to_half(x.y, a[2], a[3]);
                         e4m3x4_to_half(y.x, d[0], d[1]); e4m3x4_to_half(y.y, d[2], d[3]);
                     }
-                    // 2^-127 for a code of 0; a code of 0xFF (infinity here) is looked for above
-                    const float s0 = __uint_as_float(max((uint32_t)ks[(mt * 16 + g) * nb + b] << 23, 0x00400000u));
-                    const float s1 = __uint_as_float(max((uint32_t)ks[(mt * 16 + 8 + g) * nb + b] << 23, 0x00400000u));
+                    const float s0 = k_scale[b * kTok + mt * 16 + g], s1 = k_scale[b * kTok + mt * 16 + 8 + g];
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma16816(acc, a[0], d[0], a[1], d[1], qb[n].x, qb[n].y);
+                        float acc[4];
+                        mma16816_first(acc, a[0], d[0], a[1], d[1], qb[n].x, qb[n].y);
                         mma16816(acc, a[2], d[2], a[3], d[3], qb[n].z, qb[n].w);
                         s[mt][n][0] = fmaf(acc[0], s0, s[mt][n][0]);
                         s[mt][n][1] = fmaf(acc[1], s0, s[mt][n][1]);
@@ -283,6 +337,7 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
                 }
             }
         }
+        __syncwarp();                           // K's place is free
         // x[r][i]: row r of this lane, token g + 8 i of the tile, in units of log 2
         float x[kMine][4];
 #pragma unroll
@@ -292,7 +347,7 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
                 if (PIECES == 1) x[r][i] = s[i >> 1][r >> 1][2 * (i & 1) + (r & 1)] * mul[r];
                 else x[r][i] = fmaf(s[i >> 1][r][2 * (i & 1) + 1], 0x1p-11f, s[i >> 1][r][2 * (i & 1)]) * mul[r];
             }
-        const bool whole = there == 0xFFFFFFFFu && k_nan == 0u && t0 + kTok - 1 <= low_pos && (p.window <= 0 || t0 > high_pos - p.window);
+        const bool whole = there == 0xFFFFFFFFu && t0 + kTok - 1 <= low_pos && (p.window <= 0 || t0 > high_pos - p.window);
         if (!whole) {
 #pragma unroll
             for (int r = 0; r < kMine; ++r)
@@ -300,7 +355,6 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
                 for (int i = 0; i < 4; ++i) {
                     const int t = g + 8 * i;
                     const bool on = ((there >> t) & 1u) && sees(p, pos[r], t0 + t);
-                    if ((k_nan >> t) & 1u) x[r][i] = __uint_as_float(0x7FC00000u);
                     x[r][i] = on ? x[r][i] : -INFINITY;
                 }
         }
@@ -318,7 +372,7 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
                 m[r] = top;
                 l[r] *= fade;
 #pragma unroll
-                for (int b = 0; b < NBT; ++b)
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int jj = 0; jj < 2; ++jj) {
                         if (PIECES == 1) {
@@ -356,41 +410,95 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
                 }
                 pw[i >> 1][n][i & 1] = transpose8x8(w);
             }
+        // ---- scales of V: each lane those of its token, relative to the largest so far, as binary16 powers of two
+        issue(c.v_codes, c.v_scales, lay.v_pitch, j + kWarps, slot, page_put);
+        asm volatile("cp.async.wait_group 2;\n" ::);
+        __syncwarp();
+        bool bad = false, higher_v = false;
+        int ev[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            ev[b] = ((there >> lane) & 1u) ? v_sm[lay.scales + lane * nb + b] : 0;
+            bad |= ev[b] == 255;
+            higher_v |= ev[b] > v_top[b];
+        }
+        if (__any_sync(0xFFFFFFFFu, higher_v)) {
+            if (__any_sync(0xFFFFFFFFu, bad)) {
+                // a block scale of 0xFF: NaN for the rows that see the token, and nothing for those that do not
+                uint32_t blocks_v = 0u;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    if (ev[b] == 255) {
+                        blocks_v |= 1u << b;
+                        ev[b] = 0;
+                        for (int i = 0; i < (FP4 ? 4 : 8); ++i) reinterpret_cast<uint32_t*>(v_sm + lane * lay.v_pitch)[b * (FP4 ? 4 : 8) + i] = 0u;
+                    }
+                for (uint32_t some = __ballot_sync(0xFFFFFFFFu, blocks_v != 0u); some; some &= some - 1) {
+                    const int t = __ffs(some) - 1;
+                    const uint32_t blocks = __shfl_sync(0xFFFFFFFFu, blocks_v, t);
+#pragma unroll
+                    for (int r = 0; r < kMine; ++r)
+                        if (sees(p, pos[r], t0 + t)) poison[r] |= blocks;
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                {
+                    const int top = max(v_top[b], (int)__reduce_max_sync(0xFFFFFFFFu, (uint32_t)ev[b]));
+                    const float fade = top - v_top[b] > 126 ? 0.f : __uint_as_float((uint32_t)(127 - top + v_top[b]) << 23);
+                    v_top[b] = top;
+#pragma unroll
+                    for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[b][jj][n][i] *= fade;
+                }
+        }
+        bool far = false;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            ev[b] = v_top[b] - ev[b];
+            far |= ev[b] > 14 && ((there >> lane) & 1u);
+        }
+        far = __any_sync(0xFFFFFFFFu, far);
+        uint32_t h[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            h[b] = far ? half_power(min(ev[b], 24)) : (uint32_t)(15 - min(ev[b], 14)) << 10;
+            h[b] |= __shfl_down_sync(0xFFFFFFFFu, h[b], 1) << 16;              // whole in the even lanes
+        }
+        if (!(lane & 1)) {
+#pragma unroll
+            for (int b = 0; b < NB; b += 4)
+                *reinterpret_cast<uint4*>(v_scale + (lane >> 1) * nb4 + b) =
+                    make_uint4(h[b], h[b + 1 < NB ? b + 1 : b], h[b + 2 < NB ? b + 2 : b], h[b + 3 < NB ? b + 3 : b]);
+        }
+        if (far) {                              // binary16 has no power below 2^-24: scales further apart take a second factor
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                uint32_t x = half_power(max(ev[b] - 24, 0));
+                x |= __shfl_down_sync(0xFFFFFFFFu, x, 1) << 16;
+                if (!(lane & 1)) v_scale2[(lane >> 1) * nb4 + b] = x;
+            }
+        }
+        __syncwarp();
+
         // ---- values
 #pragma unroll
-        for (int b = 0; b < NBT; ++b) {
-            if (b < nb) {
-                uint32_t e = ((there >> lane) & 1u) ? vs[lane * nb + b] : 0u;      // this lane's token
-                e = e == 255u ? 0u : e;
-                const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, e);
-                const int down = (int)(top - e);
-                uint32_t h = half_power(min(down, 24));
-                h |= __shfl_down_sync(0xFFFFFFFFu, h, 1) << 16;                     // whole in the even lanes
-                // binary16 has no power below 2^-24: scales further apart take a second factor
-                const bool wide = __any_sync(0xFFFFFFFFu, down > 24);
-                uint32_t h2 = 0u;
-                if (wide) {
-                    h2 = half_power(max(down - 24, 0));
-                    h2 |= __shfl_down_sync(0xFFFFFFFFu, h2, 1) << 16;
-                }
-                const float up = e8m0_value(top);
-                float acc[2][NT][4];
-#pragma unroll
-                for (int jj = 0; jj < 2; ++jj)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[jj][n][i] = 0.f;
+        for (int b = 0; b < NB; ++b) {
+            {
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt) {
                     uint32_t pb[NT][2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const uint32_t sc = __shfl_sync(0xFFFFFFFFu, h, mt * 16 + i * 8 + 2 * tig);
+                        const int pair = mt * 8 + i * 4 + tig;
+                        const uint32_t sc = v_scale[pair * nb4 + b];
 #pragma unroll
                         for (int n = 0; n < NT; ++n) pb[n][i] = mul_half2(pw[mt][n][i], sc);
-                        if (wide) {
-                            const uint32_t sc2 = __shfl_sync(0xFFFFFFFFu, h2, mt * 16 + i * 8 + 2 * tig);
+                        if (far) {
+                            const uint32_t sc2 = v_scale2[pair * nb4 + b];
 #pragma unroll
                             for (int n = 0; n < NT; ++n) pb[n][i] = mul_half2(pb[n][i], sc2);
                         }
@@ -420,18 +528,14 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
 #pragma unroll
                     for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma16816(acc[jj][n], a[jj][0], a[jj][1], a[jj][2], a[jj][3], pb[n][0], pb[n][1]);
+                        for (int n = 0; n < NT; ++n) mma16816(o[b][jj][n], a[jj][0], a[jj][1], a[jj][2], a[jj][3], pb[n][0], pb[n][1]);
                 }
-#pragma unroll
-                for (int jj = 0; jj < 2; ++jj)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[b][jj][n][i] = fmaf(acc[jj][n][i], up, o[b][jj][n][i]);
             }
         }
         __syncwarp();
-        if (++stage == STAGES) stage = 0;
+        slot = slot_k;
+        there = __ballot_sync(0xFFFFFFFFu, page_put >= 0);
+        page_put = page_of(j + 2 * kWarps);
     }
     asm volatile("cp.async.wait_group 0;\n" ::);
     __syncthreads();
@@ -447,27 +551,28 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
         if (g == 0) {
             float* to = stats + (warp * kRows + at) * 3;
             to[0] = m[r];
-            to[1] = l[r];
+            to[1] = 0x1p-15f * l[r];
             to[2] = __uint_as_float(poison[r]);
         }
 #pragma unroll
-        for (int b = 0; b < NBT; ++b)
-            if (b < nb) {
+        for (int b = 0; b < NB; ++b)
+            {
                 float* to = sums + (warp * kRows + at) * dim + b * 32 + 4 * g;
+                const float up = e8m0_value(v_top[b]);             // after the 2^15 of the weights, so that no large V overflows
 #pragma unroll
                 for (int jj = 0; jj < 2; ++jj) {
                     if (PIECES == 1) {
-                        to[2 * jj] = o[b][jj][r >> 1][r & 1];
-                        to[2 * jj + 1] = o[b][jj][r >> 1][2 + (r & 1)];
+                        to[2 * jj] = up * (0x1p-15f * o[b][jj][r >> 1][r & 1]);
+                        to[2 * jj + 1] = up * (0x1p-15f * o[b][jj][r >> 1][2 + (r & 1)]);
                     } else {
-                        to[2 * jj] = fmaf(o[b][jj][r][1], 0x1p-11f, o[b][jj][r][0]);
-                        to[2 * jj + 1] = fmaf(o[b][jj][r][3], 0x1p-11f, o[b][jj][r][2]);
+                        to[2 * jj] = up * (0x1p-15f * fmaf(o[b][jj][r][1], 0x1p-11f, o[b][jj][r][0]));
+                        to[2 * jj + 1] = up * (0x1p-15f * fmaf(o[b][jj][r][3], 0x1p-11f, o[b][jj][r][2]));
                     }
                 }
             }
     }
     __syncthreads();
-    const int64_t part = ((int64_t)blockIdx.x * c.heads + head) * p.splits + split;
+    const int share = 2 * blockIdx.x + (begins ? 0 : 1);
     for (int r = warp; r < count; r += kWarps) {
         float top = -INFINITY, w[kWarps], sum = 0.f;
         uint32_t bad = 0u;
@@ -489,39 +594,55 @@ __global__ void __launch_bounds__(32 * kWarps) mx_attention_rows_kernel(const At
 #pragma unroll
             for (int k = 0; k < kWarps; ++k) v = fmaf(sums[(k * kRows + r) * dim + d], w[k], v);
             if ((bad >> b) & 1u) v = __uint_as_float(0x7FC00000u);
-            if (parts == 1) store_value(p.out, p.dtype, out_row + d, v * inv_sum);
-            else p.partial[(part * kRows + r) * dim + d] = v;
+            if (finished) store_value(p.out, p.dtype, out_row + d, v * inv_sum);
+            else p.partial[((int64_t)share * kRows + r) * dim + d] = v;
         }
-        if (parts > 1 && lane == 0) {
-            p.stats[(part * kRows + r) * 2] = top;
-            p.stats[(part * kRows + r) * 2 + 1] = sum;
+        if (!finished && lane == 0) {
+            p.stats[(share * kRows + r) * 2] = top;
+            p.stats[(share * kRows + r) * 2 + 1] = sum;
         }
+    }
+    __syncthreads();
+    // ---- the next piece of the run
+    left -= take;
+    begins = false;
+    at.piece = 0;
+    if (left > 0 && ++at.item == at.w.tiles * c.heads) {
+        at.item = 0;
+        do { at.w = work_of(p, ++at.seq); } while (at.w.tiles == 0);
+    }
     }
 }
 
-// Joins the parts of each row: a warp per row.
+// Joins the row tiles that runs end in: CTA x looks at the end of run x, where run x + 1 begins.  A warp takes a row.
 __global__ void __launch_bounds__(128) mx_attention_join_kernel(const AttentionParams p) {
     const CacheView& c = p.c;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = c.dim, nb = dim >> 5, head = blockIdx.y;
-    int seq, tile;
-    if (!find_tile(p, blockIdx.x, seq, tile)) return;
-    const int2 own = rows_of(c, seq);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = c.dim, nb = dim >> 5;
+    __shared__ int64_t place_sm[9];
+    Place at;
+    int64_t per;
+    const int run = blockIdx.x;
+    const int64_t total = find_place(p, run + 1, per, at, place_sm), cut = (run + 1) * per;
+    if (cut >= total || at.piece == 0) return;                     // nothing is cut here
+    const int64_t p0 = cut - at.piece, p1 = p0 + at.w.pieces;
+    if (run * per > p0) return;                                    // an earlier CTA joins this one
+    const int last = (int)((p1 - 1) / per);
+    const int head = at.item / at.w.tiles, tile = at.item - head * at.w.tiles;
+    const int2 own = rows_of(c, at.seq);
     const int first = tile * p.tile_rows, count = min(p.tile_rows, own.y * p.group - first);
-    if (count <= 0) return;
-    const int pos0 = __ldg(c.lens + seq) - own.y;
-    const TokenTiles<kTok> tt(p, pos0 + first / p.group, pos0 + (first + count - 1) / p.group);
-    const int parts = max(1, min(p.splits, tt.tiles / (2 * kWarps)));
-    if (parts == 1) return;
-    const int64_t part0 = ((int64_t)blockIdx.x * c.heads + head) * p.splits;
+    auto slot_of = [&](int k) { return 2 * k + (k == run && run * per < p0 ? 1 : 0); };
     for (int r = warp; r < count; r += 4) {
         float top = -INFINITY;
-        for (int k = 0; k < parts; ++k) top = fmaxf(top, p.stats[((part0 + k) * p.tile_rows + r) * 2]);
+        for (int k = run + lane; k <= last; k += 32) top = fmaxf(top, p.stats[(slot_of(k) * p.tile_rows + r) * 2]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
         float sum = 0.f, v[8] = {};
-        for (int k = 0; k < parts; ++k) {
-            const float* st = p.stats + ((part0 + k) * p.tile_rows + r) * 2;
+        for (int k = run; k <= last; ++k) {
+            const int slot = slot_of(k);
+            const float* st = p.stats + (slot * p.tile_rows + r) * 2;
             const float w = st[0] == -INFINITY ? (st[1] != st[1] ? st[1] : 0.f) : exp2_fast(st[0] - top);
             sum = fmaf(st[1], w, sum);
-            const float* from = p.partial + ((part0 + k) * p.tile_rows + r) * dim + lane;
+            const float* from = p.partial + ((int64_t)slot * p.tile_rows + r) * dim + lane;
 #pragma unroll
             for (int b = 0; b < 8; ++b)
                 if (b < nb) v[b] = fmaf(from[b * 32], w, v[b]);
@@ -535,10 +656,9 @@ __global__ void __launch_bounds__(128) mx_attention_join_kernel(const AttentionP
     }
 }
 
-// How a call is cut: columns of a tile, row tiles, parts of the tokens.
+// How a call is cut: columns of a tile, and CTAs.
 struct Plan {
-    int pieces, nt, tile_rows, tiles_per_seq, splits;
-    int64_t tiles;
+    int pieces, nt, tile_rows, runs;
     size_t partial_floats, stats_floats;
 };
 
@@ -549,41 +669,58 @@ Plan make_plan(const CacheView& c, int q_heads, int dtype, int window, int sinks
     const int64_t per_seq = c.starts == nullptr ? (int64_t)c.new_rows * group : (c.seqs ? (c.rows * group + c.seqs - 1) / c.seqs : 0);
     pl.nt = per_seq * pl.pieces > 8 ? 2 : 1;
     pl.tile_rows = 8 * pl.nt / pl.pieces;
-    pl.tiles_per_seq = (int)(((int64_t)c.new_rows * group + pl.tile_rows - 1) / pl.tile_rows);
-    pl.tiles = c.starts == nullptr ? (int64_t)c.seqs * pl.tiles_per_seq : (c.rows * group + pl.tile_rows - 1) / pl.tile_rows + c.seqs;
-    // parts: two waves of two CTAs on each SM, a part having two tiles for each warp at least
+    // at most four CTAs on each SM, and no more than there is work for if every sequence is as long as its row of the page table
     int64_t tokens = (int64_t)c.width << c.page_shift;
-    if (window > 0) tokens = tokens < (int64_t)window + sinks + 2 * kTok ? tokens : (int64_t)window + sinks + 2 * kTok;
-    const int64_t most = tokens / kTok / (2 * kWarps), want = (4 * (int64_t)sm_count() + pl.tiles * c.heads - 1) / (pl.tiles * c.heads > 0 ? pl.tiles * c.heads : 1);
-    pl.splits = (int)(want < 1 ? 1 : want > most ? (most < 1 ? 1 : most) : want);
-    if (pl.splits > 64) pl.splits = 64;
-    const size_t rows = (size_t)pl.tiles * c.heads * pl.splits * pl.tile_rows;
-    pl.partial_floats = pl.splits > 1 ? rows * c.dim : 0;
-    pl.stats_floats = pl.splits > 1 ? rows * 2 : 0;
+    if (window > 0 && tokens > (int64_t)window + sinks + 4 * kTok) tokens = (int64_t)window + sinks + 4 * kTok;
+    const int64_t tiles = c.rows * group / pl.tile_rows + c.seqs, pieces = (tokens + kTok - 1) / kTok + 1, most = 4 * (int64_t)sm_count();
+    const int64_t want = (tiles * c.heads * pieces + kLeast - 1) / kLeast;
+    pl.runs = (int)(want < 1 ? 1 : want > most ? most : want);
+    pl.partial_floats = (size_t)2 * pl.runs * pl.tile_rows * c.dim;
+    pl.stats_floats = (size_t)2 * pl.runs * pl.tile_rows * 2;
     return pl;
 }
 
-template <int NBT, bool FP4, int PIECES, int NT>
-int launch_rows(const AttentionParams& p, const Plan& pl, cudaStream_t st) {
-    constexpr int STAGES = 2;
-    const int bytes = smem_bytes(p.c.dim, FP4, NT, STAGES);
-    auto kern = mx_attention_rows_kernel<NBT, FP4, PIECES, NT, STAGES>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return check_launch("mx_attention");
-    kern<<<dim3((unsigned)pl.tiles, (unsigned)p.c.heads, (unsigned)pl.splits), 32 * kWarps, bytes, st>>>(p);
-    if (pl.splits > 1) mx_attention_join_kernel<<<dim3((unsigned)pl.tiles, (unsigned)p.c.heads), 128, 0, st>>>(p);
+template <int NB, bool FP4, int PIECES, int NT>
+int launch_rows(AttentionParams p, const Plan& pl, cudaStream_t st) {
+    const int bytes = smem_bytes(p.c.dim, FP4, NT);
+    auto kern = mx_attention_rows_kernel<NB, FP4, PIECES, NT>;
+    static std::atomic<int> resident[64];        // CTAs of this kernel on an SM, by device; 0: not asked yet
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { set_error("mx_attention: no device"); return MPT_ERR_CUDA; }
+    int fit = resident[dev].load(std::memory_order_relaxed);
+    if (fit == 0) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, 32 * kWarps, bytes) != cudaSuccess || fit < 1) {
+            check_launch("mx_attention");
+            set_error("mx_attention: the kernel does not fit this device");
+            return MPT_ERR_CUDA;
+        }
+        resident[dev].store(fit, std::memory_order_relaxed);
+    }
+    const int most = fit * sm_count();
+    p.runs = pl.runs < most ? pl.runs : most;
+    kern<<<(unsigned)p.runs, 32 * kWarps, bytes, st>>>(p);
+    if (p.runs > 1) mx_attention_join_kernel<<<(unsigned)(p.runs - 1), 128, 0, st>>>(p);
     return check_launch("mx_attention");
 }
 
-template <int NBT, bool FP4>
+template <int NB, bool FP4>
 int launch_rows(const AttentionParams& p, const Plan& pl, cudaStream_t st) {
-    if (pl.pieces == 1) return pl.nt == 1 ? launch_rows<NBT, FP4, 1, 1>(p, pl, st) : launch_rows<NBT, FP4, 1, 2>(p, pl, st);
-    return pl.nt == 1 ? launch_rows<NBT, FP4, 2, 1>(p, pl, st) : launch_rows<NBT, FP4, 2, 2>(p, pl, st);
+    if (pl.pieces == 1) return pl.nt == 1 ? launch_rows<NB, FP4, 1, 1>(p, pl, st) : launch_rows<NB, FP4, 1, 2>(p, pl, st);
+    return pl.nt == 1 ? launch_rows<NB, FP4, 2, 1>(p, pl, st) : launch_rows<NB, FP4, 2, 2>(p, pl, st);
 }
 template <bool FP4>
 int launch_rows(const AttentionParams& p, const Plan& pl, cudaStream_t st) {
-    if (p.c.dim <= 64) return launch_rows<2, FP4>(p, pl, st);
-    if (p.c.dim <= 128) return launch_rows<4, FP4>(p, pl, st);
-    return launch_rows<8, FP4>(p, pl, st);
+    switch (p.c.dim >> 5) {
+        case 1: return launch_rows<1, FP4>(p, pl, st);
+        case 2: return launch_rows<2, FP4>(p, pl, st);
+        case 3: return launch_rows<3, FP4>(p, pl, st);
+        case 4: return launch_rows<4, FP4>(p, pl, st);
+        case 5: return launch_rows<5, FP4>(p, pl, st);
+        case 6: return launch_rows<6, FP4>(p, pl, st);
+        case 7: return launch_rows<7, FP4>(p, pl, st);
+        default: return launch_rows<8, FP4>(p, pl, st);
+    }
 }
 
 }  // namespace
@@ -622,7 +759,7 @@ int mpt_mx_attention(const mpt_mx_cache* cache, const mpt_mx_batch* batch, const
     p.scale_log2 = (float)((double)scale * 1.4426950408889634);
     p.window = window; p.sinks = sinks;
     p.out = out; p.zero_tail = zero_tail;
-    p.tile_rows = pl.tile_rows; p.tiles_per_seq = pl.tiles_per_seq; p.splits = pl.splits;
+    p.tile_rows = pl.tile_rows; p.runs = pl.runs; p.least = kLeast;
     p.partial = static_cast<float*>(workspace);
     p.stats = p.partial + pl.partial_floats;
     cudaStream_t st = as_stream(stream);

@@ -14,9 +14,9 @@ struct AttentionParams {
     int window, sinks;
     void* out;
     int zero_tail;
-    int tile_rows, tiles_per_seq;      // rows of a tile; tiles of a sequence where all have the same number of new rows
-    int splits;                        // parts that the tokens of a row tile may be split into
-    float *partial, *stats;            // with splits: sums [tile, head, split, row, dim], and {maximum, sum} of each row
+    int tile_rows;                     // rows of a tile
+    int runs, least;                   // CTAs, and pieces of tokens that one takes at least
+    float *partial, *stats;            // of row tiles that two or more CTAs share: sums [slot, row, dim], and {maximum, sum} of each row
 };
 
 // New rows of sequence s, clamped to the rows there are.
@@ -24,36 +24,6 @@ __device__ __forceinline__ int2 rows_of(const CacheView& c, int s) {
     if (c.starts == nullptr) return make_int2(s * c.new_rows, c.new_rows);
     const int lo = min(max(__ldg(c.starts + s), 0), (int)c.rows), hi = min(max(__ldg(c.starts + s + 1), 0), (int)c.rows);
     return make_int2(lo, max(hi - lo, 0));
-}
-
-// Row tile x: its sequence and its number among the sequence's tiles; false behind the last.  Called by whole warps.
-__device__ __forceinline__ bool find_tile(const AttentionParams& p, int x, int& seq, int& tile) {
-    if (p.c.starts == nullptr) {
-        seq = x / p.tiles_per_seq;
-        tile = x - seq * p.tiles_per_seq;
-        return seq < p.c.seqs;
-    }
-    const int lane = threadIdx.x & 31;
-    int base = 0;
-    for (int s0 = 0; s0 < p.c.seqs; s0 += 32) {
-        const int s = s0 + lane;
-        const int mine = s < p.c.seqs ? (int)(((int64_t)rows_of(p.c, s).y * p.group + p.tile_rows - 1) / p.tile_rows) : 0;
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        const unsigned past = __ballot_sync(0xFFFFFFFFu, base + upto > x);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            seq = s0 + l;
-            tile = x - base - __shfl_sync(0xFFFFFFFFu, upto - mine, l);
-            return true;
-        }
-        base += __shfl_sync(0xFFFFFFFFu, upto, 31);
-    }
-    return false;
 }
 
 // The tokens that some row of a tile sees, in pieces of STEP: first those that hold sinks, then the rest from `main0`.
