@@ -29,7 +29,8 @@ NVCC_FLAGS = [
 # exactly as they do in the reference's CUDA build (nvcc defaults) to give the same bits.  So are the
 # products with packed weights and the attention, whose sums have no prescribed roundings.
 EXTRA_FLAGS = {"reduce.cu": [], "rows_softmax_fwd.cu": [], "rows_softmax_bwd.cu": [], "rows_softmax_lse.cu": [], "rows_layernorm_fwd.cu": [],
-               "rows_layernorm_bwd.cu": [], "blocklinear.cu": [], "attention.cu": []}
+               "rows_layernorm_bwd.cu": [], "blocklinear.cu": [], "attention.cu": [],
+               "attention_chunk.cu": []}
 DEFAULT_EXTRA = ["-fmad=false"]
 
 

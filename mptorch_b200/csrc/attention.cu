@@ -18,6 +18,7 @@
 #include <atomic>
 
 #include "attention.cuh"
+#include "attention_chunk.cuh"
 
 namespace mpt {
 namespace {
@@ -25,6 +26,7 @@ namespace {
 #ifndef MPT_ATT_WARPS
 #define MPT_ATT_WARPS 4
 #define MPT_ATT_LEAST 8
+#define MPT_ATT_CHUNK 40
 #endif
 constexpr int kWarps = MPT_ATT_WARPS, kTok = 32, kLeast = MPT_ATT_LEAST;
 
@@ -77,69 +79,6 @@ __host__ __device__ __forceinline__ int smem_bytes(int dim, bool fp4, int nt) {
     return cols * l.q_pitch + (ring > merge ? ring : merge);
 }
 
-// How the work is shared out.  A sequence's row tiles have `pieces` pieces of 32 tokens each (as many as its last one, or what a
-// window leaves; one at least, so that rows that see nothing are written); all pieces of all (sequence, kv head, row tile) in that
-// order are cut into equal runs, one for each CTA.  A row tile that lies in one run is finished there; of one that is cut each
-// CTA leaves its sums in a slot, which mx_attention_join_kernel joins.
-struct Work { int tiles, pieces; };            // of a sequence, for each kv head
-
-__device__ __forceinline__ Work work_of(const AttentionParams& p, int seq) {
-    Work w;
-    w.tiles = (int)(((int64_t)rows_of(p.c, seq).y * p.group + p.tile_rows - 1) / p.tile_rows);
-    const int end = min(__ldg(p.c.lens + seq), p.c.capacity());
-    int most = (end + kTok - 1) / kTok;
-    if (p.window > 0) most = (int)min((int64_t)most, ((int64_t)p.sinks + kTok - 1) / kTok + ((int64_t)p.window + p.tile_rows + kTok - 1) / kTok + 1);
-    w.pieces = max(most, 1);
-    return w;
-}
-
-// A place in the run of all pieces.
-struct Place { int seq, item, piece; Work w; };
-
-// Finds where run `run` begins (`place` means nothing behind the last one); `per`: pieces of a run; returns the number of all pieces.  Called by whole blocks of 128 threads; `sm` has room for 8 words.
-__device__ __forceinline__ int64_t find_place(const AttentionParams& p, int run, int64_t& per, Place& place, int64_t* sm) {
-    const int each = (p.c.seqs + blockDim.x - 1) / blockDim.x, s0 = min((int)threadIdx.x * each, p.c.seqs), s1 = min(s0 + each, p.c.seqs);
-    int64_t mine = 0;
-    for (int s = s0; s < s1; ++s) {
-        const Work w = work_of(p, s);
-        mine += (int64_t)w.tiles * w.pieces;
-    }
-    mine *= p.c.heads;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-        if (lane >= o) upto += v;
-    }
-    if (lane == 31) sm[warp] = upto;
-    __syncthreads();
-    int64_t before = 0, total = 0;
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) {
-        if (w < warp) before += sm[w];
-        total += sm[w];
-    }
-    upto += before;
-    per = max((total + p.runs - 1) / p.runs, (int64_t)p.least);
-    const int64_t at = run * per;
-    Place* out = reinterpret_cast<Place*>(sm + 4);
-    if (at >= upto - mine && at < upto) {
-        int64_t rest = at - (upto - mine);
-        for (int s = s0; s < s1; ++s) {
-            const Work w = work_of(p, s);
-            const int64_t all = (int64_t)w.tiles * w.pieces * p.c.heads;
-            if (rest < all) {
-                *out = Place{s, (int)(rest / w.pieces), (int)(rest % w.pieces), w};
-                break;
-            }
-            rest -= all;
-        }
-    }
-    __syncthreads();
-    place = *out;
-    return total;
-}
-
 template <int NB, bool FP4, int PIECES, int NT>
 __global__ void __launch_bounds__(32 * kWarps, NT == 1 && NB <= 4 ? 4 : NB * NT <= 8 ? 3 : 2) mx_attention_rows_kernel(const AttentionParams p) {
     constexpr int kCols = 8 * NT, kRows = kCols / PIECES, kMine = PIECES == 1 ? 2 * NT : NT;   // columns and rows of the CTA; rows that a lane holds
@@ -148,22 +87,22 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 && NB <= 4 ? 4 : NB * NT 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, tig = lane & 3;
     constexpr int dim = 32 * NB, nb = NB;
     constexpr Layout lay(dim, FP4);
-    __shared__ int64_t place_sm[9];
+    __shared__ int64_t place_sm[kPlaceWords];
     __shared__ float row_mul[kRows];
     zero_outside(p);
     Place at;
     int64_t per;
-    const int64_t total = find_place(p, blockIdx.x, per, at, place_sm);
+    const int64_t total = find_place<kTok>(p, blockIdx.x, per, at, place_sm);
     int64_t left = min(per, total - blockIdx.x * per);
     bool begins = true;                         // the segment stands at the beginning of this CTA's run
     while (left > 0) {
-    const int seq = at.seq, head = at.item / at.w.tiles, tile = at.item - head * at.w.tiles;
-    const int take = (int)min((int64_t)(at.w.pieces - at.piece), left);
+    const int seq = at.seq, head = at.head, tile = at.tile, pieces = at.w.pieces(tile);
+    const int take = (int)min((int64_t)(pieces - at.piece), left);
     const int2 own = rows_of(c, seq);
     const int first = tile * kRows, count = min(kRows, own.y * p.group - first);
     const int len = __ldg(c.lens + seq), pos0 = len - own.y;
     const TokenTiles<kTok> tt(p, pos0 + first / p.group, pos0 + (first + count - 1) / p.group);
-    const bool finished = take == at.w.pieces;
+    const bool finished = take == pieces;
     const int j_lo = min(at.piece, tt.tiles), j_hi = min(at.piece + take, tt.tiles);
 
     uint8_t* q_sm = smem;
@@ -603,56 +542,9 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 && NB <= 4 ? 4 : NB * NT 
         }
     }
     __syncthreads();
-    // ---- the next piece of the run
     left -= take;
     begins = false;
-    at.piece = 0;
-    if (left > 0 && ++at.item == at.w.tiles * c.heads) {
-        at.item = 0;
-        do { at.w = work_of(p, ++at.seq); } while (at.w.tiles == 0);
-    }
-    }
-}
-
-// Joins the row tiles that runs end in: CTA x looks at the end of run x, where run x + 1 begins.  A warp takes a row.
-__global__ void __launch_bounds__(128) mx_attention_join_kernel(const AttentionParams p) {
-    const CacheView& c = p.c;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = c.dim, nb = dim >> 5;
-    __shared__ int64_t place_sm[9];
-    Place at;
-    int64_t per;
-    const int run = blockIdx.x;
-    const int64_t total = find_place(p, run + 1, per, at, place_sm), cut = (run + 1) * per;
-    if (cut >= total || at.piece == 0) return;                     // nothing is cut here
-    const int64_t p0 = cut - at.piece, p1 = p0 + at.w.pieces;
-    if (run * per > p0) return;                                    // an earlier CTA joins this one
-    const int last = (int)((p1 - 1) / per);
-    const int head = at.item / at.w.tiles, tile = at.item - head * at.w.tiles;
-    const int2 own = rows_of(c, at.seq);
-    const int first = tile * p.tile_rows, count = min(p.tile_rows, own.y * p.group - first);
-    auto slot_of = [&](int k) { return 2 * k + (k == run && run * per < p0 ? 1 : 0); };
-    for (int r = warp; r < count; r += 4) {
-        float top = -INFINITY;
-        for (int k = run + lane; k <= last; k += 32) top = fmaxf(top, p.stats[(slot_of(k) * p.tile_rows + r) * 2]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        float sum = 0.f, v[8] = {};
-        for (int k = run; k <= last; ++k) {
-            const int slot = slot_of(k);
-            const float* st = p.stats + (slot * p.tile_rows + r) * 2;
-            const float w = st[0] == -INFINITY ? (st[1] != st[1] ? st[1] : 0.f) : exp2_fast(st[0] - top);
-            sum = fmaf(st[1], w, sum);
-            const float* from = p.partial + ((int64_t)slot * p.tile_rows + r) * dim + lane;
-#pragma unroll
-            for (int b = 0; b < 8; ++b)
-                if (b < nb) v[b] = fmaf(from[b * 32], w, v[b]);
-        }
-        const int rr = first + r, i = rr / p.group;
-        const int64_t out_row = ((int64_t)(own.x + i) * p.q_heads + head * p.group + rr - i * p.group) * dim;
-        const float inv_sum = sum == 0.f ? 0.f : __frcp_rn(sum);
-#pragma unroll
-        for (int b = 0; b < 8; ++b)
-            if (b < nb) store_value(p.out, p.dtype, out_row + b * 32 + lane, v[b] * inv_sum);
+    if (left > 0) at.next_tile<kTok>(p);
     }
 }
 
@@ -680,6 +572,27 @@ Plan make_plan(const CacheView& c, int q_heads, int dtype, int window, int sinks
     return pl;
 }
 
+// Which kernel a call takes, and the workspace it needs.
+struct CallShape {
+    bool chunk;
+    Plan rows;
+    ChunkPlan chunks;
+    size_t bytes() const {
+        return chunk ? chunks.tile_bytes + 4 * (chunks.partial_floats + chunks.stats_floats) : 4 * (rows.partial_floats + rows.stats_floats);
+    }
+};
+
+CallShape shape_of(const CacheView& c, int q_heads, int dtype, int window, int sinks) {
+    CallShape s{};
+    const int64_t per_seq = c.seqs ? c.rows * (q_heads / c.heads) / c.seqs : 0;
+    if (per_seq >= MPT_ATT_CHUNK && chunk_kernel_exists(c.dim, dtype)) {
+        s.chunks = chunk_plan(c, q_heads);
+        s.chunk = s.chunks.tile_bytes <= ((size_t)4 << 30);
+    }
+    if (!s.chunk) s.rows = make_plan(c, q_heads, dtype, window, sinks);
+    return s;
+}
+
 template <int NB, bool FP4, int PIECES, int NT>
 int launch_rows(AttentionParams p, const Plan& pl, cudaStream_t st) {
     const int bytes = smem_bytes(p.c.dim, FP4, NT);
@@ -700,7 +613,7 @@ int launch_rows(AttentionParams p, const Plan& pl, cudaStream_t st) {
     const int most = fit * sm_count();
     p.runs = pl.runs < most ? pl.runs : most;
     kern<<<(unsigned)p.runs, 32 * kWarps, bytes, st>>>(p);
-    if (p.runs > 1) mx_attention_join_kernel<<<(unsigned)(p.runs - 1), 128, 0, st>>>(p);
+    if (p.runs > 1) mx_attention_join_kernel<kTok><<<(unsigned)(p.runs - 1), 128, 0, st>>>(p);
     return check_launch("mx_attention");
 }
 
@@ -733,8 +646,7 @@ extern "C" {
 size_t mpt_mx_attention_workspace_bytes(const mpt_mx_cache* cache, const mpt_mx_batch* batch, int q_heads, int dtype, int window, int sinks) {
     CacheView c;
     if (!convert_cache("mx_attention", cache, batch, &c) || q_heads < 1 || q_heads % c.heads || c.rows == 0) return 0;
-    const Plan pl = make_plan(c, q_heads, dtype, window, sinks);
-    return 4 * (pl.partial_floats + pl.stats_floats);
+    return shape_of(c, q_heads, dtype, window, sinks).bytes();
 }
 
 int mpt_mx_attention(const mpt_mx_cache* cache, const mpt_mx_batch* batch, const void* q, int dtype, const int64_t* q_strides, int q_heads, float scale,
@@ -748,22 +660,32 @@ int mpt_mx_attention(const mpt_mx_cache* cache, const mpt_mx_batch* batch, const
     if (c.rows == 0) return MPT_OK;
     MPT_REQUIRE(q && q_strides && out, "mx_attention: null pointer");
     MPT_REQUIRE(c.rows * q_heads <= 0x7FFFFFFF, "mx_attention: more than 2^31 - 1 rows of heads");
-    const Plan pl = make_plan(c, q_heads, dtype, window, sinks);
-    if (workspace_bytes < 4 * (pl.partial_floats + pl.stats_floats) || (pl.partial_floats && !workspace) || ((uintptr_t)workspace & 15u)) {
-        set_error("mx_attention: a workspace of %zu bytes at a multiple of 256 is needed", 4 * (pl.partial_floats + pl.stats_floats));
+    const CallShape call = shape_of(c, q_heads, dtype, window, sinks);
+    if (workspace_bytes < call.bytes() || !workspace || ((uintptr_t)workspace & 255u)) {
+        set_error("mx_attention: a workspace of %zu bytes at a multiple of 256 is needed", call.bytes());
         return MPT_ERR_WORKSPACE;
     }
+    const int64_t size = dtype == MPT_DTYPE_F32 ? 4 : 2;
     p.q = q; p.dtype = dtype;
     p.q_seq = q_strides[0]; p.q_row = q_strides[1]; p.q_head = q_strides[2];
+    p.q_vec = (((int64_t)(uintptr_t)q | size * (p.q_row | p.q_head | (c.starts ? 0 : p.q_seq))) & 15) == 0;
+    p.out_vec = ((uintptr_t)out & 15u) == 0;
     p.q_heads = q_heads; p.group = q_heads / c.heads;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634);
     p.window = window; p.sinks = sinks;
     p.out = out; p.zero_tail = zero_tail;
-    p.tile_rows = pl.tile_rows; p.runs = pl.runs; p.least = kLeast;
-    p.partial = static_cast<float*>(workspace);
-    p.stats = p.partial + pl.partial_floats;
     cudaStream_t st = as_stream(stream);
-    return cache->elem_format == MPT_ELEM_E2M1 ? launch_rows<true>(p, pl, st) : launch_rows<false>(p, pl, st);
+    const bool fp4 = cache->elem_format == MPT_ELEM_E2M1;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    if (call.chunk) {
+        p.partial = reinterpret_cast<float*>(ws + call.chunks.tile_bytes);
+        p.stats = p.partial + call.chunks.partial_floats;
+        return launch_chunk(p, call.chunks, ws, fp4, st);
+    }
+    p.tile_rows = call.rows.tile_rows; p.least = kLeast;
+    p.partial = reinterpret_cast<float*>(ws);
+    p.stats = p.partial + call.rows.partial_floats;
+    return fp4 ? launch_rows<true>(p, call.rows, st) : launch_rows<false>(p, call.rows, st);
 }
 
 }

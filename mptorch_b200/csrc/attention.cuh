@@ -9,6 +9,7 @@ struct AttentionParams {
     const void* q;
     int dtype;
     int64_t q_seq, q_row, q_head;      // element strides of q
+    bool q_vec, out_vec;               // rows of q, of out, begin at multiples of 16 bytes
     int q_heads, group;                // query heads, query heads of a kv head
     float scale_log2;                  // scale * log2(e)
     int window, sinks;
@@ -48,6 +49,120 @@ __device__ __forceinline__ bool sees(const AttentionParams& p, int pos, int t) {
     return t <= pos && (p.window <= 0 || t > pos - p.window || t < p.sinks);
 }
 
+// How the work is shared out.  Row tile t of a sequence has as many pieces of STEP tokens as its last row sees, one at least (so
+// that rows that see nothing are written); the pieces of all (sequence, kv head, row tile) in that order are cut into equal
+// runs, one for each CTA.  A row tile that lies in one run is finished there; of one that is cut each CTA leaves its sums in a
+// slot, which mx_attention_join_kernel joins.
+//
+// Without a window row tile t ends at position pos0 + (R (t + 1) - 1) / G (R rows a tile, G query heads a kv head); with
+// pos0 = STEP a + b that makes a + 1 + floor((t + 1 + c) / g) pieces, g = STEP G / R, c = floor((b G - 1) / R), and sums of it
+// over t are closed.  With a window, with rows before the first token or with more tokens than places every tile counts the same.
+struct Work {
+    int tiles, base, c, g;                     // of a sequence, for each kv head; g: 0 where all tiles count `base`
+    __device__ __forceinline__ int pieces(int t) const { return g ? base + (t + 1 + c) / g : base; }
+    __device__ __forceinline__ int64_t upto(int t) const {        // pieces of the tiles before t
+        if (g == 0) return (int64_t)t * base;
+        return (int64_t)t * base + steps(t + 1 + c) - steps(1 + c);
+    }
+    __device__ __forceinline__ int64_t steps(int m) const {       // sum of floor(i / g) over i < m
+        const int64_t q = m / g;
+        return g * (q * (q - 1) / 2) + q * (m - q * g);
+    }
+};
+
+template <int STEP>
+__device__ __forceinline__ Work work_of(const AttentionParams& p, int seq) {
+    Work w;
+    const int n = rows_of(p.c, seq).y, len = __ldg(p.c.lens + seq), pos0 = len - n, end = min(len, p.c.capacity());
+    w.tiles = (int)(((int64_t)n * p.group + p.tile_rows - 1) / p.tile_rows);
+    w.c = w.g = 0;
+    if (p.window > 0) {
+        const int64_t most = ((int64_t)p.sinks + STEP - 1) / STEP + ((int64_t)p.window + p.tile_rows + STEP - 1) / STEP + 1;
+        w.base = (int)max(min((int64_t)(end + STEP - 1) / STEP, most), (int64_t)1);
+    } else if (pos0 < 0 || len > end) {
+        w.base = max((end + STEP - 1) / STEP, 1);
+    } else {
+        w.base = pos0 / STEP + 1;
+        const int bg = pos0 % STEP * p.group;
+        w.c = bg ? (bg - 1) / p.tile_rows : -1;
+        w.g = STEP * p.group / p.tile_rows;
+    }
+    return w;
+}
+
+// A place in the run of all pieces.
+struct Place {
+    int seq, head, tile, piece;
+    Work w;
+    template <int STEP>
+    __device__ __forceinline__ void next_tile(const AttentionParams& p) {
+        piece = 0;
+        if (++tile < w.tiles) return;
+        tile = 0;
+        if (++head < p.c.heads) return;
+        head = 0;
+        do { w = work_of<STEP>(p, ++seq); } while (w.tiles == 0);
+    }
+};
+
+constexpr int kPlaceWords = 8 + (sizeof(Place) + 7) / 8;
+
+// Finds where run `run` begins (`place` means nothing behind the last one); `per`: pieces of a run; returns the number of all
+// pieces.  Called by whole blocks of up to 256 threads; `sm` has room for kPlaceWords.
+template <int STEP>
+__device__ __forceinline__ int64_t find_place(const AttentionParams& p, int run, int64_t& per, Place& place, int64_t* sm) {
+    const int each = (p.c.seqs + blockDim.x - 1) / blockDim.x, s0 = min((int)threadIdx.x * each, p.c.seqs), s1 = min(s0 + each, p.c.seqs);
+    int64_t mine = 0;
+    for (int s = s0; s < s1; ++s) {
+        const Work w = work_of<STEP>(p, s);
+        mine += w.upto(w.tiles);
+    }
+    mine *= p.c.heads;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) sm[warp] = upto;
+    __syncthreads();
+    int64_t before = 0, total = 0;
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) {
+        if (w < warp) before += sm[w];
+        total += sm[w];
+    }
+    upto += before;
+    per = max((total + p.runs - 1) / p.runs, (int64_t)p.least);
+    const int64_t at = run * per;
+    Place* out = reinterpret_cast<Place*>(sm + 8);
+    if (at >= upto - mine && at < upto) {
+        int64_t rest = at - (upto - mine);
+        for (int s = s0; s < s1; ++s) {
+            const Work w = work_of<STEP>(p, s);
+            const int64_t head = w.upto(w.tiles);
+            if (rest < head * p.c.heads) {
+                out->seq = s;
+                out->head = (int)(rest / head);
+                rest %= head;
+                int lo = 0, hi = w.tiles - 1;                      // the last tile that begins at or before it
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) >> 1;
+                    if (w.upto(mid) <= rest) lo = mid; else hi = mid - 1;
+                }
+                out->tile = lo;
+                out->piece = (int)(rest - w.upto(lo));
+                out->w = w;
+                break;
+            }
+            rest -= head * p.c.heads;
+        }
+    }
+    __syncthreads();
+    place = *out;
+    return total;
+}
+
 // Rows that belong to no sequence: zeros, where the output is this library's own.
 template <typename T>
 __device__ __forceinline__ void zero_rows(const AttentionParams& p, int64_t lo, int64_t hi) {
@@ -82,6 +197,48 @@ __device__ __forceinline__ float exp2_fast(float x) {       // relative error 2^
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Joins the row tiles that runs end in: CTA x looks at the end of run x, where run x + 1 begins.  A warp takes a row.
+template <int STEP>
+__global__ void __launch_bounds__(128) mx_attention_join_kernel(const AttentionParams p) {
+    const CacheView& c = p.c;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = c.dim, nb = dim >> 5;
+    __shared__ int64_t place_sm[kPlaceWords];
+    Place at;
+    int64_t per;
+    const int run = blockIdx.x;
+    const int64_t total = find_place<STEP>(p, run + 1, per, at, place_sm), cut = (run + 1) * per;
+    if (cut >= total || at.piece == 0) return;                     // nothing is cut here
+    const int64_t p0 = cut - at.piece, p1 = p0 + at.w.pieces(at.tile);
+    if (run * per > p0) return;                                    // an earlier CTA joins this one
+    const int last = (int)((p1 - 1) / per);
+    const int2 own = rows_of(c, at.seq);
+    const int first = at.tile * p.tile_rows, count = min(p.tile_rows, own.y * p.group - first);
+    auto slot_of = [&](int k) { return 2 * k + (k == run && run * per < p0 ? 1 : 0); };
+    for (int r = warp; r < count; r += 4) {
+        float top = -INFINITY;
+        for (int k = run + lane; k <= last; k += 32) top = fmaxf(top, p.stats[(slot_of(k) * p.tile_rows + r) * 2]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        float sum = 0.f, v[8] = {};
+        for (int k = run; k <= last; ++k) {
+            const int slot = slot_of(k);
+            const float* st = p.stats + (slot * p.tile_rows + r) * 2;
+            const float w = st[0] == -INFINITY ? (st[1] != st[1] ? st[1] : 0.f) : exp2_fast(st[0] - top);   // a NaN sum stays one
+            sum = fmaf(st[1], w, sum);
+            const float* from = p.partial + ((int64_t)slot * p.tile_rows + r) * dim + lane;
+#pragma unroll
+            for (int b = 0; b < 8; ++b)
+                if (b < nb) v[b] = fmaf(from[b * 32], w, v[b]);
+        }
+        const int rr = first + r, i = rr / p.group;
+        const int64_t out_row = ((int64_t)(own.x + i) * p.q_heads + at.head * p.group + rr - i * p.group) * dim;
+        const float inv_sum = sum == 0.f ? 0.f : __frcp_rn(sum);
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+            if (b < nb) store_value(p.out, p.dtype, out_row + b * 32 + lane, v[b] * inv_sum);
+    }
 }
 
 }  // namespace mpt
