@@ -613,7 +613,7 @@ int launch_rows(AttentionParams p, const Plan& pl, cudaStream_t st) {
     const int most = fit * sm_count();
     p.runs = pl.runs < most ? pl.runs : most;
     kern<<<(unsigned)p.runs, 32 * kWarps, bytes, st>>>(p);
-    if (p.runs > 1) mx_attention_join_kernel<kTok><<<(unsigned)(p.runs - 1), 128, 0, st>>>(p);
+    if (p.runs > 1) mx_attention_join_kernel<kTok><<<dim3((unsigned)(p.runs - 1), (unsigned)(p.tile_rows + 7) / 8), 128, 0, st>>>(p);
     return check_launch("mx_attention");
 }
 

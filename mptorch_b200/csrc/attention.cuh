@@ -199,7 +199,8 @@ __device__ __forceinline__ float exp2_fast(float x) {       // relative error 2^
     return y;
 }
 
-// Joins the row tiles that runs end in: CTA x looks at the end of run x, where run x + 1 begins.  A warp takes a row.
+// Joins the row tiles that runs end in: CTAs (x, .) look at the end of run x, where run x + 1 begins.  A warp
+// takes a row.
 template <int STEP>
 __global__ void __launch_bounds__(128) mx_attention_join_kernel(const AttentionParams p) {
     const CacheView& c = p.c;
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(128) mx_attention_join_kernel(const AttentionP
     const int2 own = rows_of(c, at.seq);
     const int first = at.tile * p.tile_rows, count = min(p.tile_rows, own.y * p.group - first);
     auto slot_of = [&](int k) { return 2 * k + (k == run && run * per < p0 ? 1 : 0); };
-    for (int r = warp; r < count; r += 4) {
+    for (int r = warp + 4 * blockIdx.y; r < count; r += 4 * gridDim.y) {
         float top = -INFINITY;
         for (int k = run + lane; k <= last; k += 32) top = fmaxf(top, p.stats[(slot_of(k) * p.tile_rows + r) * 2]);
 #pragma unroll

@@ -4,7 +4,7 @@
 // clock on an SM).  Two kernels.  The first expands the sequences' K and V into bfloat16, where a code times its scale is exact, as
 // tiles of 128 tokens in the very layout that the second one's operands have in shared memory, so that a tile is one bulk copy: it
 // costs one pass over the cache (a byte read and two written an element), where expanding inside the second kernel would repeat it
-// for every 128 rows.  The second is a warp that copies, a warp that issues products, and four warps with a row a thread:
+// for every 128 rows.  The second is a warp that copies, a warp that issues products, and eight warps with half a row a thread:
 //   S = Q K^T (tensor memory) -> p = exp(s - m) as bfloat16 over S's own columns -> O += P V, P read from tensor memory.
 // m is moved, and O multiplied, only when a row's maximum has grown by more than 2^8 over it; p is at most 2^8 then.
 //
@@ -34,6 +34,12 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 __device__ __forceinline__ float bf16_lo(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t x) { return __uint_as_float(x & 0xFFFF0000u); }
+
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }   // the lowest n bits
+__device__ __forceinline__ uint32_t opaque(uint32_t x) {
+    asm volatile("" : "+r"(x));
+    return x;
+}
 
 // ---- expanding.  One CTA for 128 tokens of a (sequence, kv head).
 template <bool FP4>
@@ -97,21 +103,23 @@ __global__ void __launch_bounds__(256) mx_expand_kernel(const AttentionParams p,
 }
 
 // ---- attention
-constexpr int kThreads = 192;                                     // four warps of rows, one that copies, one that issues products
+constexpr int kRowThreads = 256, kThreads = kRowThreads + 64;     // two threads a row, each with half of the tokens; a warp that copies, one that issues products
 enum { kKFull, kKEmpty, kVFull, kVEmpty, kScores, kScores2, kWeights, kWeights2, kValues, kBars };
 
 template <int DIM, int PIECES, int NS>
 struct ChunkShape {
     static constexpr int parts = parts_for(DIM), q_bytes = PIECES * parts * kPart, side = parts * kPart;
     static constexpr int smem = 1024 + q_bytes + 2 * side + 4 * kTrailer;
-    // columns of tensor memory: scores (a set for each of NS), sums, and weights that do not fit over the scores
-    static constexpr int sums = NS * 128, more = sums + DIM, used = more + (PIECES == 3 ? 64 * NS : 0), columns = used <= 256 ? 256 : 512;
+    // columns of tensor memory: scores (a set for each of NS), sums, and for three pieces sums of the smaller ones (so that the tensor
+    // cores, which cut sums off, do so with the large sums once a product and not three times) and weights that do not fit over the scores
+    static constexpr int sums = NS * 128, small = sums + DIM, more = small + (PIECES == 3 ? DIM : 0), used = more + (PIECES == 3 ? 64 * NS : 0);
+    static constexpr int columns = used <= 256 ? 256 : 512;
     static_assert(used <= 512, "tensor memory");
     static_assert(smem <= 227 * 1024, "shared memory");
 };
 
 template <int DIM, int PIECES, int NS>
-__global__ void __launch_bounds__(kThreads, NS == 1 ? 2 : 1) mx_attention_chunk_kernel(const AttentionParams p, const uint8_t* __restrict__ tiles, int tiles_per_seq) {
+__global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_attention_chunk_kernel(const AttentionParams p, const uint8_t* __restrict__ tiles, int tiles_per_seq) {
     using Shape = ChunkShape<DIM, PIECES, NS>;
     extern __shared__ uint8_t smem_raw[];
     const CacheView& c = p.c;
@@ -123,6 +131,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 ? 2 : 1) mx_attention_chunk_
     __shared__ int64_t place_sm[kPlaceWords];
     __shared__ __align__(8) uint64_t bars[kBars];
     __shared__ uint32_t tmem_slot, failed;
+    __shared__ float tops[2][kTile], sums_sm[kTile];
 
     zero_outside(p);
     Place at;
@@ -132,12 +141,13 @@ __global__ void __launch_bounds__(kThreads, NS == 1 ? 2 : 1) mx_attention_chunk_
     if (left <= 0) return;
 
     auto bar = [&](int i) { return smem_at(&bars[i]); };
+    auto wait = [&](int i, uint32_t parity) { return bar_wait(bar(i), parity & 1u, &failed); };
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kBars; ++i) bar_init(bar(i), i == kWeights || i == kWeights2 ? 128 : 1);
+        for (int i = 0; i < kBars; ++i) bar_init(bar(i), i == kWeights || i == kWeights2 ? kRowThreads : 1);
         failed = 0u;
         fence_barrier_init();
     }
-    if (warp == 5) tmem_alloc(smem_at(&tmem_slot), Shape::columns);
+    if (warp == 9) tmem_alloc(smem_at(&tmem_slot), Shape::columns);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
@@ -159,6 +169,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 ? 2 : 1) mx_attention_chunk_
         const int j_lo = min(at.piece, tt.tiles), n = min(at.piece + take, tt.tiles) - j_lo;
 
         // ---- q, in pieces
+#pragma unroll 1
         for (int i = threadIdx.x; i < kTile * (DIM / 8); i += kThreads) {
             const int r = i / (DIM / 8), ch = i - r * (DIM / 8);
             float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -190,37 +201,40 @@ __global__ void __launch_bounds__(kThreads, NS == 1 ? 2 : 1) mx_attention_chunk_
         fence_async_proxy();
         __syncthreads();
 
-        if (warp == 4) {
+        if (warp == 8) {
             if (lane == 0) {
                 const uint8_t* from = tiles + ((int64_t)seq * c.heads + head) * tiles_per_seq * tile_bytes(DIM);
                 for (int i = 0; i < n; ++i) {
                     const uint32_t it = it0 + i;
                     const uint8_t* src = from + (int64_t)(tt.start(j_lo + i) / kTile) * tile_bytes(DIM);
-                    if (it > 0 && !bar_wait(bar(kKEmpty), (it - 1) & 1)) { failed = 1u; break; }
+                    if (it > 0 && !wait(kKEmpty, it - 1)) break;
                     bar_expect(bar(kKFull), Shape::side + kTrailer);
                     bulk_load(k_at, src, Shape::side, bar(kKFull));
                     bulk_load(tail_at + (it & 3) * kTrailer, src + 2 * Shape::side, kTrailer, bar(kKFull));
-                    if (it > 0 && !bar_wait(bar(kVEmpty), (it - 1) & 1)) { failed = 1u; break; }
+                    if (it > 0 && !wait(kVEmpty, it - 1)) break;
                     bar_expect(bar(kVFull), Shape::side);
                     bulk_load(v_at, src + Shape::side, Shape::side, bar(kVFull));
                 }
             }
             __syncwarp();
-        } else if (warp == 5) {
+        } else if (warp == 9) {
             if (lane == 0) {
                 constexpr uint32_t score_desc = product_descriptor(128, false), value_desc = product_descriptor(DIM, true);
                 auto scores = [&](int i) -> bool {
                     const uint32_t it = it0 + i;
-                    if (!bar_wait(bar(kKFull), it & 1)) return false;
+                    if (!wait(kKFull, it)) return false;
                     // the columns are free when the product that read the weights in them is done (the segment before is done)
-                    if (i >= NS && !bar_wait(bar(kValues), (it - NS) & 1)) return false;
+                    if (i >= NS && !wait(kValues, it - NS)) return false;
                     tmem_fence_after();
+                    // (addresses are opaque to the compiler, which would keep every descriptor in registers of its own)
+                    const uint64_t q_desc = tile_descriptor(opaque(q_at), 16), k_desc = tile_descriptor(opaque(k_at), 16);
+                    const uint32_t to = tmem + (NS == 2 ? (it & 1) * 128 : 0);
 #pragma unroll
                     for (int k = 0; k < PIECES; ++k)
 #pragma unroll
                         for (int s = 0; s < DIM / 16; ++s)
-                            mma_ss(tmem + (NS == 2 ? (it & 1) * 128 : 0), tile_descriptor(q_at + (k * Shape::parts + (s >> 2)) * kPart + (s & 3) * 32, 16),
-                                   tile_descriptor(k_at + (s >> 2) * kPart + (s & 3) * 32, 16), score_desc, k + s > 0);
+                            mma_ss(to, q_desc + (((k * Shape::parts + (s >> 2)) * kPart + (s & 3) * 32) >> 4), k_desc + (((s >> 2) * kPart + (s & 3) * 32) >> 4), score_desc,
+                                   k + s > 0);
                     mma_commit(bar(NS == 2 && (it & 1) ? kScores2 : kScores));
                     mma_commit(bar(kKEmpty));
                     return true;
@@ -230,56 +244,55 @@ __global__ void __launch_bounds__(kThreads, NS == 1 ? 2 : 1) mx_attention_chunk_
                     const uint32_t it = it0 + i;
                     if (NS == 2 && i + 1 < n && !(ok = scores(i + 1))) break;
                     const uint32_t turn = NS == 2 ? it & 1 : 0;
-                    if (!(ok = bar_wait(bar(turn ? kWeights2 : kWeights), NS == 2 ? (it >> 1) & 1 : it & 1))) break;
-                    if (!(ok = bar_wait(bar(kVFull), it & 1))) break;
+                    if (!(ok = wait(turn ? kWeights2 : kWeights, NS == 2 ? it >> 1 : it))) break;
+                    if (!(ok = wait(kVFull, it))) break;
                     tmem_fence_after();
+                    const uint64_t v_desc = tile_descriptor(opaque(v_at), kPart);
 #pragma unroll
                     for (int k = 0; k < PIECES; ++k) {
                         const uint32_t w = tmem + (k < 2 ? turn * 128 + k * 64 : Shape::more + turn * 64);
 #pragma unroll
                         for (int s = 0; s < 8; ++s)
-                            mma_ts(tmem + Shape::sums, w + s * 8, tile_descriptor(v_at + s * 2048, kPart), value_desc, i > 0 || k + s > 0);
+                            mma_ts(tmem + (PIECES == 3 && k > 0 ? Shape::small : Shape::sums), w + s * 8, v_desc + (s * 2048 >> 4), value_desc,
+                                   i > 0 || s > 0 || k > (PIECES == 3 ? 1 : 0));
                     }
                     mma_commit(bar(kValues));
                     mma_commit(bar(kVEmpty));
                     if (NS == 1 && i + 1 < n) ok = scores(i + 1);
                 }
-                if (!ok) failed = 1u;
             }
             __syncwarp();
         } else {
-            const int r = threadIdx.x;                            // this thread's row
-            const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+            const int half = warp >> 2, r = threadIdx.x & (kTile - 1);   // this thread's row, and its half of the tokens
+            const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
             const int pos = r < count ? pos0 + (first + r) / p.group : -1;
             float m = -INFINITY, l = 0.f;
             uint32_t poison = 0u;
-            bool ok = true;
             for (int i = 0; i < n; ++i) {
                 const uint32_t it = it0 + i, turn = NS == 2 ? it & 1 : 0, set = turn * 128;
-                ok = bar_wait(bar(turn ? kScores2 : kScores), NS == 2 ? (it >> 1) & 1 : it & 1);
-                if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+                wait(turn ? kScores2 : kScores, NS == 2 ? it >> 1 : it);
+                __syncwarp();
                 tmem_fence_after();
+                uint32_t s[64];
+                tmem_load32(mine + set + 64 * half, s);
+                tmem_load32(mine + set + 64 * half + 32, s + 32);
                 const uint32_t* tail = reinterpret_cast<const uint32_t*>(tails + (it & 3) * kTrailer);
                 const int t0 = tt.start(j_lo + i);
                 const uint4 there = *reinterpret_cast<const uint4*>(tail);
+                const uint32_t any_nan = tail[4];
                 const bool whole = (there.x & there.y & there.z & there.w) == 0xFFFFFFFFu && t0 + kTile - 1 <= low_pos && (p.window <= 0 || t0 > high_pos - p.window);
-                const int upto = pos - t0, from = p.window > 0 ? pos - p.window - t0 : -1, sinks = p.sinks - t0;
-                uint32_t s[64];                                   // half of the row's scores
-                auto load = [&](int half) {
-                    tmem_load32(mine + set + 64 * half, s);
-                    tmem_load32(mine + set + 64 * half + 32, s + 32);
-                    tmem_wait_load();
-                    if (!whole) {
+                tmem_wait_load();
+                if (!whole) {
+                    const int t1 = t0 + 64 * half, from = p.window > 0 ? pos - p.window + 1 - t1 : 0, sinks = p.window > 0 ? p.sinks - t1 : 0;
+                    uint32_t seen[2];
 #pragma unroll
-                        for (int k = 0; k < 64; ++k) {
-                            const int col = 64 * half + k;
-                            const uint32_t word = half == 0 ? (k < 32 ? there.x : there.y) : (k < 32 ? there.z : there.w);
-                            const bool on = col <= upto && (col > from || col < sinks) && ((word >> (k & 31)) & 1u);
-                            s[k] = on ? s[k] : 0xFF800000u;
-                        }
-                    }
-                };
-                if (tail[4]) {                                    // V holds blocks that are NaN
+                    for (int w = 0; w < 2; ++w)
+                        seen[w] = (half ? (w ? there.w : there.z) : (w ? there.y : there.x)) & below(pos + 1 - t1 - 32 * w) &
+                                  (~below(from - 32 * w) | below(sinks - 32 * w));
+#pragma unroll
+                    for (int k = 0; k < 64; ++k) s[k] = (seen[k >> 5] >> (k & 31)) & 1u ? s[k] : 0xFF800000u;
+                }
+                if (any_nan) {                                    // V holds blocks that are NaN
                     for (int k = 0; k < kTile; ++k) {
                         const uint32_t blocks = reinterpret_cast<const uint8_t*>(tail)[32 + k];
                         if (blocks && sees(p, pos, t0 + k)) poison |= blocks;
@@ -287,89 +300,104 @@ __global__ void __launch_bounds__(kThreads, NS == 1 ? 2 : 1) mx_attention_chunk_
                 }
                 float top = -INFINITY, top2 = -INFINITY;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    load(half);
-#pragma unroll
-                    for (int k = 0; k < 64; k += 2) {
-                        top = fmaxf(top, __uint_as_float(s[k]));
-                        top2 = fmaxf(top2, __uint_as_float(s[k + 1]));
-                    }
+                for (int k = 0; k < 64; k += 2) {
+                    top = fmaxf(top, __uint_as_float(s[k]));
+                    top2 = fmaxf(top2, __uint_as_float(s[k + 1]));
                 }
-                top = fmaxf(top, top2) * mul;
+                top = fmaxf(top, top2);
+                // the other half's; from here on the scores' columns are free
+                tops[half][r] = top;
+                tmem_fence_before();
+                asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads) : "memory");
+                tmem_fence_after();
+                top = fmaxf(top, tops[half ^ 1][r]) * mul;
                 if (__any_sync(0xFFFFFFFFu, top > m + 8.f)) {
                     const float next = fmaxf(m, top), fade = next == -INFINITY ? 1.f : exp2_fast(m - next);
                     m = next;
                     l *= fade;
                     if (i > 0) {
-                        ok = bar_wait(bar(kValues), (it - 1) & 1);
-                        if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; break; }
+                        wait(kValues, it - 1);
+                        __syncwarp();
                         tmem_fence_after();
+                        // the halves take blocks of 16 columns in turn; few registers are free here
+                        for (int b = 16 * half; b < DIM; b += 32) {
+                            uint32_t o[16];
 #pragma unroll
-                        for (int b = 0; b < DIM; b += 32) {
-                            uint32_t o[32];
-                            tmem_load32(mine + Shape::sums + b, o);
-                            tmem_wait_load();
+                            for (int side = 0; side < (PIECES == 3 ? 2 : 1); ++side) {
+                                const uint32_t where = mine + (side ? Shape::small : Shape::sums) + b;
+                                tmem_load16(where, o);
+                                tmem_wait_load();
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fade);
-                            tmem_store32(mine + Shape::sums + b, o);
+                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fade);
+                                tmem_store16(where, o);
+                            }
                         }
                     }
                 }
                 const float base = m == -INFINITY ? 0.f : m;
-                // the first half's weights lie over its scores; its second pieces over the second half's scores, once these are read
-                uint32_t w2[2][32];
+                float sum = 0.f, sum2 = 0.f;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    load(half);
-                    if (PIECES > 1 && half == 1) tmem_store32(mine + set + 64, w2[0]);
-                    uint32_t w[32], w3[32];
-                    float sum = 0.f, sum2 = 0.f;
+                for (int k = 0; k < 64; k += 32) {
+                    uint32_t w[16], w2[16], w3[16];
 #pragma unroll
-                    for (int e = 0; e < 64; e += 2) {
-                        float a = exp2_fast(fmaf(__uint_as_float(s[e]), mul, -base)), b = exp2_fast(fmaf(__uint_as_float(s[e + 1]), mul, -base));
+                    for (int e = 0; e < 32; e += 2) {
+                        float a = exp2_fast(fmaf(__uint_as_float(s[k + e]), mul, -base)), b = exp2_fast(fmaf(__uint_as_float(s[k + e + 1]), mul, -base));
                         sum += a;
                         sum2 += b;
                         w[e >> 1] = pack_bf16(a, b);
                         if (PIECES > 1) {
                             a -= bf16_lo(w[e >> 1]);
                             b -= bf16_hi(w[e >> 1]);
-                            w2[half][e >> 1] = pack_bf16(a, b);
+                            w2[e >> 1] = pack_bf16(a, b);
                         }
-                        if (PIECES > 2) w3[e >> 1] = pack_bf16(a - bf16_lo(w2[half][e >> 1]), b - bf16_hi(w2[half][e >> 1]));
+                        if (PIECES > 2) w3[e >> 1] = pack_bf16(a - bf16_lo(w2[e >> 1]), b - bf16_hi(w2[e >> 1]));
                     }
-                    l += sum + sum2;
-                    tmem_store32(mine + set + 32 * half, w);
-                    if (PIECES > 1 && half == 1) tmem_store32(mine + set + 96, w2[1]);
-                    if (PIECES > 2) tmem_store32(mine + Shape::more + turn * 64 + 32 * half, w3);
+                    const uint32_t to = mine + 32 * half + (k >> 1);
+                    tmem_store16(to + set, w);
+                    if (PIECES > 1) tmem_store16(to + set + 64, w2);
+                    if (PIECES > 2) tmem_store16(to + Shape::more + turn * 64, w3);
                 }
+                l += sum + sum2;
                 tmem_wait_store();
                 tmem_fence_before();
                 bar_arrive(bar(turn ? kWeights2 : kWeights));
             }
-            if (ok && n > 0) ok = bar_wait(bar(kValues), (it0 + n - 1) & 1);
-            if (!__all_sync(0xFFFFFFFFu, ok)) { ok = false; failed = 1u; }
+            if (n > 0) wait(kValues, it0 + n - 1);
+            if (half) sums_sm[r] = l;
+            __syncwarp();
+            asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads) : "memory");
             tmem_fence_after();
+            if (!half) sums_sm[r] = l += sums_sm[r];
+            asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads) : "memory");
+            l = sums_sm[r];
+            const bool ok = *(volatile uint32_t*)&failed == 0u;
             // ---- the row's result, or its share
             const int rr = first + r, tok = rr / p.group;
             const int64_t out_row = ((int64_t)(own.x + tok) * p.q_heads + head * p.group + rr - tok * p.group) * DIM;
             const int share = 2 * blockIdx.x + (begins ? 0 : 1);
             const float times = !ok ? __uint_as_float(0x7FC00000u) : finished ? (l == 0.f ? 0.f : __frcp_rn(l)) : 1.f;
-#pragma unroll
-            for (int b = 0; b < DIM; b += 32) {
-                uint32_t o[32];
-                if (n > 0) {
-                    tmem_load32(mine + Shape::sums + b, o);
+#pragma unroll 1
+            for (int b = 16 * half; b < DIM; b += 32) {           // the halves take blocks of 16 columns in turn
+                uint32_t o[16];
+                tmem_load16(mine + Shape::sums + b, o);
+                tmem_wait_load();
+                if (PIECES == 3) {
+                    uint32_t o2[16];
+                    tmem_load16(mine + Shape::small + b, o2);
                     tmem_wait_load();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) + __uint_as_float(o2[k]));
                 }
                 if (r < count) {
                     const bool bad = (poison >> (b >> 5)) & 1u;
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
+                    for (int k = 0; k < 16; k += 8) {
                         float v[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = bad ? __uint_as_float(0x7FC00000u) : (n > 0 ? __uint_as_float(o[k + e]) : 0.f) * times;
-                        if (!finished) store8(p.partial + ((int64_t)share * kTile + r) * DIM + b + k, v);
-                        else if (p.out_vec) {
+                        for (int e = 0; e < 8; ++e) v[e] = bad ? __uint_as_float(0x7FC00000u) : n > 0 ? __uint_as_float(o[k + e]) * times : 0.f;
+                        if (!finished) {
+                            store8(p.partial + ((int64_t)share * kTile + r) * DIM + b + k, v);
+                        } else if (p.out_vec) {
                             if (PIECES == 3) store8(static_cast<float*>(p.out) + out_row + b + k, v);
                             else if (PIECES == 2) store8(static_cast<__half*>(p.out) + out_row + b + k, v);
                             else store8(static_cast<__nv_bfloat16*>(p.out) + out_row + b + k, v);
@@ -379,8 +407,9 @@ __global__ void __launch_bounds__(kThreads, NS == 1 ? 2 : 1) mx_attention_chunk_
                         }
                     }
                 }
+                __syncwarp();
             }
-            if (!finished && r < count) {
+            if (!finished && !half && r < count) {
                 p.stats[(share * kTile + r) * 2] = m;
                 p.stats[(share * kTile + r) * 2 + 1] = l;
             }
@@ -394,12 +423,13 @@ __global__ void __launch_bounds__(kThreads, NS == 1 ? 2 : 1) mx_attention_chunk_
         begins = false;
         if (left > 0) at.next_tile<kTile>(p);
     }
-    if (failed && warp == 4 && lane == 0) {                       // copies on the way write to this CTA's memory
-        bar_wait(bar(kKFull), 0); bar_wait(bar(kKFull), 1);
-        bar_wait(bar(kVFull), 0); bar_wait(bar(kVFull), 1);
+    if (failed && warp == 8 && lane == 0) {                       // copies on the way write to this CTA's memory
+        failed = 0u;
+        wait(kKFull, 0); wait(kKFull, 1);
+        wait(kVFull, 0); wait(kVFull, 1);
     }
     __syncthreads();
-    if (warp == 5) tmem_free(tmem, Shape::columns);
+    if (warp == 9) tmem_free(tmem, Shape::columns);
 }
 
 template <int DIM, int PIECES, int NS>
@@ -422,7 +452,7 @@ int launch(AttentionParams p, const ChunkPlan& pl, uint8_t* tiles, cudaStream_t 
     }
     p.runs = pl.runs < fit * sm_count() ? pl.runs : fit * sm_count();
     kern<<<(unsigned)p.runs, kThreads, Shape::smem, st>>>(p, tiles, pl.tiles_per_seq);
-    if (p.runs > 1) mx_attention_join_kernel<kTile><<<(unsigned)(p.runs - 1), 128, 0, st>>>(p);
+    if (p.runs > 1) mx_attention_join_kernel<kTile><<<dim3((unsigned)(p.runs - 1), kTile / 8), 128, 0, st>>>(p);
     return check_launch("mx_attention");
 }
 
@@ -435,7 +465,8 @@ int launch(const AttentionParams& p, const ChunkPlan& pl, uint8_t* tiles, cudaSt
     if (p.dtype == MPT_DTYPE_F16) {
         if constexpr (DIM <= 192) return launch<DIM, 2, 2>(p, pl, tiles, st);
     } else {
-        if constexpr (DIM <= 128) return launch<DIM, 3, 2>(p, pl, tiles, st);
+        if constexpr (DIM <= 64) return launch<DIM, 3, 2>(p, pl, tiles, st);
+        else if constexpr (DIM <= 128) return launch<DIM, 3, 1>(p, pl, tiles, st);
     }
     set_error("mx_attention: no chunk kernel for this size");
     return MPT_ERR_INVALID_ARGUMENT;

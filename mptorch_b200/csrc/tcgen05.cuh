@@ -1,7 +1,7 @@
 // Inline PTX of the fifth-generation tensor cores as this library uses them: one CTA, 16-bit operands, fp32 accumulators in tensor
 // memory; mbarriers; copies from global to shared memory by the bulk-copy engine.
 //
-// Every wait has a limit: a wait that runs out returns false, and the kernels then end without their result instead of hanging.
+// Every wait has a limit: the kernels end with NaN for their result instead of hanging.
 #pragma once
 #include <cstdint>
 #include <cuda_runtime.h>
@@ -17,13 +17,16 @@ __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrie
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Waits until the phase of the given parity is over.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+// Waits until the phase of the given parity is over.  A wait that runs out sets `*failed` (in shared memory), and no wait of the CTA
+// is long after that.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
     for (uint32_t i = 0; i < kWaitLimit; ++i) {
         uint32_t done;
         asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
         if (done) return true;
+        if ((i & 255u) == 255u && *failed) return false;
     }
+    *failed = 1u;
     return false;
 }
 __device__ __forceinline__ void fence_barrier_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
@@ -54,6 +57,12 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t* r) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
                    "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
                    "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(at));
+}
+__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(at));
 }
 __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* r) {
