@@ -15,8 +15,6 @@
 // moved only when a tile exceeds it.
 //
 // Measured figures stand at the launch rule below.
-#include <atomic>
-
 #include "attention.cuh"
 #include "attention_chunk.cuh"
 
@@ -79,8 +77,10 @@ __host__ __device__ __forceinline__ int smem_bytes(int dim, bool fp4, int nt) {
     return cols * l.q_pitch + (ring > merge ? ring : merge);
 }
 
+constexpr int ctas_by_registers(int nb, int nt) { return nt == 1 && nb <= 4 ? 4 : nb * nt <= 8 ? 3 : 2; }
+
 template <int NB, bool FP4, int PIECES, int NT>
-__global__ void __launch_bounds__(32 * kWarps, NT == 1 && NB <= 4 ? 4 : NB * NT <= 8 ? 3 : 2) mx_attention_rows_kernel(const AttentionParams p) {
+__global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_attention_rows_kernel(const AttentionParams p) {
     constexpr int kCols = 8 * NT, kRows = kCols / PIECES, kMine = PIECES == 1 ? 2 * NT : NT;   // columns and rows of the CTA; rows that a lane holds
     extern __shared__ __align__(16) uint8_t smem[];
     const CacheView& c = p.c;
@@ -597,19 +597,9 @@ template <int NB, bool FP4, int PIECES, int NT>
 int launch_rows(AttentionParams p, const Plan& pl, cudaStream_t st) {
     const int bytes = smem_bytes(p.c.dim, FP4, NT);
     auto kern = mx_attention_rows_kernel<NB, FP4, PIECES, NT>;
-    static std::atomic<int> resident[64];        // CTAs of this kernel on an SM, by device; 0: not asked yet
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { set_error("mx_attention: no device"); return MPT_ERR_CUDA; }
-    int fit = resident[dev].load(std::memory_order_relaxed);
-    if (fit == 0) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, 32 * kWarps, bytes) != cudaSuccess || fit < 1) {
-            check_launch("mx_attention");
-            set_error("mx_attention: the kernel does not fit this device");
-            return MPT_ERR_CUDA;
-        }
-        resident[dev].store(fit, std::memory_order_relaxed);
-    }
+    // CTAs on an SM, by registers (launch bounds) and shared memory (2 kB a CTA beside the dynamic part)
+    const int by_memory = 228 * 1024 / (bytes + 2048), fit = by_memory < ctas_by_registers(NB, NT) ? (by_memory < 1 ? 1 : by_memory) : ctas_by_registers(NB, NT);
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return check_launch("mx_attention");
     const int most = fit * sm_count();
     p.runs = pl.runs < most ? pl.runs : most;
     kern<<<(unsigned)p.runs, 32 * kWarps, bytes, st>>>(p);

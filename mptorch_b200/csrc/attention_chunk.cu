@@ -12,8 +12,6 @@
 // bits), and so are their weights p; sums are fp32 throughout.
 //
 // Measured figures stand at the launch rule below.
-#include <atomic>
-
 #include "attention.cuh"
 #include "attention_chunk.cuh"
 #include "tcgen05.cuh"
@@ -436,20 +434,9 @@ template <int DIM, int PIECES, int NS>
 int launch(AttentionParams p, const ChunkPlan& pl, uint8_t* tiles, cudaStream_t st) {
     using Shape = ChunkShape<DIM, PIECES, NS>;
     auto kern = mx_attention_chunk_kernel<DIM, PIECES, NS>;
-    static std::atomic<int> resident[64];                         // CTAs of this kernel on an SM, by device; 0: not asked yet
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { set_error("mx_attention: no device"); return MPT_ERR_CUDA; }
-    int fit = resident[dev].load(std::memory_order_relaxed);
-    if (fit == 0) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem) != cudaSuccess ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, kThreads, Shape::smem) != cudaSuccess || fit < 1) {
-            check_launch("mx_attention");
-            set_error("mx_attention: the kernel does not fit this device");
-            return MPT_ERR_CUDA;
-        }
-        fit = fit * Shape::columns > 512 ? 512 / Shape::columns : fit;      // tensor memory: 512 columns an SM
-        resident[dev].store(fit, std::memory_order_relaxed);
-    }
+    // CTAs on an SM, by tensor memory (512 columns), shared memory (3 kB a CTA beside the dynamic part) and registers (launch bounds)
+    const int fit = Shape::columns == 256 && 2 * (Shape::smem + 3 * 1024) <= 228 * 1024 && NS == 1 && PIECES == 1 ? 2 : 1;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem) != cudaSuccess) return check_launch("mx_attention");
     p.runs = pl.runs < fit * sm_count() ? pl.runs : fit * sm_count();
     kern<<<(unsigned)p.runs, kThreads, Shape::smem, st>>>(p, tiles, pl.tiles_per_seq);
     if (p.runs > 1) mx_attention_join_kernel<kTile><<<dim3((unsigned)(p.runs - 1), kTile / 8), 128, 0, st>>>(p);
