@@ -30,7 +30,7 @@ NVCC_FLAGS = [
 # products with packed weights and the attention, whose sums have no prescribed roundings.
 EXTRA_FLAGS = {"reduce.cu": [], "rows_softmax_fwd.cu": [], "rows_softmax_bwd.cu": [], "rows_softmax_lse.cu": [], "rows_layernorm_fwd.cu": [],
                "rows_layernorm_bwd.cu": [], "blocklinear.cu": [], "attention.cu": [],
-               "attention_chunk.cu": []}
+               "attention_chunk.cu": [], "linear_tiles.cu": []}
 DEFAULT_EXTRA = ["-fmad=false"]
 
 

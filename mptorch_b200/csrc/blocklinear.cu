@@ -1,57 +1,262 @@
-// y = x W^T + b with W held as packed E2M1 codes and group scales (MXFP4, NVFP4).
+// y = x W^T + b for a few rows of x, with W held as packed E2M1 codes and group scales (MXFP4, NVFP4).
 //
-// One warp per output column and four rows of x at a time: a lane takes eight codes (a 32-bit word), decodes them, multiplies by
-// the group's scale and by the rows' values in fp32, and the warp adds up at the end.
-#include "blockcodes.cuh"
+// Bound: HBM, the codes and scales of W (half a byte and 1/32 or 1/16 of one for each weight).  At the measured bandwidth that is
+// 46 weights a clock on each SM, which leaves less than three instructions a weight: E2M1 is exact in binary16, so codes go to
+// the m16n8k16 tensor-core products after one conversion for two of them.  A CTA keeps x in shared memory and walks tiles of 16
+// rows of W; its eight warps take pieces of 128 of the sum in turn, each with a ring of its own that cp.async fills.
+//
+// x is scaled for each row by a power of two to a largest value in [2^14, 2^15) and held as binary16: bfloat16 and float16 in one
+// column (exact unless a value is 2^-29 of the largest or less), float32 in two, the second 2^11 times what the first leaves (22
+// bits).  NVFP4: a code times its E4M3 scale is exact in binary16 (six bits), so the weights are scaled and the products summed in
+// fp32 as they are.  MXFP4: the scale of a block multiplies the fp32 sum of its 32 products, relative to an exponent that is kept
+// for each row of W and raised when a block exceeds it by 2^60, so that no range of scales overflows.
+//
+// Measured figures stand at the launch rule below.
+#include "blocklinear.cuh"
 
 namespace mpt {
 namespace {
 
-constexpr int kWarps = 8, kRows = 4;
+constexpr int kWarps = 8, kChunk = 128, kPitch = 80, kStages = 4;          // pitch: eight rows of four words meet no bank twice
 
-template <typename T, bool NV>
-__global__ void __launch_bounds__(32 * kWarps) block_linear_kernel(const T* __restrict__ x, const uint8_t* __restrict__ codes,
-                                                                   const uint8_t* __restrict__ scales, const float* __restrict__ global_scale,
-                                                                   const T* __restrict__ bias, T* __restrict__ y, int64_t rows, int64_t n_out,
-                                                                   int64_t n_in) {
-    const int lane = threadIdx.x & 31;
-    const int64_t n = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    if (n >= n_out) return;
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(codes + n * (n_in >> 1));
-    const uint8_t* s = scales + n * (n_in / (NV ? 16 : 32));
-    const float glob = global_scale != nullptr ? *global_scale : 1.0f;
-    for (int64_t m0 = (int64_t)blockIdx.y * kRows; m0 < rows; m0 += (int64_t)gridDim.y * kRows) {
-        float acc[kRows] = {};
-        for (int64_t k = 8 * lane; k < n_in; k += 256) {
-            float v[8];
-            decode8<true>(make_uint2(w[k >> 3], 0u), v);
-            float sc;
-            if (NV) {
-                uint32_t lo, hi;
-                e4m3x4_to_half(s[k >> 4], lo, hi);
-                sc = half2_value(lo).x;
-            } else {
-                sc = e8m0_value(s[k >> 5]);
-            }
+__device__ __forceinline__ void cp_bytes(uint32_t dst, const void* src, int bytes) {   // 16
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes));
+}
+template <int N>
+__device__ __forceinline__ void cp_small(uint32_t dst, const void* src, int bytes) {   // 4 or 8
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(dst), "l"(src), "n"(N), "r"(bytes));
+}
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t times(uint32_t a, __half2 s) {
+    const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), s);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// 2^(e - ref), zero below 2^-149
+__device__ __forceinline__ float relative_power(int e, int ref) {
+    const int d = e - ref;
+    return d >= -126 ? __uint_as_float((uint32_t)(d + 127) << 23) : d >= -149 ? __uint_as_float(1u << (d + 149)) : 0.f;
+}
+
+__host__ __device__ constexpr int stage_bytes(bool nv) { return 16 * kPitch + 16 * (nv ? 8 : 4); }
+__host__ __device__ inline int x_pitch(int n_in) { return n_in * 2 + ((n_in & 63) ? 0 : 64); }   // 64 bytes behind a multiple of 128
+inline int few_smem(int n_in, int columns, bool nv, int nt) {
+    const int ring = kWarps * kStages * stage_bytes(nv), sums = kWarps * 16 * 8 * nt * 4;
+    return columns * x_pitch(n_in) + ring + sums;
+}
+
+template <bool NV, int PIECES, int NT>
+__global__ void __launch_bounds__(32 * kWarps, 2) block_linear_few_kernel(const LinearParams p, int tiles) {
+    constexpr int kScaleRow = NV ? 8 : 4;                                 // bytes of scales of a row in a piece of 128
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, tig = lane & 3;
+    const int pitch = x_pitch(p.n_in), columns = p.rows * PIECES, row_bytes = p.n_in >> 1, scale_row = p.n_in / (NV ? 16 : 32);
+    const int chunks = (p.n_in + kChunk - 1) / kChunk;
+    const bool even = p.n_in % kChunk == 0 && (reinterpret_cast<uintptr_t>(p.scales) & 7u) == 0;     // scales can be copied by words
+    uint8_t* ring = smem + columns * pitch + warp * kStages * stage_bytes(NV);
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    float* sums = reinterpret_cast<float*>(smem + columns * pitch + kWarps * kStages * stage_bytes(NV));   // [warp][column][16]
+    __shared__ int exponent[16], refs[kWarps][16];
+
+    // this warp's pieces, through all tiles of the CTA
+    int put_tile = blockIdx.x, put_chunk = warp;
+    auto advance = [&](int& tile, int& chunk) {
+        chunk += kWarps;
+        if (chunk >= chunks) { chunk = warp; tile += gridDim.x; }
+    };
+    const bool busy = warp < chunks;
+    auto issue = [&](int stage) {
+        if (busy && put_tile < tiles) {
+            const uint32_t at = ring_at + stage * stage_bytes(NV);
+            const int n0 = put_tile * 16;
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                if (m0 + r >= rows) break;
-                float d = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) d = fmaf(v[e], to_float(x[(m0 + r) * n_in + k + e]), d);
-                acc[r] = fmaf(d, sc, acc[r]);
+            for (int i = 0; i < 2; ++i) {
+                const int r = i * 8 + (lane >> 2), ch = lane & 3;
+                const bool live = n0 + r < p.n_out && put_chunk * kChunk + ch * 32 < p.n_in;
+                cp_bytes(at + r * kPitch + ch * 16, p.codes + (live ? (int64_t)(n0 + r) * row_bytes + put_chunk * (kChunk / 2) + ch * 16 : 0), live ? 16 : 0);
             }
+            if (lane < 16) {
+                const bool live = n0 + lane < p.n_out;
+                const uint8_t* src = p.scales + (live ? (int64_t)(n0 + lane) * scale_row + put_chunk * kScaleRow : 0);
+                const uint32_t to = at + 16 * kPitch + lane * kScaleRow;
+                if (even) {
+                    cp_small<kScaleRow>(to, src, live ? kScaleRow : 0);
+                } else {
+                    uint8_t* dst = ring + stage * stage_bytes(NV) + 16 * kPitch + lane * kScaleRow;
+                    const int have = live ? min(kScaleRow, scale_row - put_chunk * kScaleRow) : 0;
+                    for (int i = 0; i < kScaleRow; ++i) dst[i] = i < have ? src[i] : (uint8_t)0;
+                }
+            }
+            advance(put_tile, put_chunk);
         }
+        asm volatile("cp.async.commit_group;\n" ::);
+    };
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-            for (int o = 16; o > 0; o >>= 1) acc[r] += __shfl_xor_sync(0xFFFFFFFFu, acc[r], o);
-            if (lane == 0 && m0 + r < rows) {
-                float v = acc[r] * glob;
-                if (bias != nullptr) v += to_float(bias[n]);
-                y[(m0 + r) * n_out + n] = from_float<T>(v);
+    for (int s = 0; s < kStages - 1; ++s) issue(s);
+
+    // ---- x: a warp takes a row at a time
+    for (int m = warp; m < p.rows; m += kWarps) {
+        float top = 0.f;
+        for (int k = 8 * lane; k < p.n_in; k += 256) {
+            float v[8];
+            read8(p.x, p.dtype, p.x_vec, (int64_t)m * p.n_in + k, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { const float a = fabsf(v[e]); if (a < INFINITY) top = fmaxf(top, a); }
+        }
+        const int e = row_exponent(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top)));
+        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+        if (lane == 0) exponent[m] = e;
+        for (int k = 8 * lane; k < p.n_in; k += 256) {
+            float v[8];
+            read8(p.x, p.dtype, p.x_vec, (int64_t)m * p.n_in + k, v);
+            __half hi[8], lo[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[i] *= up;
+                hi[i] = __float2half_rn(v[i]);
+                lo[i] = fabsf(v[i]) < INFINITY ? __float2half_rn((v[i] - __half2float(hi[i])) * 2048.f) : __float2half_rn(0.f);
             }
+            *reinterpret_cast<uint4*>(smem + m * PIECES * pitch + k * 2) = *reinterpret_cast<uint4*>(hi);
+            if (PIECES == 2) *reinterpret_cast<uint4*>(smem + (m * 2 + 1) * pitch + k * 2) = *reinterpret_cast<uint4*>(lo);
         }
     }
+    __syncthreads();
+
+    const float glob = p.global_scale != nullptr ? __ldg(p.global_scale) : 1.f;
+    int stage = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        float acc[NT][4];
+        int ref0 = 127, ref1 = 127;                                        // MXFP4: the exponents of rows g and g + 8 that the sums are relative to
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+        for (int chunk = warp; chunk < chunks; chunk += kWarps) {
+            issue(stage == 0 ? kStages - 1 : stage - 1);
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 1));
+            __syncwarp();
+            const uint8_t* w = ring + stage * stage_bytes(NV);
+            const uint8_t* sc = w + 16 * kPitch;
+            uint2 s0, s1;
+            if (NV) {
+                s0 = *reinterpret_cast<const uint2*>(sc + g * 8);
+                s1 = *reinterpret_cast<const uint2*>(sc + (g + 8) * 8);
+            } else {
+                s0.x = *reinterpret_cast<const uint32_t*>(sc + g * 4);
+                s1.x = *reinterpret_cast<const uint32_t*>(sc + (g + 8) * 4);
+                // the largest of the four, as long as none is far above the reference
+                const uint32_t t0 = __vmaxu4(s0.x, s0.x >> 16), t1 = __vmaxu4(s1.x, s1.x >> 16);
+                const int top0 = max(t0 & 255u, (t0 >> 8) & 255u), top1 = max(t1 & 255u, (t1 >> 8) & 255u);
+                if (top0 > ref0 + 60) {
+                    const float fade = relative_power(ref0, top0);
+                    ref0 = top0;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) { acc[n][0] *= fade; acc[n][1] *= fade; }
+                }
+                if (top1 > ref1 + 60) {
+                    const float fade = relative_power(ref1, top1);
+                    ref1 = top1;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) { acc[n][2] *= fade; acc[n][3] *= fade; }
+                }
+            }
+            const int k0 = chunk * kChunk;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                if (k0 + b * 32 >= p.n_in) break;
+                uint32_t a[4], d[4];
+                e2m1x8_to_half(*reinterpret_cast<const uint32_t*>(w + g * kPitch + b * 16 + tig * 4), a);
+                e2m1x8_to_half(*reinterpret_cast<const uint32_t*>(w + (g + 8) * kPitch + b * 16 + tig * 4), d);
+                uint4 x[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    x[n] = make_uint4(0u, 0u, 0u, 0u);
+                    if (n * 8 + g < columns) x[n] = *reinterpret_cast<const uint4*>(smem + (n * 8 + g) * pitch + (k0 + b * 32 + tig * 8) * 2);
+                }
+                if (NV) {
+                    const uint32_t sel = 0x11u * (2 * (b & 1) + (tig >> 1));     // this lane's byte, twice
+                    uint32_t h0, h1, unused;
+                    e4m3x4_to_half(__byte_perm(b < 2 ? s0.x : s0.y, 0u, sel), h0, unused);
+                    e4m3x4_to_half(__byte_perm(b < 2 ? s1.x : s1.y, 0u, sel), h1, unused);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        a[i] = times(a[i], *reinterpret_cast<__half2*>(&h0));
+                        d[i] = times(d[i], *reinterpret_cast<__half2*>(&h1));
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma(acc[n], a[0], d[0], a[1], d[1], x[n].x, x[n].y);
+                        mma(acc[n], a[2], d[2], a[3], d[3], x[n].z, x[n].w);
+                    }
+                } else {
+                    const int e0 = (s0.x >> (8 * b)) & 255u, e1 = (s1.x >> (8 * b)) & 255u;
+                    const float f0 = e0 == 255 ? __uint_as_float(0x7FC00000u) : relative_power(e0, ref0);
+                    const float f1 = e1 == 255 ? __uint_as_float(0x7FC00000u) : relative_power(e1, ref1);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float c[4];
+                        mma_first(c, a[0], d[0], a[1], d[1], x[n].x, x[n].y);
+                        mma(c, a[2], d[2], a[3], d[3], x[n].z, x[n].w);
+                        acc[n][0] = fmaf(c[0], f0, acc[n][0]);
+                        acc[n][1] = fmaf(c[1], f0, acc[n][1]);
+                        acc[n][2] = fmaf(c[2], f1, acc[n][2]);
+                        acc[n][3] = fmaf(c[3], f1, acc[n][3]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (++stage == kStages) stage = 0;
+        }
+        // ---- the warps' sums
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[(warp * 8 * NT + n * 8 + 2 * tig + (i & 1)) * 16 + g + 8 * (i >> 1)] = acc[n][i];
+        if (!NV && tig == 0) { refs[warp][g] = ref0; refs[warp][g + 8] = ref1; }
+        __syncthreads();
+        for (int i = threadIdx.x; i < p.rows * 16; i += 32 * kWarps) {
+            const int m = i >> 4, r = i & 15, n = tile * 16 + r;
+            int ref = 127;
+            if (!NV)
+                for (int w = 0; w < kWarps; ++w) ref = max(ref, refs[w][r]);
+            float v = 0.f, v2 = 0.f;
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = NV ? 1.f : relative_power(refs[w][r], ref);
+                v = fmaf(sums[(w * 8 * NT + m * PIECES) * 16 + r], f, v);
+                if (PIECES == 2) v2 = fmaf(sums[(w * 8 * NT + m * 2 + 1) * 16 + r], f, v2);
+            }
+            if (PIECES == 2) v = fmaf(v2, 0x1p-11f, v);
+            if (n < p.n_out) {
+                v = scale_by_power(v, (NV ? 0 : ref - 127) - exponent[m]) * glob;
+                if (p.bias != nullptr) v += read_value(p.bias, p.dtype, n);
+                write_value(p.y, p.dtype, (int64_t)m * p.n_out + n, v);
+            }
+        }
+        __syncthreads();
+    }
+    asm volatile("cp.async.wait_group 0;\n" ::);
+}
+
+template <bool NV, int PIECES, int NT>
+int launch_few(const LinearParams& p, cudaStream_t st) {
+    const int bytes = few_smem(p.n_in, p.rows * PIECES, NV, NT), tiles = (p.n_out + 15) / 16;
+    auto kern = block_linear_few_kernel<NV, PIECES, NT>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return check_launch("block_linear");
+    const int most = (2 * (bytes + 2048) <= 228 * 1024 ? 2 : 1) * sm_count();
+    kern<<<(unsigned)(tiles < most ? tiles : most), 32 * kWarps, bytes, st>>>(p, tiles);
+    return check_launch("block_linear");
+}
+
+// Few rows: at most 16 columns (a float32 row takes two), x within the shared memory that leaves room for a second CTA.
+bool few_rows(int64_t rows, int64_t n_in, int dtype) {
+    const int64_t columns = rows * (dtype == MPT_DTYPE_F32 ? 2 : 1);
+    return columns <= 16 && columns * (2 * n_in + 64) <= 56 * 1024;
 }
 
 }  // namespace
@@ -61,25 +266,38 @@ using namespace mpt;
 
 extern "C" {
 
-size_t mpt_block_linear_workspace_bytes(int64_t, int64_t, int64_t, int, int) { return 0; }
+size_t mpt_block_linear_workspace_bytes(int64_t rows, int64_t n_out, int64_t n_in, int format, int dtype) {
+    (void)format;
+    if (rows <= 0 || n_out <= 0 || n_in < 0 || rows > 0x7FFFFFFF || n_out > 0x7FFFFFFF || n_in > 0x7FFFFFFF || few_rows(rows, n_in, dtype)) return 0;
+    return tiles_plan(rows, n_out, n_in, dtype).bytes;
+}
 
 int mpt_block_linear(const void* x, const uint8_t* codes, const uint8_t* scales, const float* global_scale, const void* bias, void* y,
                      int64_t rows, int64_t n_out, int64_t n_in, int format, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
-    (void)workspace; (void)workspace_bytes;
-    MPT_REQUIRE(rows >= 0 && n_out >= 0 && n_in >= 0 && rows <= 0x7FFFFFFF && n_out <= 0x7FFFFFFF && n_in <= 0x7FFFFFFF, "block_linear: bad extents");
+    MPT_REQUIRE(rows >= 0 && n_out >= 0 && n_in >= 0 && rows <= 0x7FFFFF00 && n_out <= 0x7FFFFF00 && n_in <= 0x3FFFFF00, "block_linear: bad extents");
     MPT_REQUIRE(n_in % 32 == 0, "block_linear: n_in %lld is not a multiple of 32", (long long)n_in);
     MPT_REQUIRE(format == MPT_BLOCK_MXFP4 || format == MPT_BLOCK_NVFP4, "block_linear: unknown format %d", format);
-    return with_dtype("block_linear", dtype, [&](auto t) -> int {
-        using T = decltype(t);
-        if (rows == 0 || n_out == 0) return MPT_OK;
-        MPT_REQUIRE(y && (n_in == 0 || (x && codes && scales)), "block_linear: null pointer");
-        MPT_REQUIRE(((uintptr_t)codes & 15u) == 0, "block_linear: the codes must begin at a multiple of 16 bytes");
-        const dim3 grid((unsigned)((n_out + kWarps - 1) / kWarps), (unsigned)((rows + kRows - 1) / kRows < 256 ? (rows + kRows - 1) / kRows : 256));
-        auto kern = format == MPT_BLOCK_NVFP4 ? block_linear_kernel<T, true> : block_linear_kernel<T, false>;
-        kern<<<grid, 32 * kWarps, 0, as_stream(stream)>>>(static_cast<const T*>(x), codes, scales, global_scale, static_cast<const T*>(bias),
-                                                        static_cast<T*>(y), rows, n_out, n_in);
-        return check_launch("block_linear");
-    });
+    MPT_REQUIRE(dtype == MPT_DTYPE_F32 || dtype == MPT_DTYPE_BF16 || dtype == MPT_DTYPE_F16, "block_linear: unknown data type %d", dtype);
+    if (rows == 0 || n_out == 0) return MPT_OK;
+    MPT_REQUIRE(y && (n_in == 0 || (x && codes && scales)), "block_linear: null pointer");
+    MPT_REQUIRE(((uintptr_t)codes & 15u) == 0, "block_linear: the codes must begin at a multiple of 16 bytes");
+    LinearParams p{x, codes, scales, global_scale, bias, y, dtype, (int)rows, (int)n_out, (int)n_in, ((uintptr_t)x & 15u) == 0};
+    cudaStream_t st = as_stream(stream);
+    if (few_rows(rows, n_in, dtype)) {
+        const bool nv = format == MPT_BLOCK_NVFP4;
+        if (dtype == MPT_DTYPE_F32) {
+            if (rows <= 4) return nv ? launch_few<true, 2, 1>(p, st) : launch_few<false, 2, 1>(p, st);
+            return nv ? launch_few<true, 2, 2>(p, st) : launch_few<false, 2, 2>(p, st);
+        }
+        if (rows <= 8) return nv ? launch_few<true, 1, 1>(p, st) : launch_few<false, 1, 1>(p, st);
+        return nv ? launch_few<true, 1, 2>(p, st) : launch_few<false, 1, 2>(p, st);
+    }
+    const TilesPlan pl = tiles_plan(rows, n_out, n_in, dtype);
+    if (workspace_bytes < pl.bytes || !workspace || ((uintptr_t)workspace & 255u)) {
+        set_error("block_linear: a workspace of %zu bytes at a multiple of 256 is needed", pl.bytes);
+        return MPT_ERR_WORKSPACE;
+    }
+    return launch_tiles(p, pl, format, static_cast<uint8_t*>(workspace), st);
 }
 
 }
