@@ -92,7 +92,7 @@ struct CacheView {
     // Sequence and position of a new row; false where it has none (behind the last sequence, or before the first token).
     __device__ __forceinline__ bool locate(int64_t row, int& seq, int& pos) const {
         if (starts == nullptr) {
-            seq = (int)(row / new_rows);
+            seq = (int)((uint32_t)row / (uint32_t)new_rows);      // fewer than 2^31 rows
             const int i = (int)(row - (int64_t)seq * new_rows);
             pos = __ldg(lens + seq) - new_rows + i;
         } else {
