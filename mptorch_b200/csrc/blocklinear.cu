@@ -393,6 +393,7 @@ int mpt_block_linear(const void* x, const uint8_t* codes, const uint8_t* scales,
     if (rows == 0 || n_out == 0) return MPT_OK;
     MPT_REQUIRE(y && (n_in == 0 || (x && codes && scales)), "block_linear: null pointer");
     MPT_REQUIRE(((uintptr_t)codes & 15u) == 0, "block_linear: the codes must begin at a multiple of 16 bytes");
+    MPT_REQUIRE(format != MPT_BLOCK_NVFP4 || ((uintptr_t)scales & 1u) == 0, "block_linear: NVFP4 scales must begin at an even address");
     LinearParams p{x, codes, scales, global_scale, bias, y, dtype, (int)rows, (int)n_out, (int)n_in, ((uintptr_t)x & 15u) == 0};
     cudaStream_t st = as_stream(stream);
     if (few_rows(rows, n_in, dtype)) {

@@ -5,32 +5,38 @@
 //   1. x is scaled for each row by a power of two to a largest value in [2^14, 2^15) and laid out as binary16 tiles of 64 of the sum, in
 //      the layout of the products' operands in shared memory, so that a tile is one bulk copy.  float32 takes two such pieces (22
 //      bits); bfloat16 and float16 one (exact unless a value is 2^-29 of the row's largest or less).
-//   2. A warp copies x's tiles, a warp issues products, and eight warps turn codes into binary16 weights in shared memory: one
-//      conversion and one multiplication for two of them.  NVFP4: a code times its E4M3 scale is exact (six bits).  MXFP4: a code times
+//   2. The pieces of 256 of the sum of all tiles (128 rows of W by up to 256 columns) are cut into equal runs, one for each SM.  A warp
+//      copies x's tiles, a warp issues products, and sixteen warps turn codes into binary16 weights in shared memory, four blocks of
+//      64 at a time (a warp then reads 128 bytes of each of four rows), two pieces ahead in registers: one conversion and one
+//      multiplication for two weights.  NVFP4: a code times its E4M3 scale is exact (six bits).  MXFP4: a code times
 //      2^(13 + e - E), E the row's largest exponent, is exact down to e = E - 36; smaller blocks count less than 2^-36 of the largest.
 //      Sums are fp32 in tensor memory, those of float32's second pieces apart, and the powers of two are put back at the end.
-//   3. Where there are too few tiles for the SMs the sum is split, and the parts are added up in order.
+//   3. A tile that a run ends in is left in parts, which are added up in order.
 //
 // Measured figures stand at the launch rule below.
 #include "blocklinear.cuh"
+#include "launch.cuh"
 #include "tcgen05.cuh"
 
 namespace mpt {
 namespace {
 
-constexpr int kRowsW = 128, kBlock = 64, kWorkers = 256, kThreads = kWorkers + 64;
+constexpr int kRowsW = 128, kBlock = 64, kSuper = 4, kWorkers = 512, kThreads = kWorkers + 64;   // codes are read in pieces of four blocks
 constexpr int kPartW = kRowsW * 128;                               // bytes of a tile of W: 128 rows of 64 weights
 
 struct TilesParams {
     LinearParams l;
-    int cols, pieces, k_blocks, splits, stages, columns;
+    int cols, pieces, k_blocks, col_tiles, w_stages, x_stages, columns;
+    int k_supers;                      // pieces of four blocks of a tile
+    int64_t units, per;                // such pieces of all tiles, and of a run
     const uint8_t* image;              // x: [column tile][block of 64][piece][cols][128 bytes]
     int* exponent;                     // of each row of x
-    float* partial;                    // [split][rows][n_out]
+    float* partial;                    // of tiles that are cut: [slot][column][128]
 };
 
 // ---- x into tiles: a CTA for a row
 __global__ void __launch_bounds__(256) linear_split_kernel(const TilesParams p, uint8_t* __restrict__ image) {
+    next_may_start();
     const LinearParams& l = p.l;
     const int m = blockIdx.x, ct = m / p.cols, r = m - ct * p.cols, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     __shared__ uint32_t tops[8];
@@ -73,200 +79,327 @@ __device__ __forceinline__ uint32_t half_product_descriptor(int n) { return (1u 
 // 2^(13 - d) as binary16, zero below 2^-24
 __device__ __forceinline__ uint32_t half_weight_power(int d) { return d <= 27 ? (uint32_t)(28 - d) << 10 : d <= 37 ? 1u << (37 - d) : 0u; }
 
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 12;                                      // of W's ring; x's has at most eight
 
+// MXFP4: the largest exponent of row n of W, found by the eight lanes c of a row (255 is a NaN and no exponent); bytes up to an aligned
+// word, then words.
 template <bool NV>
-__global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const TilesParams p) {
+__device__ __forceinline__ int row_top(const TilesParams& p, int n, int c) {
+    if (NV) return 0;
+    int top = 0;
+    const int groups = p.l.n_in / 32;
+    if (n < p.l.n_out) {
+        const uint8_t* sc = p.l.scales + (int64_t)n * groups;
+        auto take = [&](uint32_t e) { top = max(top, e == 255u ? 0 : (int)e); };
+        const int head = min((int)((4 - (reinterpret_cast<uintptr_t>(sc) & 3)) & 3), groups), words = (groups - head) >> 2;
+        if (c < head) take(__ldg(sc + c));
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(sc + head);
+#pragma unroll 4
+        for (int k = c; k < words; k += 8) {
+            const uint32_t w = __ldg(from + k);
+            take(w & 255u); take((w >> 8) & 255u); take((w >> 16) & 255u); take(w >> 24);
+        }
+        if (head + 4 * words + c < groups) take(__ldg(sc + head + 4 * words + c));
+    }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    return top;
+}
+
+// A tile's sums, or a run's part of them: a thread has one row of W; the warps of each quarter of rows take every fourth 16 columns.
+template <bool NV>
+__device__ __noinline__ void tile_end(const TilesParams& p, uint32_t tmem, const int* top_e, int tile, bool whole, bool begins, bool ok) {
+    const LinearParams& l = p.l;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rt = tile / p.col_tiles, ct = tile - rt * p.col_tiles;
+    tmem_fence_after();
+    const int rw = (warp & 3) * 32 + lane, n = rt * kRowsW + rw;
+    const float glob = NV && l.global_scale != nullptr ? __ldg(l.global_scale) : 1.f;
+    const float bias = whole && l.bias != nullptr && n < l.n_out ? read_value(l.bias, l.dtype, n) : 0.f;
+    const int we = NV ? 0 : top_e[rw] - 140;
+    const bool near = we >= -60 && we <= 60;                       // no product leaves fp32's range on the way
+    const float wpow = __uint_as_float((uint32_t)(127 + (near ? we : 0)) << 23);
+    float* part = p.partial + (2 * (int64_t)blockIdx.x + (begins ? 0 : 1)) * p.cols * kRowsW + rw;
+    for (int c0 = 16 * (warp >> 2); c0 < p.cols; c0 += 64) {
+        uint32_t v[16], v2[16];
+        const int m_lane = ct * p.cols + c0 + (lane & 15), mine = m_lane < l.rows ? p.exponent[m_lane] : 0;
+        tmem_load16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0, v);
+        if (p.pieces == 2) tmem_load16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + p.cols + c0, v2);
+        tmem_wait_load();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int m = ct * p.cols + c0 + k, xe = __shfl_sync(0xFFFFFFFFu, mine, k);
+            if (m < l.rows) {
+                float y = __uint_as_float(v[k]);
+                if (p.pieces == 2) y = fmaf(__uint_as_float(v2[k]), 0x1p-11f, y);
+                if (near) y = y * wpow * __uint_as_float((uint32_t)(127 - xe) << 23);
+                else y = scale_by_power(y, we - xe);
+                y *= glob;
+                if (!ok) y = __uint_as_float(0x7FC00000u);
+                if (!whole) part[(c0 + k) * kRowsW] = y;
+                else if (n < l.n_out) write_value(l.y, l.dtype, (int64_t)m * l.n_out + n, y + bias);
+            }
+        }
+        __syncwarp();
+    }
+    tmem_fence_before();
+}
+
+// PER: blocks of a place in the rings, one or (where x's tiles are small) the four of a piece: what is waited for and handed on costs some
+// hundred clocks each time.
+template <bool NV, int PER>
+__global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_constant__ TilesParams p) {
+    next_may_start();
     extern __shared__ uint8_t smem_raw[];
     const LinearParams& l = p.l;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t base = (smem_at(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (base - smem_at(smem_raw));
-    const int x_bytes = p.pieces * p.cols * 128, stage_bytes = kPartW + x_bytes;
-    const int ct = blockIdx.x, n0 = blockIdx.y * kRowsW, split = blockIdx.z;
-    const int b_lo = (int)((int64_t)p.k_blocks * split / p.splits), b_hi = (int)((int64_t)p.k_blocks * (split + 1) / p.splits), blocks = b_hi - b_lo;
-    __shared__ __align__(8) uint64_t bars[3 * kMaxStages + 1];
+    const int x_bytes = p.pieces * p.cols * 128, x_base = p.w_stages * PER * kPartW;
+    const int64_t u0 = blockIdx.x * p.per, u1 = u0 + p.per < p.units ? u0 + p.per : p.units;
+    if (u0 >= u1) return;
+    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 16 + 4];
     __shared__ uint32_t tmem_slot, failed;
-    __shared__ int top_e[kRowsW];
-    auto x_full = [&](int s) { return smem_at(&bars[s]); };
-    auto w_full = [&](int s) { return smem_at(&bars[kMaxStages + s]); };
-    auto empty = [&](int s) { return smem_at(&bars[2 * kMaxStages + s]); };
-    const uint32_t done = smem_at(&bars[3 * kMaxStages]);
+    __shared__ int top_e[2][kRowsW];
+    auto w_full = [&](int s) { return smem_at(&bars[s]); };
+    auto w_empty = [&](int s) { return smem_at(&bars[kMaxStages + s]); };
+    auto x_full = [&](int s) { return smem_at(&bars[2 * kMaxStages + s]); };
+    auto x_empty = [&](int s) { return smem_at(&bars[2 * kMaxStages + 8 + s]); };
+    auto done = [&](int t) { return smem_at(&bars[2 * kMaxStages + 16 + (t & 1)]); };      // the sums of tile t of the run are there
+    auto taken = [&](int t) { return smem_at(&bars[2 * kMaxStages + 18 + (t & 1)]); };     // and have been read
     if (threadIdx.x == 0) {
-        for (int s = 0; s < p.stages; ++s) {
-            bar_init(x_full(s), 1);
-            bar_init(w_full(s), kWorkers);
-            bar_init(empty(s), 1);
-        }
-        bar_init(done, 1);
+        for (int s = 0; s < p.w_stages; ++s) { bar_init(w_full(s), kWorkers / kSuper * PER); bar_init(w_empty(s), 1); }
+        for (int s = 0; s < p.x_stages; ++s) { bar_init(x_full(s), 1); bar_init(x_empty(s), 1); }
+        for (int t = 0; t < 2; ++t) { bar_init(done(t), 1); bar_init(taken(t), kWorkers); }
         failed = 0u;
         fence_barrier_init();
     }
-    if (warp == 9) tmem_alloc(smem_at(&tmem_slot), p.columns);
+    if (warp == kWorkers / 32 + 1) tmem_alloc(smem_at(&tmem_slot), p.columns);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = tmem_slot;
+    const int tile0 = (int)(u0 / p.k_supers), super0 = (int)(u0 % p.k_supers), count = (int)(u1 - u0);
+    auto blocks_of = [&](int super) { return min(kSuper, p.k_blocks - super * kSuper); };
 
-    if (warp == 8) {
+    if (warp == kWorkers / 32) {
         if (lane == 0) {
-            const uint8_t* src = p.image + ((int64_t)ct * p.k_blocks + b_lo) * x_bytes;
-            for (int i = 0; i < blocks; ++i) {
-                const int s = i % p.stages;
-                if (i >= p.stages && !bar_wait(empty(s), (i / p.stages - 1) & 1, &failed)) break;
-                bar_expect(x_full(s), x_bytes);
-                bulk_load(base + s * stage_bytes + kPartW, src + (int64_t)i * x_bytes, x_bytes, x_full(s));
+            wait_for_previous();                                   // x's tiles
+            int tile = tile0, super = super0, stage = 0, turn = 0;
+            bool ok = true;
+            for (int i = 0; ok && i < count; ++i) {
+                const uint8_t* from = p.image + ((int64_t)(tile % p.col_tiles) * p.k_blocks + super * kSuper) * x_bytes;
+                const int blocks = blocks_of(super);
+                for (int q = 0; q < blocks; q += PER) {
+                    const uint32_t bytes = min(PER, blocks - q) * x_bytes;
+                    if (turn > 0 && !(ok = bar_wait(x_empty(stage), (turn - 1) & 1, &failed))) break;
+                    bar_expect(x_full(stage), bytes);
+                    bulk_load(base + x_base + stage * PER * x_bytes, from + (int64_t)q * x_bytes, bytes, x_full(stage));
+                    if (++stage == p.x_stages) { stage = 0; ++turn; }
+                }
+                if (++super == p.k_supers) { super = 0; ++tile; }
             }
         }
         __syncwarp();
-    } else if (warp == 9) {
+    } else if (warp == kWorkers / 32 + 1) {
         if (lane == 0) {
-            const uint32_t desc = half_product_descriptor(p.cols);
-            for (int i = 0; i < blocks; ++i) {
-                const int s = i % p.stages;
-                if (!bar_wait(x_full(s), (i / p.stages) & 1, &failed) || !bar_wait(w_full(s), (i / p.stages) & 1, &failed)) break;
-                tmem_fence_after();
-                const uint64_t w = tile_descriptor(base + s * stage_bytes, 16), x = tile_descriptor(base + s * stage_bytes + kPartW, 16);
+            const int n = p.pieces * p.cols;                       // the pieces' columns side by side, sums apart
+            const uint32_t desc = half_product_descriptor(n);
+            int super = super0, ws = 0, wt = 0, xs = 0, xt = 0, t = 0;
+            bool first = true, ok = true;
+            for (int i = 0; ok && i < count; ++i) {
+                if (first && t > 1 && !(ok = bar_wait(taken(t), ((t >> 1) - 1) & 1, &failed))) break;
+                const uint32_t to = tmem + (t & 1) * (p.columns >> 1);
+                const int blocks = blocks_of(super);
+                for (int q = 0; q < blocks; q += PER) {
+                    ok = bar_wait(x_full(xs), xt & 1, &failed) && bar_wait(w_full(ws), wt & 1, &failed);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    uint64_t w = tile_descriptor(base + ws * PER * kPartW, 16), x = tile_descriptor(base + x_base + xs * PER * x_bytes, 16);
 #pragma unroll
-                for (int k = 0; k < kBlock / 16; ++k) mma_ss(tmem, w + 2 * k, x + 2 * k, desc, i + k > 0);
-                if (p.pieces == 2) {
+                    for (int b = 0; b < PER; ++b) {
+                        if (q + b < blocks) {
 #pragma unroll
-                    for (int k = 0; k < kBlock / 16; ++k) mma_ss(tmem + p.cols, w + 2 * k, x + (p.cols * 128 >> 4) + 2 * k, desc, i + k > 0);
+                            for (int k = 0; k < kBlock / 16; ++k) mma_ss(to, w + 2 * k, x + 2 * k, desc, !first || k > 0);
+                            first = false;
+                            w += kPartW >> 4;
+                            x += x_bytes >> 4;
+                        }
+                    }
+                    mma_commit(w_empty(ws));
+                    mma_commit(x_empty(xs));
+                    if (++ws == p.w_stages) { ws = 0; ++wt; }
+                    if (++xs == p.x_stages) { xs = 0; ++xt; }
                 }
-                mma_commit(empty(s));
+                if (++super == p.k_supers) super = 0;
+                if (super == 0 || i + 1 == count) {
+                    mma_commit(done(t));
+                    ++t;
+                    first = true;
+                }
             }
-            mma_commit(done);
         }
         __syncwarp();
     } else {
-        // ---- weights: two threads a row, each 32 of a block's 64
-        const int r = threadIdx.x >> 1, half = threadIdx.x & 1, n = n0 + r;
-        const bool live = n < l.n_out;
+        // ---- weights: lane (c, row) takes 32 weights, half of block c / 2 of the piece, of rows r and r + 64
+        const int c = lane >> 2, r = warp * 4 + (lane & 3), q_mine = c >> 1, half = c & 1;
         const int groups = l.n_in / (NV ? 16 : 32);
-        const uint4* codes = reinterpret_cast<const uint4*>(l.codes + (live ? (int64_t)n * (l.n_in >> 1) : 0)) + half;
-        const uint8_t* scales = l.scales + (live ? (int64_t)n * groups : 0);
-        int top = 0;
-        if (!NV) {
-            if (live) {
-                // the row's largest exponent (255 is a NaN and no exponent); bytes up to an aligned word, then words
-                auto take = [&](uint32_t e) { top = max(top, e == 255u ? 0 : (int)e); };
-                int k = half;
-                const int head = min((int)((4 - (reinterpret_cast<uintptr_t>(scales) & 3)) & 3), groups);
-                if (half == 0)
-                    for (int j = 0; j < head; ++j) take(__ldg(scales + j));
-                const int words = (groups - head) >> 2;
-                const uint32_t* at = reinterpret_cast<const uint32_t*>(scales + head);
-#pragma unroll 4
-                for (k = half; k < words; k += 2) {
-                    const uint32_t w = __ldg(at + k);
-                    take(w & 255u); take((w >> 8) & 255u); take((w >> 16) & 255u); take(w >> 24);
+        constexpr int kAhead = 2;
+        uint4 ahead[kAhead][2] = {};
+        uint32_t ahead_s[kAhead][2] = {};
+        int next_tile = tile0, next_super = super0, next_i = 0, next_row = -1;
+        const uint8_t *codes0 = l.codes, *codes1 = l.codes, *scales0 = l.scales, *scales1 = l.scales;
+        // What lies outside the matrix is read from a place inside (and scaled by zero when it is used: a choice made here would wait
+        // for the load).
+        auto fetch = [&](uint4 (&w)[2], uint32_t (&sc)[2]) {
+            if (next_i < count) {
+                const int rt = next_tile / p.col_tiles;
+                if (rt != next_row) {
+                    next_row = rt;
+                    const int64_t n0 = min(rt * kRowsW + r, l.n_out - 1), n1 = min(rt * kRowsW + r + 64, l.n_out - 1);
+                    codes0 = l.codes + n0 * (l.n_in >> 1);
+                    codes1 = l.codes + n1 * (l.n_in >> 1);
+                    scales0 = l.scales + n0 * groups;
+                    scales1 = l.scales + n1 * groups;
                 }
-                if (half == 1)
-                    for (int j = head + 4 * words; j < groups; ++j) take(__ldg(scales + j));
-            }
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            if (half == 0) top_e[r] = top;
-        }
-        constexpr int kAhead = 4;
-        uint4 ahead[kAhead];
-        uint32_t ahead_s[kAhead];
-        auto fetch = [&](int i, uint4& w, uint32_t& sc) {
-            const int b = b_lo + i;
-            w = make_uint4(0u, 0u, 0u, 0u);
-            sc = NV ? 0u : (uint32_t)top;
-            if (i < blocks && live && b * 64 + half * 32 < l.n_in) {
-                w = __ldg(codes + b * 2);
-                if (NV) sc = __ldg(scales + b * 4 + half * 2) | ((uint32_t)__ldg(scales + b * 4 + half * 2 + 1) << 8);
-                else sc = __ldg(scales + b * 2 + half);
+                const int at = min(next_super * 8 + c, l.n_in / 32 - 1);
+                if (at >= 0) {
+                    w[0] = __ldg(reinterpret_cast<const uint4*>(codes0) + at);
+                    w[1] = __ldg(reinterpret_cast<const uint4*>(codes1) + at);
+                    if (NV) {
+                        sc[0] = __ldg(reinterpret_cast<const uint16_t*>(scales0) + at);
+                        sc[1] = __ldg(reinterpret_cast<const uint16_t*>(scales1) + at);
+                    } else {
+                        sc[0] = __ldg(scales0 + at);
+                        sc[1] = __ldg(scales1 + at);
+                    }
+                }
+                ++next_i;
+                if (++next_super == p.k_supers) { next_super = 0; ++next_tile; }
             }
         };
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) fetch(a, ahead[a], ahead_s[a]);
-        for (int i0 = 0; i0 < blocks; i0 += kAhead) {
+        for (int a = 0; a < kAhead; ++a) fetch(ahead[a], ahead_s[a]);
+
+        int tile = tile0, super = super0, seg_end = min(p.k_supers - super0, count), tiles = 0, i = 0, stage = 0, turn = 0, top[2];
+        bool whole = seg_end == p.k_supers;                        // the run has all pieces of the tile
+        int ended = -1;                                            // a tile whose sums have not been read yet
+        bool ended_whole = false;
+        auto begin_rows = [&](int t) {
+            const int n = tile / p.col_tiles * kRowsW + r;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (t == 0 || tile % p.col_tiles == 0) top[h] = row_top<NV>(p, n + 64 * h, c);     // otherwise the same rows again
+                if (!NV && c == 0) top_e[t & 1][r + 64 * h] = top[h];
+            }
+        };
+        auto end_tile = [&]() {                                    // tile `tiles - 1` of the run
+            bar_wait(done(tiles - 1), ((tiles - 1) >> 1) & 1, &failed);
+            if (tiles == 1) wait_for_previous();                   // the exponents of x
+            asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory");      // and every thread's part of top_e
+            tile_end<NV>(p, tmem + ((tiles - 1) & 1) * (p.columns >> 1), top_e[(tiles - 1) & 1], ended, ended_whole, tiles == 1, *(volatile uint32_t*)&failed == 0u);
+            bar_arrive(taken(tiles - 1));
+            ended = -1;
+            asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory");      // top_e has been read
+        };
+        begin_rows(0);
+        while (i < count || ended >= 0) {
 #pragma unroll
             for (int a = 0; a < kAhead; ++a) {
-                const int i = i0 + a;
-                if (i >= blocks) break;
-                const uint4 w = ahead[a];
-                const uint32_t sc = ahead_s[a];
-                fetch(i + kAhead, ahead[a], ahead_s[a]);
-                uint32_t h[16];
-                e2m1x8_to_half(w.x, *reinterpret_cast<uint32_t(*)[4]>(h));
-                e2m1x8_to_half(w.y, *reinterpret_cast<uint32_t(*)[4]>(h + 4));
-                e2m1x8_to_half(w.z, *reinterpret_cast<uint32_t(*)[4]>(h + 8));
-                e2m1x8_to_half(w.w, *reinterpret_cast<uint32_t(*)[4]>(h + 12));
-                uint32_t f[2];
-                if (NV) {
-                    uint32_t u;
-                    e4m3x4_to_half(__byte_perm(sc, 0u, 0x0000), f[0], u);
-                    e4m3x4_to_half(__byte_perm(sc, 0u, 0x1111), f[1], u);
-                } else {
-                    const uint32_t q = sc == 255u ? 0x7E00u : half_weight_power(top - (int)sc);
-                    f[0] = f[1] = q | (q << 16);
-                }
+                if (i < count) {
+                    const int blocks = blocks_of(super);
+                    int s = stage, t = turn;
+                    if (PER == 1) {
+                        s += q_mine;
+                        if (s >= p.w_stages) { s -= p.w_stages; ++t; }
+                    }
+                    if (PER > 1 || q_mine < blocks) {
+                        if (t > 0) bar_wait(w_empty(s), (t - 1) & 1, &failed);
+                        const bool inside = super * 8 + c < l.n_in / 32;
+                        const int n = tile / p.col_tiles * kRowsW + r;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&h[k]), *reinterpret_cast<__half2*>(&f[k >> 3]));
-                    h[k] = *reinterpret_cast<const uint32_t*>(&v);
-                }
-                const int s = i % p.stages;
-                if (i >= p.stages) bar_wait(empty(s), (i / p.stages - 1) & 1, &failed);
-                uint8_t* to = smem + s * stage_bytes + r * 128;
+                        for (int v = 0; v < 2; ++v) {
+                            const uint4 w = ahead[a][v];
+                            const uint32_t sc = ahead_s[a][v];
+                            const bool on = inside && n + 64 * v < l.n_out;
+                            uint32_t h[16], f[2];
+                            e2m1x8_to_half(w.x, *reinterpret_cast<uint32_t(*)[4]>(h));
+                            e2m1x8_to_half(w.y, *reinterpret_cast<uint32_t(*)[4]>(h + 4));
+                            e2m1x8_to_half(w.z, *reinterpret_cast<uint32_t(*)[4]>(h + 8));
+                            e2m1x8_to_half(w.w, *reinterpret_cast<uint32_t(*)[4]>(h + 12));
+                            if (NV) {
+                                uint32_t u;
+                                e4m3x4_to_half(on ? __byte_perm(sc, 0u, 0x0000) : 0u, f[0], u);
+                                e4m3x4_to_half(on ? __byte_perm(sc, 0u, 0x1111) : 0u, f[1], u);
+                            } else {
+                                const uint32_t q = !on ? 0u : sc == 255u ? 0x7E00u : half_weight_power(top[v] - (int)sc);
+                                f[0] = f[1] = q | (q << 16);
+                            }
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<uint4*>(to + (((half * 4 + q) ^ (r & 7)) << 4)) = make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
-                fence_async_proxy();
-                bar_arrive(w_full(s));
+                            for (int q = 0; q < 16; ++q) {
+                                const __half2 x = __hmul2(*reinterpret_cast<__half2*>(&h[q]), *reinterpret_cast<__half2*>(&f[q >> 3]));
+                                h[q] = *reinterpret_cast<const uint32_t*>(&x);
+                            }
+                            const int row = r + 64 * v;
+                            uint8_t* to = smem + (PER == 1 ? s : s * PER + q_mine) * kPartW + row * 128;
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                *reinterpret_cast<uint4*>(to + (((half * 4 + q) ^ (row & 7)) << 4)) = make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
+                        }
+                        fence_async_proxy();
+                        bar_arrive(w_full(s));
+                    }
+                    fetch(ahead[a], ahead_s[a]);
+                    stage += PER == 1 ? blocks : 1;
+                    if (stage >= p.w_stages) { stage -= p.w_stages; ++turn; }
+                    if (++super == p.k_supers) super = 0;
+                    ++i;
+                }
+                // the sums of a tile are read when the first piece of the next one is under way
+                if (ended >= 0) end_tile();
+                if (i == seg_end) {
+                    ended = tile;
+                    ended_whole = whole;
+                    ++tiles;
+                    if (i < count) {
+                        seg_end = min(i + p.k_supers, count);
+                        whole = seg_end - i == p.k_supers;
+                        ++tile;
+                        begin_rows(tiles);
+                    } else {
+                        seg_end = -1;
+                        end_tile();
+                    }
+                }
             }
         }
-        // ---- results: a thread has one row of W; the warps of each half every other 16 columns
-        bar_wait(done, 0, &failed);
-        asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory");
-        tmem_fence_after();
-        const bool ok = *(volatile uint32_t*)&failed == 0u;
-        const int rw = (warp & 3) * 32 + lane, nw = n0 + rw;
-        const float glob = NV && l.global_scale != nullptr ? __ldg(l.global_scale) : 1.f;
-        const float bias = l.bias != nullptr && nw < l.n_out && p.splits == 1 ? read_value(l.bias, l.dtype, nw) : 0.f;
-        const int we = NV ? 0 : top_e[rw] - 140;
-        for (int c0 = 16 * (warp >> 2); c0 < p.cols; c0 += 32) {
-            uint32_t v[16], v2[16];
-            tmem_load16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0, v);
-            if (p.pieces == 2) tmem_load16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + p.cols + c0, v2);
-            tmem_wait_load();
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const int m = ct * p.cols + c0 + k;
-                if (m >= l.rows) break;
-                float y = __uint_as_float(v[k]);
-                if (p.pieces == 2) y = fmaf(__uint_as_float(v2[k]), 0x1p-11f, y);
-                y = blocks == 0 ? 0.f : scale_by_power(y, we - __ldg(p.exponent + m)) * glob;
-                if (!ok) y = __uint_as_float(0x7FC00000u);
-                if (nw < l.n_out) {
-                    if (p.splits > 1) p.partial[((int64_t)split * l.rows + m) * l.n_out + nw] = y;
-                    else write_value(l.y, l.dtype, (int64_t)m * l.n_out + nw, y + bias);
-                }
-            }
-            __syncwarp();
-        }
-        tmem_fence_before();
     }
     __syncthreads();
     if (failed && threadIdx.x == 0) {                              // copies on the way write to this CTA's memory
         failed = 0u;
-        for (int s = 0; s < p.stages; ++s) { bar_wait(x_full(s), 0, &failed); bar_wait(x_full(s), 1, &failed); }
+        for (int s = 0; s < p.x_stages; ++s) { bar_wait(x_full(s), 0, &failed); bar_wait(x_full(s), 1, &failed); }
     }
     __syncthreads();
-    if (warp == 9) tmem_free(tmem, p.columns);
+    if (warp == kWorkers / 32 + 1) tmem_free(tmem, p.columns);
 }
 
+// Adds up the tiles that runs end in: CTAs (x, .) look at the end of run x.
 __global__ void __launch_bounds__(256) linear_join_kernel(const TilesParams p) {
     const LinearParams& l = p.l;
-    const int64_t all = (int64_t)l.rows * l.n_out;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t cut = (blockIdx.x + 1) * p.per;
+    wait_for_previous();
+    if (cut >= p.units || cut % p.k_supers == 0) return;           // nothing is cut here
+    const int64_t tile = cut / p.k_supers, p0 = tile * p.k_supers, p1 = p0 + p.k_supers;
+    if ((int64_t)blockIdx.x * p.per > p0) return;                  // an earlier CTA adds this one up
+    const int last = (int)((p1 - 1) / p.per);
+    const int rt = (int)(tile / p.col_tiles), ct = (int)(tile - (int64_t)rt * p.col_tiles), here = min(p.cols, l.rows - ct * p.cols);
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < here * kRowsW; i += gridDim.y * 256) {
+        const int m = ct * p.cols + i / kRowsW, n = rt * kRowsW + i % kRowsW;
+        if (n >= l.n_out) continue;
         float y = 0.f;
-        for (int s = 0; s < p.splits; ++s) y += p.partial[s * all + i];
-        if (l.bias != nullptr) y += read_value(l.bias, l.dtype, i % l.n_out);
-        write_value(l.y, l.dtype, i, y);
+        for (int k = blockIdx.x; k <= last; ++k)
+            y += p.partial[(2 * (int64_t)k + (k == (int)blockIdx.x && k * p.per < p0 ? 1 : 0)) * p.cols * kRowsW + i];
+        if (l.bias != nullptr) y += read_value(l.bias, l.dtype, n);
+        write_value(l.y, l.dtype, (int64_t)m * l.n_out + n, y);
     }
 }
 
@@ -277,47 +410,47 @@ TilesPlan tiles_plan(int64_t rows, int64_t n_out, int64_t n_in, int dtype) {
     pl.pieces = dtype == MPT_DTYPE_F32 ? 2 : 1;
     const int64_t most = 256 / pl.pieces;
     // even column tiles: of 16 columns each, as few as hold the rows
-    const int64_t tiles = (rows + most - 1) / most;
-    pl.cols = (int)(((rows + tiles - 1) / tiles + 15) / 16 * 16);
+    const int64_t parts = (rows + most - 1) / most;
+    pl.cols = (int)(((rows + parts - 1) / parts + 15) / 16 * 16);
     pl.col_tiles = (int)((rows + pl.cols - 1) / pl.cols);
     pl.row_tiles = (int)((n_out + kRowsW - 1) / kRowsW);
-    pl.k_blocks = (int)((n_in + kBlock - 1) / kBlock);
-    const int stage = kPartW + pl.pieces * pl.cols * 128, sms = sm_count();
-    // two CTAs on an SM where their rings leave room for it, one with a longer ring otherwise
-    const int two = (110 * 1024 - 1024) / stage, one = (220 * 1024 - 1024) / stage;
-    pl.stages = two >= 3 ? two : one;
-    if (pl.stages > kMaxStages) pl.stages = kMaxStages;
-    const int64_t ctas = (int64_t)pl.row_tiles * pl.col_tiles, slots = (two >= 3 ? 2 : 1) * (int64_t)sms;
-    pl.splits = 1;
-    if (ctas * 2 <= slots) {
-        const int64_t want = slots / ctas, fit = pl.k_blocks / 4;
-        pl.splits = (int)(want > fit ? (fit < 1 ? 1 : fit) : want);
-    }
+    pl.k_blocks = n_in > 0 ? (int)((n_in + kBlock - 1) / kBlock) : 1;
+    // rings: where x's tiles are small, places of four blocks; else single blocks, x's ring covering the latency of a copy with three, the
+    // rest being W's (four blocks at least, a piece of which is written before it is waited for)
+    const int x_bytes = pl.pieces * pl.cols * 128, room = 219 * 1024;
+    pl.ring_blocks = x_bytes <= 8 * 1024 ? kSuper : 1;
+    pl.x_stages = pl.ring_blocks > 1 ? 2 : x_bytes <= 16 * 1024 ? 4 : 3;
+    pl.w_stages = (room - pl.x_stages * pl.ring_blocks * x_bytes) / (pl.ring_blocks * kPartW);
+    if (pl.w_stages > kMaxStages) pl.w_stages = kMaxStages;
+    // equal runs, one for each SM; or whole tiles, where their number leaves hardly an SM idle
+    const int64_t tiles = (int64_t)pl.row_tiles * pl.col_tiles, sms = sm_count(), rounds = (tiles + sms - 1) / sms;
+    pl.k_supers = (pl.k_blocks + kSuper - 1) / kSuper;
+    pl.units = tiles * pl.k_supers;
+    pl.per = (pl.units + sms - 1) / sms;
+    if (tiles >= sms && tiles * 16 >= rounds * sms * 15) pl.per = rounds * pl.k_supers;
+    pl.runs = (int)((pl.units + pl.per - 1) / pl.per);
     const int used = pl.pieces * pl.cols;
-    pl.columns = used <= 32 ? 32 : used <= 64 ? 64 : used <= 128 ? 128 : 256;
+    pl.columns = used <= 16 ? 32 : used <= 32 ? 64 : used <= 64 ? 128 : used <= 128 ? 256 : 512;      // two sets of sums
     pl.image_bytes = (size_t)pl.col_tiles * pl.k_blocks * pl.pieces * pl.cols * 128;
-    pl.partial_bytes = pl.splits > 1 ? (size_t)pl.splits * rows * n_out * 4 : 0;
+    pl.partial_bytes = pl.runs > 1 && pl.per % pl.k_supers ? (size_t)2 * pl.runs * pl.cols * kRowsW * 4 : 0;
     pl.bytes = pl.image_bytes + ((size_t)rows * 4 + 255) / 256 * 256 + pl.partial_bytes;
     return pl;
 }
 
 int launch_tiles(const LinearParams& l, const TilesPlan& pl, int format, uint8_t* workspace, cudaStream_t st) {
-    if (pl.row_tiles > 65535) { set_error("block_linear: more than %d outputs", 65535 * kRowsW); return MPT_ERR_INVALID_ARGUMENT; }
     TilesParams p;
     p.l = l;
-    p.cols = pl.cols; p.pieces = pl.pieces; p.k_blocks = pl.k_blocks; p.splits = pl.splits; p.stages = pl.stages; p.columns = pl.columns;
+    p.cols = pl.cols; p.pieces = pl.pieces; p.k_blocks = pl.k_blocks; p.col_tiles = pl.col_tiles; p.k_supers = pl.k_supers; p.units = pl.units; p.per = pl.per; p.w_stages = pl.w_stages; p.x_stages = pl.x_stages; p.columns = pl.columns;
     p.image = workspace;
     p.exponent = reinterpret_cast<int*>(workspace + pl.image_bytes);
     p.partial = reinterpret_cast<float*>(workspace + pl.image_bytes + ((size_t)l.rows * 4 + 255) / 256 * 256);
     linear_split_kernel<<<(unsigned)l.rows, 256, 0, st>>>(p, workspace);
-    const int bytes = 1024 + pl.stages * (kPartW + pl.pieces * pl.cols * 128);
-    auto kern = format == MPT_BLOCK_NVFP4 ? linear_tiles_kernel<true> : linear_tiles_kernel<false>;
+    const int bytes = 1024 + pl.ring_blocks * (pl.w_stages * kPartW + pl.x_stages * pl.pieces * pl.cols * 128);
+    const bool nv = format == MPT_BLOCK_NVFP4, single = pl.ring_blocks == 1;
+    auto kern = nv ? (single ? linear_tiles_kernel<true, 1> : linear_tiles_kernel<true, kSuper>) : (single ? linear_tiles_kernel<false, 1> : linear_tiles_kernel<false, kSuper>);
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return check_launch("block_linear");
-    kern<<<dim3((unsigned)pl.col_tiles, (unsigned)pl.row_tiles, (unsigned)pl.splits), kThreads, bytes, st>>>(p);
-    if (pl.splits > 1) {
-        const int64_t blocks = ((int64_t)l.rows * l.n_out + 255) / 256, most = 8 * (int64_t)sm_count();
-        linear_join_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(p);
-    }
+    launch_after(kern, dim3((unsigned)pl.runs), dim3(kThreads), bytes, st, p);
+    if (pl.partial_bytes) launch_after(linear_join_kernel, dim3((unsigned)(pl.runs - 1), 4), dim3(256), 0, st, p);
     return check_launch("block_linear");
 }
 
