@@ -24,9 +24,10 @@ namespace {
 #ifndef MPT_ATT_WARPS
 #define MPT_ATT_WARPS 4
 #define MPT_ATT_LEAST 8
+#define MPT_ATT_WHOLE 64
 #define MPT_ATT_CHUNK 40
 #endif
-constexpr int kWarps = MPT_ATT_WARPS, kTok = 32, kLeast = MPT_ATT_LEAST;
+constexpr int kWarps = MPT_ATT_WARPS, kTok = 32, kLeast = MPT_ATT_LEAST, kWhole = MPT_ATT_WHOLE;
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(live ? 16 : 0));
@@ -89,21 +90,18 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_att
     constexpr Layout lay(dim, FP4);
     __shared__ int64_t place_sm[kPlaceWords];
     __shared__ float row_mul[kRows];
+    next_may_start();
     zero_outside(p);
-    Place at;
-    int64_t per;
-    const int64_t total = find_place<kTok>(p, blockIdx.x, per, at, place_sm);
-    int64_t left = min(per, total - blockIdx.x * per);
-    bool begins = true;                         // the segment stands at the beginning of this CTA's run
-    while (left > 0) {
-    const int seq = at.seq, head = at.head, tile = at.tile, pieces = at.w.pieces(tile);
-    const int take = (int)min((int64_t)(pieces - at.piece), left);
+    RunOf<kTok> run(p, place_sm);
+    while (run.left > 0) {
+    const int seq = run.at.seq, head = run.at.head, tile = run.at.tile, pieces = run.at.w.pieces(tile), take = run.take(p, pieces);
+    if (take == 0) break;
     const int2 own = rows_of(c, seq);
     const int first = tile * kRows, count = min(kRows, own.y * p.group - first);
     const int len = __ldg(c.lens + seq), pos0 = len - own.y;
     const TokenTiles<kTok> tt(p, pos0 + first / p.group, pos0 + (first + count - 1) / p.group);
     const bool finished = take == pieces;
-    const int j_lo = min(at.piece, tt.tiles), j_hi = min(at.piece + take, tt.tiles);
+    const int j_lo = min(run.at.piece, tt.tiles), j_hi = min(run.at.piece + take, tt.tiles);
 
     uint8_t* q_sm = smem;
     uint8_t* ring = smem + kCols * lay.q_pitch + warp * (3 * lay.half + lay.expand);
@@ -511,7 +509,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_att
             }
     }
     __syncthreads();
-    const int share = 2 * blockIdx.x + (begins ? 0 : 1);
+    const int share = 2 * blockIdx.x + (run.begins ? 0 : 1);
     for (int r = warp; r < count; r += kWarps) {
         float top = -INFINITY, w[kWarps], sum = 0.f;
         uint32_t bad = 0u;
@@ -542,15 +540,14 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_att
         }
     }
     __syncthreads();
-    left -= take;
-    begins = false;
-    if (left > 0) at.next_tile<kTok>(p);
+    run.advance(p, take);
     }
 }
 
 // How a call is cut: columns of a tile, and CTAs.
 struct Plan {
     int pieces, nt, tile_rows, runs;
+    int64_t row_tiles, most_pieces;            // row tiles (about), and pieces of tokens of one at most
     size_t partial_floats, stats_floats;
 };
 
@@ -567,6 +564,8 @@ Plan make_plan(const CacheView& c, int q_heads, int dtype, int window, int sinks
     const int64_t tiles = c.rows * group / pl.tile_rows + c.seqs, pieces = (tokens + kTok - 1) / kTok + 1, most = 4 * (int64_t)sm_count();
     const int64_t want = (tiles * c.heads * pieces + kLeast - 1) / kLeast;
     pl.runs = (int)(want < 1 ? 1 : want > most ? most : want);
+    pl.row_tiles = tiles * c.heads;
+    pl.most_pieces = pieces;
     pl.partial_floats = (size_t)2 * pl.runs * pl.tile_rows * c.dim;
     pl.stats_floats = (size_t)2 * pl.runs * pl.tile_rows * 2;
     return pl;
@@ -596,14 +595,15 @@ CallShape shape_of(const CacheView& c, int q_heads, int dtype, int window, int s
 template <int NB, bool FP4, int PIECES, int NT>
 int launch_rows(AttentionParams p, const Plan& pl, cudaStream_t st) {
     const int bytes = smem_bytes(p.c.dim, FP4, NT);
-    auto kern = mx_attention_rows_kernel<NB, FP4, PIECES, NT>;
+    constexpr auto kern = mx_attention_rows_kernel<NB, FP4, PIECES, NT>;
     // CTAs on an SM, by registers (launch bounds) and shared memory (2 kB a CTA beside the dynamic part)
     const int by_memory = 228 * 1024 / (bytes + 2048), fit = by_memory < ctas_by_registers(NB, NT) ? (by_memory < 1 ? 1 : by_memory) : ctas_by_registers(NB, NT);
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return check_launch("mx_attention");
+    if (!allow_shared<kern>(bytes)) return check_launch("mx_attention");
     const int most = fit * sm_count();
     p.runs = pl.runs < most ? pl.runs : most;
+    p.whole = pl.row_tiles >= p.runs ? kWhole : 0;
     kern<<<(unsigned)p.runs, 32 * kWarps, bytes, st>>>(p);
-    if (p.runs > 1) mx_attention_join_kernel<kTok><<<dim3((unsigned)(p.runs - 1), (unsigned)(p.tile_rows + 7) / 8), 128, 0, st>>>(p);
+    if (p.runs > 1 && pl.most_pieces > p.whole) launch_after(mx_attention_join_kernel<kTok>, dim3((unsigned)(p.runs - 1), (unsigned)(p.tile_rows + 7) / 8), dim3(128), 0, st, p);
     return check_launch("mx_attention");
 }
 

@@ -1,6 +1,7 @@
 // What the attention kernels share: the call's parameters, how row tiles map to sequences, and which tokens a row sees.
 #pragma once
 #include "blockcodes.cuh"
+#include "launch.cuh"
 
 namespace mpt {
 
@@ -17,6 +18,7 @@ struct AttentionParams {
     int zero_tail;
     int tile_rows;                     // rows of a tile
     int runs, least;                   // CTAs, and pieces of tokens that one takes at least
+    int whole;                         // row tiles of at most so many pieces are not cut
     float *partial, *stats;            // of row tiles that two or more CTAs share: sums [slot, row, dim], and {maximum, sum} of each row
 };
 
@@ -52,7 +54,8 @@ __device__ __forceinline__ bool sees(const AttentionParams& p, int pos, int t) {
 // How the work is shared out.  Row tile t of a sequence has as many pieces of STEP tokens as its last row sees, one at least (so
 // that rows that see nothing are written); the pieces of all (sequence, kv head, row tile) in that order are cut into equal
 // runs, one for each CTA.  A row tile that lies in one run is finished there; of one that is cut each CTA leaves its sums in a
-// slot, which mx_attention_join_kernel joins.
+// slot, which mx_attention_join_kernel joins.  Where there are at least as many row tiles as CTAs, short ones are not cut: an end of
+// a run that falls inside of one moves to its beginning.
 //
 // Without a window row tile t ends at position pos0 + (R (t + 1) - 1) / G (R rows a tile, G query heads a kv head); with
 // pos0 = STEP a + b that makes a + 1 + floor((t + 1 + c) / g) pieces, g = STEP G / R, c = floor((b G - 1) / R), and sums of it
@@ -199,6 +202,33 @@ __device__ __forceinline__ float exp2_fast(float x) {       // relative error 2^
     return y;
 }
 
+// What a CTA has to do of its run: from its beginning, moved as above, as long as take() gives pieces.
+template <int STEP>
+struct RunOf {
+    Place at;
+    int64_t left;
+    bool begins = true;                        // the segment stands at the beginning of the run
+    __device__ __forceinline__ RunOf(const AttentionParams& p, int64_t* sm) {
+        int64_t per;
+        const int64_t total = find_place<STEP>(p, blockIdx.x, per, at, sm);
+        left = min(per, total - blockIdx.x * per);
+        if (left > 0 && at.piece > 0 && at.w.pieces(at.tile) <= p.whole) {
+            left += at.piece;
+            at.piece = 0;
+        }
+    }
+    // pieces of the row tile at `at`, 0 at the end of the run
+    __device__ __forceinline__ int take(const AttentionParams& p, int pieces) const {
+        const int rest = pieces - at.piece;
+        return left >= rest ? rest : left <= 0 || pieces <= p.whole ? 0 : (int)left;
+    }
+    __device__ __forceinline__ void advance(const AttentionParams& p, int took) {
+        left -= took;
+        begins = false;
+        if (left > 0) at.template next_tile<STEP>(p);
+    }
+};
+
 // Joins the row tiles that runs end in: CTAs (x, .) look at the end of run x, where run x + 1 begins.  A warp
 // takes a row.
 template <int STEP>
@@ -210,7 +240,8 @@ __global__ void __launch_bounds__(128) mx_attention_join_kernel(const AttentionP
     int64_t per;
     const int run = blockIdx.x;
     const int64_t total = find_place<STEP>(p, run + 1, per, at, place_sm), cut = (run + 1) * per;
-    if (cut >= total || at.piece == 0) return;                     // nothing is cut here
+    wait_for_previous();                                           // whatever follows: this kernel is not done before the one it follows
+    if (cut >= total || at.piece == 0 || at.w.pieces(at.tile) <= p.whole) return;       // nothing is cut here
     const int64_t p0 = cut - at.piece, p1 = p0 + at.w.pieces(at.tile);
     if (run * per > p0) return;                                    // an earlier CTA joins this one
     const int last = (int)((p1 - 1) / per);

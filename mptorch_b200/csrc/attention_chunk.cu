@@ -42,6 +42,7 @@ __device__ __forceinline__ uint32_t opaque(uint32_t x) {
 // ---- expanding.  One CTA for 128 tokens of a (sequence, kv head).
 template <bool FP4>
 __global__ void __launch_bounds__(256) mx_expand_kernel(const AttentionParams p, uint8_t* __restrict__ tiles, int tiles_per_seq) {
+    next_may_start();
     const CacheView& c = p.c;
     const int head = blockIdx.y, t0 = blockIdx.x * kTile, nb = c.dim >> 5;
     for (int seq = blockIdx.z; seq < c.seqs; seq += gridDim.z) {
@@ -131,12 +132,13 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
     __shared__ uint32_t tmem_slot, failed;
     __shared__ float tops[2][kTile], sums_sm[kTile];
 
+    next_may_start();
     zero_outside(p);
-    Place at;
-    int64_t per;
-    const int64_t total = find_place<kTile>(p, blockIdx.x, per, at, place_sm);
-    int64_t left = min(per, total - blockIdx.x * per);
-    if (left <= 0) return;
+    RunOf<kTile> run(p, place_sm);
+    if (run.left <= 0) {
+        wait_for_previous();                                      // no CTA is done before the kernel that this one follows
+        return;
+    }
 
     auto bar = [&](int i) { return smem_at(&bars[i]); };
     auto wait = [&](int i, uint32_t parity) { return bar_wait(bar(i), parity & 1u, &failed); };
@@ -154,17 +156,16 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
     const float sign = p.scale_log2 > 0.f ? 1.f : p.scale_log2 < 0.f ? -1.f : 0.f;      // of q, so that the largest score is of the largest sum
     const float mul = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
     uint32_t it0 = 0;                                             // pieces before this segment
-    bool begins = true;
-    while (left > 0) {
-        const int seq = at.seq, head = at.head, pieces = at.w.pieces(at.tile);
-        const int take = (int)min((int64_t)(pieces - at.piece), left);
+    while (run.left > 0) {
+        const int seq = run.at.seq, head = run.at.head, pieces = run.at.w.pieces(run.at.tile), take = run.take(p, pieces);
+        if (take == 0) break;
         const int2 own = rows_of(c, seq);
-        const int first = at.tile * kTile, count = min(kTile, own.y * p.group - first);
+        const int first = run.at.tile * kTile, count = min(kTile, own.y * p.group - first);
         const int pos0 = __ldg(c.lens + seq) - own.y;
         const int low_pos = pos0 + first / p.group, high_pos = pos0 + (first + count - 1) / p.group;
         const TokenTiles<kTile> tt(p, low_pos, high_pos);
         const bool finished = take == pieces;
-        const int j_lo = min(at.piece, tt.tiles), n = min(at.piece + take, tt.tiles) - j_lo;
+        const int j_lo = min(run.at.piece, tt.tiles), n = min(run.at.piece + take, tt.tiles) - j_lo;
 
         // ---- q, in pieces
 #pragma unroll 1
@@ -201,6 +202,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
 
         if (warp == 8) {
             if (lane == 0) {
+                if (run.begins) wait_for_previous();                  // the expanded tiles
                 const uint8_t* from = tiles + ((int64_t)seq * c.heads + head) * tiles_per_seq * tile_bytes(DIM);
                 for (int i = 0; i < n; ++i) {
                     const uint32_t it = it0 + i;
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
             // ---- the row's result, or its share
             const int rr = first + r, tok = rr / p.group;
             const int64_t out_row = ((int64_t)(own.x + tok) * p.q_heads + head * p.group + rr - tok * p.group) * DIM;
-            const int share = 2 * blockIdx.x + (begins ? 0 : 1);
+            const int share = 2 * blockIdx.x + (run.begins ? 0 : 1);
             const float times = !ok ? __uint_as_float(0x7FC00000u) : finished ? (l == 0.f ? 0.f : __frcp_rn(l)) : 1.f;
 #pragma unroll 1
             for (int b = 16 * half; b < DIM; b += 32) {           // the halves take blocks of 16 columns in turn
@@ -417,9 +419,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
         tmem_fence_after();
         if (failed) break;
         it0 += n;
-        left -= take;
-        begins = false;
-        if (left > 0) at.next_tile<kTile>(p);
+        run.advance(p, take);
     }
     if (failed && warp == 8 && lane == 0) {                       // copies on the way write to this CTA's memory
         failed = 0u;
@@ -433,13 +433,14 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
 template <int DIM, int PIECES, int NS>
 int launch(AttentionParams p, const ChunkPlan& pl, uint8_t* tiles, cudaStream_t st) {
     using Shape = ChunkShape<DIM, PIECES, NS>;
-    auto kern = mx_attention_chunk_kernel<DIM, PIECES, NS>;
+    constexpr auto kern = mx_attention_chunk_kernel<DIM, PIECES, NS>;
     // CTAs on an SM, by tensor memory (512 columns), shared memory (3 kB a CTA beside the dynamic part) and registers (launch bounds)
     const int fit = Shape::columns == 256 && 2 * (Shape::smem + 3 * 1024) <= 228 * 1024 && NS == 1 && PIECES == 1 ? 2 : 1;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem) != cudaSuccess) return check_launch("mx_attention");
+    if (!allow_shared<kern>(Shape::smem)) return check_launch("mx_attention");
     p.runs = pl.runs < fit * sm_count() ? pl.runs : fit * sm_count();
-    kern<<<(unsigned)p.runs, kThreads, Shape::smem, st>>>(p, tiles, pl.tiles_per_seq);
-    if (p.runs > 1) mx_attention_join_kernel<kTile><<<dim3((unsigned)(p.runs - 1), kTile / 8), 128, 0, st>>>(p);
+    p.whole = 0;
+    launch_after(kern, dim3((unsigned)p.runs), dim3(kThreads), Shape::smem, st, p, tiles, pl.tiles_per_seq);
+    if (p.runs > 1) launch_after(mx_attention_join_kernel<kTile>, dim3((unsigned)(p.runs - 1), kTile / 8), dim3(128), 0, st, p);
     return check_launch("mx_attention");
 }
 

@@ -14,6 +14,7 @@
 //
 // Measured figures stand at the launch rule below.
 #include "blocklinear.cuh"
+#include "launch.cuh"
 
 namespace mpt {
 namespace {
@@ -351,8 +352,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const 
 template <bool NV, int PIECES, int NT, bool GROUPS>
 int launch_few(const LinearParams& p, cudaStream_t st) {
     const int bytes = few_smem(p.n_in, p.rows * PIECES, NV, NT), tiles = (p.n_out + 15) / 16;
-    auto kern = block_linear_few_kernel<NV, PIECES, NT, GROUPS>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return check_launch("block_linear");
+    constexpr auto kern = block_linear_few_kernel<NV, PIECES, NT, GROUPS>;
+    if (!allow_shared<kern>(220 * 1024)) return check_launch("block_linear");
     // One CTA on each SM.  As many warps share a tile as take the least time: rounds of tiles times pieces of a warp, with two for the end.
     const int chunks = (p.n_in + kChunk - 1) / kChunk;
     int share = 1;

@@ -1,6 +1,8 @@
 // Kernels of one call that follow one another: the second may start while the first still runs, does what does not depend on it, and
 // then waits for it (programmatic dependent launch).
 #pragma once
+#include <atomic>
+
 #include "common.cuh"
 
 namespace mpt {
@@ -8,6 +10,19 @@ namespace mpt {
 // In the first kernel: the next one may start.  In the second: everything the first one wrote is visible from here on.
 __device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Allows `Kern` up to `bytes` of dynamic shared memory, asked of the runtime once for each device.
+template <auto Kern>
+bool allow_shared(int bytes) {
+    static std::atomic<uint64_t> asked{0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    const uint64_t bit = (uint64_t)1 << dev;
+    if (asked.load(std::memory_order_relaxed) & bit) return true;
+    if (cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    asked.fetch_or(bit, std::memory_order_relaxed);
+    return true;
+}
 
 // Launches `kern` so that it may start before the kernel launched just before it on the stream is done.
 template <typename... P, typename... A>

@@ -156,7 +156,10 @@ __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_con
     uint8_t* smem = smem_raw + (base - smem_at(smem_raw));
     const int x_bytes = p.pieces * p.cols * 128, x_base = p.w_stages * PER * kPartW;
     const int64_t u0 = blockIdx.x * p.per, u1 = u0 + p.per < p.units ? u0 + p.per : p.units;
-    if (u0 >= u1) return;
+    if (u0 >= u1) {
+        wait_for_previous();                                       // no CTA is done before the kernel that this one follows
+        return;
+    }
     __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 16 + 4];
     __shared__ uint32_t tmem_slot, failed;
     __shared__ int top_e[2][kRowsW];
@@ -447,9 +450,21 @@ int launch_tiles(const LinearParams& l, const TilesPlan& pl, int format, uint8_t
     linear_split_kernel<<<(unsigned)l.rows, 256, 0, st>>>(p, workspace);
     const int bytes = 1024 + pl.ring_blocks * (pl.w_stages * kPartW + pl.x_stages * pl.pieces * pl.cols * 128);
     const bool nv = format == MPT_BLOCK_NVFP4, single = pl.ring_blocks == 1;
-    auto kern = nv ? (single ? linear_tiles_kernel<true, 1> : linear_tiles_kernel<true, kSuper>) : (single ? linear_tiles_kernel<false, 1> : linear_tiles_kernel<false, kSuper>);
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return check_launch("block_linear");
-    launch_after(kern, dim3((unsigned)pl.runs), dim3(kThreads), bytes, st, p);
+    constexpr int most = 221 * 1024;                               // beside 3 kB of its own
+    auto launch = [&](auto kern, bool allowed) {
+        if (!allowed) return false;
+        launch_after(kern, dim3((unsigned)pl.runs), dim3(kThreads), bytes, st, p);
+        return true;
+    };
+    const bool fine = nv ? (single ? launch(linear_tiles_kernel<true, 1>, allow_shared<linear_tiles_kernel<true, 1>>(most))
+                                   : launch(linear_tiles_kernel<true, kSuper>, allow_shared<linear_tiles_kernel<true, kSuper>>(most)))
+                         : (single ? launch(linear_tiles_kernel<false, 1>, allow_shared<linear_tiles_kernel<false, 1>>(most))
+                                   : launch(linear_tiles_kernel<false, kSuper>, allow_shared<linear_tiles_kernel<false, kSuper>>(most)));
+    if (!fine) {
+        check_launch("block_linear");
+        set_error("block_linear: the kernel does not fit this device");
+        return MPT_ERR_CUDA;
+    }
     if (pl.partial_bytes) launch_after(linear_join_kernel, dim3((unsigned)(pl.runs - 1), 4), dim3(256), 0, st, p);
     return check_launch("block_linear");
 }
