@@ -11,10 +11,11 @@ import torch
 import torch.nn as nn
 
 from .number import FloatingPoint
-from .quant import QAffineFormats, QLayerNorm, QLayerNormFormats, QLinear, QSoftmax, QSoftmaxFormats
+from .quant import (MXCache, QAffineFormats, QLayerNorm, QLayerNormFormats, QLinear, QPackedLinear, QSoftmax, QSoftmaxFormats, mx_attention,
+                    mx_cache_write)
 from .quant.functional import qmatmul
 
-__all__ = ["BlockConfig", "QBlock", "QTinyGPT", "default_formats"]
+__all__ = ["BlockConfig", "QBlock", "QTinyGPT", "ServedBlock", "ServedGPT", "default_formats"]
 
 
 class BlockConfig:
@@ -86,3 +87,56 @@ class QTinyGPT(nn.Module):
         rows = batch * seq
         fwd = rows * c.d_model * (3 * c.d_model + c.d_model + 2 * c.d_mlp) + 2 * batch * c.n_head * seq * seq * (c.d_model // c.n_head)
         return 3 * fwd
+
+
+class ServedBlock(nn.Module):
+    """A trained ``QBlock`` as it answers: the four weights packed in a 4-bit block format, K and V in the pages of an MX cache.
+    New tokens come in chunks or one by one; ``pages``, ``lens`` and ``starts`` are those of ``quant.mx_attention``."""
+
+    def __init__(self, block: QBlock, weights: str = "mxfp4"):
+        super().__init__()
+        self.n_head, self.ln1, self.ln2 = block.cfg.n_head, block.ln1, block.ln2
+        self.qkv, self.proj, self.fc, self.out = (QPackedLinear.from_linear(m, weights) for m in (block.qkv, block.proj, block.fc, block.out))
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor, cache: MXCache, pages: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor | None = None) -> torch.Tensor:
+        q, k, v = (t.unflatten(-1, (self.n_head, -1)) for t in self.qkv(self.ln1(x)).chunk(3, dim=-1))
+        mx_cache_write(k, v, cache, pages, lens, starts)
+        x = x + self.proj(mx_attention(q, cache, pages, lens, starts).flatten(-2))
+        return x + self.out(torch.nn.functional.gelu(self.fc(self.ln2(x))))
+
+
+class ServedGPT(nn.Module):
+    """A trained ``QTinyGPT`` as it answers: ``ServedBlock`` between the embeddings and the (tied) packed vocabulary head."""
+
+    def __init__(self, model: QTinyGPT, weights: str = "mxfp4"):
+        super().__init__()
+        self.cfg, self.wte, self.wpe = model.cfg, model.wte, model.wpe
+        self.block = ServedBlock(model.block, weights)
+        self.head = QPackedLinear(model.wte.weight, None, weights)
+
+    def new_cache(self, pages: int, page: int = 64, elem_format: str = "e4m3") -> MXCache:
+        return MXCache.empty(pages, self.cfg.n_head, self.cfg.d_model // self.cfg.n_head, page, elem_format, self.wte.weight.device)
+
+    @torch.no_grad()
+    def forward(self, idx: torch.Tensor, cache: MXCache, pages: torch.Tensor, lens: torch.Tensor) -> torch.Tensor:
+        """Logits of the new tokens ``idx`` [sequences, new]; ``lens`` counts each sequence with them."""
+        at = lens[:, None] - idx.shape[1] + torch.arange(idx.shape[1], device=idx.device)
+        x = self.wte(idx) + self.wpe(at.clamp(0, self.cfg.seq_len - 1))
+        return self.head(self.block(x, cache, pages, lens))
+
+    @torch.no_grad()
+    def generate(self, idx: torch.Tensor, new: int, page: int = 64, elem_format: str = "e4m3") -> torch.Tensor:
+        """The most likely continuation of prompts of one length: [sequences, prompt + new] tokens."""
+        b, t = idx.shape
+        if t < 1 or t + new > self.cfg.seq_len:
+            raise ValueError("prompt and continuation must fit seq_len")
+        width = -(-(t + new) // page)
+        cache = self.new_cache(b * width, page, elem_format)
+        pages = torch.arange(b * width, device=idx.device, dtype=torch.int32).view(b, width)
+        lens, chunk = torch.full((b,), t, device=idx.device, dtype=torch.int32), idx
+        for _ in range(new):
+            chunk = self(chunk, cache, pages, lens)[:, -1].argmax(-1, keepdim=True)
+            idx = torch.cat([idx, chunk], dim=1)
+            lens = lens + 1
+        return idx

@@ -4,7 +4,7 @@ Subclasses of the corresponding ``torch.nn`` layers (so ``state_dict`` layouts a
 arguments and behaviour of the reference's ``mptorch/quant/modules``: ``QLinear`` (linear.py:12-135), ``QSoftmax``
 (softmax.py:14-94), ``QLayerNorm`` (layernorm.py:13-172), ``QConv2d`` (conv.py:326-640, as unfold + qlinear) and
 ``Quantizer`` (quantizer.py:8).  Transposed / 1-D / 3-D convolutions, batch norm, GELU and pooling of the reference
-are not on the accelerated path and are not provided.
+are not on the accelerated path and are not provided.  ``QPackedLinear``, new, answers with weights in a 4-bit block format.
 """
 from __future__ import annotations
 
@@ -17,9 +17,10 @@ import torch.nn.functional as F
 from ..number import Number
 from .functional import implicit_conv_eligible, qconv2d, qlayernorm, qlinear, qsoftmax
 from .quant_format import QAffineFormats, QLayerNormFormats, QSoftmaxFormats
-from .quant_function import quantizer
+from .quant_function import mx_quantize, nvfp4_quantize, quantizer
+from .serving import mx_linear, nvfp4_linear
 
-__all__ = ["Quantizer", "QLinear", "QLazyLinear", "QConv2d", "QLayerNorm", "QSoftmax"]
+__all__ = ["Quantizer", "QLinear", "QLazyLinear", "QConv2d", "QLayerNorm", "QSoftmax", "QPackedLinear"]
 
 
 def ste_function(fwd_quant: Callable[[torch.Tensor], torch.Tensor], bwd_quant: Callable[[torch.Tensor], torch.Tensor]):
@@ -196,3 +197,39 @@ class QLayerNorm(nn.LayerNorm, _QuantSignals):
             return self.Qo(F.layer_norm(self.Qi(input), list(self.normalized_shape), self.Qw(self.weight), self.Qb(self.bias), self.eps))
         return qlayernorm(input, normalized_shape=list(self.normalized_shape), weight=self.weight, bias=self.bias,
                           eps=self.eps, formats=self.formats)
+
+
+class QPackedLinear(nn.Module):
+    """A linear layer that answers with its weight in MXFP4 or NVFP4: the packed codes and scales are its buffers, and nothing of
+    the dense weight is kept.  Made from a layer (``from_linear``); it has no backward pass."""
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None, fmt: str = "mxfp4") -> None:
+        super().__init__()
+        if fmt not in ("mxfp4", "nvfp4"):
+            raise ValueError("fmt must be 'mxfp4' or 'nvfp4'")
+        if weight.dim() != 2 or weight.shape[1] % 32:
+            raise ValueError("the weight must be [out, in] with in a multiple of 32")
+        self.fmt, (self.out_features, self.in_features) = fmt, weight.shape
+        weight = weight.detach()
+        if fmt == "mxfp4":
+            _, scales, codes = mx_quantize(weight, "e2m1", 32, return_scales=True, return_codes=True)
+            self.register_buffer("global_scale", None)
+        else:
+            _, _, glob, codes, scales = nvfp4_quantize(weight, None, return_scales=True, return_codes=True)
+            self.register_buffer("global_scale", glob)
+        self.register_buffer("codes", codes)
+        self.register_buffer("scales", scales)
+        self.register_buffer("bias", None if bias is None else bias.detach().clone())
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, fmt: str = "mxfp4") -> "QPackedLinear":
+        return cls(linear.weight, linear.bias, fmt)
+
+    def extra_repr(self) -> str:
+        return "in_features=%d, out_features=%d, bias=%s, fmt=%s" % (self.in_features, self.out_features, self.bias is not None, self.fmt)
+
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        bias = None if self.bias is None else self.bias.to(input.dtype)
+        if self.fmt == "mxfp4":
+            return mx_linear(input, self.codes, self.scales, bias)
+        return nvfp4_linear(input, self.codes, self.scales, self.global_scale, bias)
