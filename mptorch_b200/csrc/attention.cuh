@@ -108,10 +108,10 @@ struct Place {
     }
 };
 
-constexpr int kPlaceWords = 8 + (sizeof(Place) + 7) / 8;
+constexpr int kPlaceWords = 16 + (sizeof(Place) + 7) / 8;
 
 // Finds where run `run` begins (`place` means nothing behind the last one); `per`: pieces of a run; returns the number of all
-// pieces.  Called by whole blocks of up to 256 threads; `sm` has room for kPlaceWords.
+// pieces.  Called by whole blocks of up to 512 threads; `sm` has room for kPlaceWords.
 template <int STEP>
 __device__ __forceinline__ int64_t find_place(const AttentionParams& p, int run, int64_t& per, Place& place, int64_t* sm) {
     const int each = (p.c.seqs + blockDim.x - 1) / blockDim.x, s0 = min((int)threadIdx.x * each, p.c.seqs), s1 = min(s0 + each, p.c.seqs);
@@ -138,7 +138,7 @@ __device__ __forceinline__ int64_t find_place(const AttentionParams& p, int run,
     upto += before;
     per = max((total + p.runs - 1) / p.runs, (int64_t)p.least);
     const int64_t at = run * per;
-    Place* out = reinterpret_cast<Place*>(sm + 8);
+    Place* out = reinterpret_cast<Place*>(sm + 16);
     if (at >= upto - mine && at < upto) {
         int64_t rest = at - (upto - mine);
         for (int s = s0; s < s1; ++s) {
@@ -146,8 +146,13 @@ __device__ __forceinline__ int64_t find_place(const AttentionParams& p, int run,
             const int64_t head = w.upto(w.tiles);
             if (rest < head * p.c.heads) {
                 out->seq = s;
-                out->head = (int)(rest / head);
-                rest %= head;
+                if (head * p.c.heads <= 0x7FFFFFFF) {
+                    out->head = (int)((uint32_t)rest / (uint32_t)head);
+                    rest = (uint32_t)rest % (uint32_t)head;
+                } else {
+                    out->head = (int)(rest / head);
+                    rest %= head;
+                }
                 int lo = 0, hi = w.tiles - 1;                      // the last tile that begins at or before it
                 while (lo < hi) {
                     const int mid = (lo + hi + 1) >> 1;
@@ -232,7 +237,7 @@ struct RunOf {
 // Joins the row tiles that runs end in: CTAs (x, .) look at the end of run x, where run x + 1 begins.  A warp
 // takes a row.
 template <int STEP>
-__global__ void __launch_bounds__(128) mx_attention_join_kernel(const AttentionParams p) {
+__global__ void __launch_bounds__(512) mx_attention_join_kernel(const AttentionParams p) {
     const CacheView& c = p.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = c.dim, nb = dim >> 5;
     __shared__ int64_t place_sm[kPlaceWords];
@@ -248,7 +253,8 @@ __global__ void __launch_bounds__(128) mx_attention_join_kernel(const AttentionP
     const int2 own = rows_of(c, at.seq);
     const int first = at.tile * p.tile_rows, count = min(p.tile_rows, own.y * p.group - first);
     auto slot_of = [&](int k) { return 2 * k + (k == run && run * per < p0 ? 1 : 0); };
-    for (int r = warp + 4 * blockIdx.y; r < count; r += 4 * gridDim.y) {
+    const int warps = blockDim.x >> 5;
+    for (int r = warp + warps * blockIdx.y; r < count; r += warps * gridDim.y) {
         float top = -INFINITY;
         for (int k = run + lane; k <= last; k += 32) top = fmaxf(top, p.stats[(slot_of(k) * p.tile_rows + r) * 2]);
 #pragma unroll

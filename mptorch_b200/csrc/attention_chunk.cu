@@ -69,29 +69,41 @@ __global__ void __launch_bounds__(256) mx_expand_kernel(const AttentionParams p,
             if (bad) any_nan = 1u;
         }
         __syncthreads();
-        const int pieces = c.dim >> 3, row_bytes = FP4 ? c.dim >> 1 : c.dim;
-        for (int i = threadIdx.x; i < kTile * pieces; i += 256) {
-            const int tok = i / pieces, ch = i - tok * pieces;
-            const int64_t row = row_at[tok];
-            const int at = (ch >> 3) * kPart + tok * 128 + (((ch & 7) ^ (tok & 7)) << 4);
-#pragma unroll
-            for (int side = 0; side < 2; ++side) {
-                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        // a thread keeps its piece of eight values and goes through the tokens
+        const int pieces = c.dim >> 3, row_bytes = FP4 ? c.dim >> 1 : c.dim, step = 256 / pieces, ch = threadIdx.x % pieces, first = threadIdx.x / pieces;
+        const int side_bytes = parts_for(c.dim) * kPart;
+        if (first < step) {
+#pragma unroll 2
+            for (int tok = first; tok < kTile; tok += step) {
+                const int64_t row = row_at[tok];
+                const int64_t at = max(row, (int64_t)0);
+                const uint8_t *kf = c.k_codes + at * row_bytes + (FP4 ? ch * 4 : ch * 8), *vf = c.v_codes + at * row_bytes + (FP4 ? ch * 4 : ch * 8);
+                uint2 kw = make_uint2(0u, 0u), vw = kw;
+                uint32_t ks = 0u, vs = 0u;
                 if (row >= 0) {
-                    const uint8_t* from = (side ? c.v_codes : c.k_codes) + row * row_bytes + (FP4 ? ch * 4 : ch * 8);
-                    const uint32_t sc = __ldg((side ? c.v_scales : c.k_scales) + row * nb + (ch >> 2));
-                    uint2 w;
-                    if (FP4) w = make_uint2(__ldg(reinterpret_cast<const uint32_t*>(from)), 0u);
-                    else w = __ldg(reinterpret_cast<const uint2*>(from));
-                    decode8<FP4>(w, x);
-                    const float s = e8m0_value(sc);
-                    // a block of V that is NaN takes no part in the product; its rows are told at the end
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = side && sc == 255u ? 0.f : x[e] * s;
+                    if (FP4) {
+                        kw.x = __ldg(reinterpret_cast<const uint32_t*>(kf));
+                        vw.x = __ldg(reinterpret_cast<const uint32_t*>(vf));
+                    } else {
+                        kw = __ldg(reinterpret_cast<const uint2*>(kf));
+                        vw = __ldg(reinterpret_cast<const uint2*>(vf));
+                    }
+                    ks = __ldg(c.k_scales + at * nb + (ch >> 2));
+                    vs = __ldg(c.v_scales + at * nb + (ch >> 2));
                 }
-                uint4 v;
-                v.x = pack_bf16(x[0], x[1]); v.y = pack_bf16(x[2], x[3]); v.z = pack_bf16(x[4], x[5]); v.w = pack_bf16(x[6], x[7]);
-                *reinterpret_cast<uint4*>(out + side * parts_for(c.dim) * kPart + at) = v;
+                uint8_t* to = out + (ch >> 3) * kPart + tok * 128 + (((ch & 7) ^ (tok & 7)) << 4);
+                auto put = [&](uint2 w, float s, uint8_t* to) {
+                    float x[8];
+                    decode8<FP4>(w, x);
+                    uint4 v;
+                    v.x = pack_bf16(x[0] * s, x[1] * s); v.y = pack_bf16(x[2] * s, x[3] * s);
+                    v.z = pack_bf16(x[4] * s, x[5] * s); v.w = pack_bf16(x[6] * s, x[7] * s);
+                    *reinterpret_cast<uint4*>(to) = v;
+                };
+                put(kw, e8m0_value(ks), to);
+                // a block of V that is NaN takes no part in the product; its rows are told at the end
+                if (vs == 255u) vw = make_uint2(0u, 0u);
+                put(vw, vs == 255u ? 0.f : e8m0_value(vs), to + side_bytes);
             }
         }
         uint32_t* tail = reinterpret_cast<uint32_t*>(out + 2 * parts_for(c.dim) * kPart);
@@ -244,8 +256,8 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
                     const uint32_t it = it0 + i;
                     if (NS == 2 && i + 1 < n && !(ok = scores(i + 1))) break;
                     const uint32_t turn = NS == 2 ? it & 1 : 0;
-                    if (!(ok = wait(turn ? kWeights2 : kWeights, NS == 2 ? it >> 1 : it))) break;
                     if (!(ok = wait(kVFull, it))) break;
+                    if (!(ok = wait(turn ? kWeights2 : kWeights, NS == 2 ? it >> 1 : it))) break;
                     tmem_fence_after();
                     const uint64_t v_desc = tile_descriptor(opaque(v_at), kPart);
 #pragma unroll
@@ -264,6 +276,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
             __syncwarp();
         } else {
             const int half = warp >> 2, r = threadIdx.x & (kTile - 1);   // this thread's row, and its half of the tokens
+            auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory"); };      // the two warps of the same rows
             const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
             const int pos = r < count ? pos0 + (first + r) / p.group : -1;
             float m = -INFINITY, l = 0.f;
@@ -308,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
                 // the other half's; from here on the scores' columns are free
                 tops[half][r] = top;
                 tmem_fence_before();
-                asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads) : "memory");
+                pair_sync();
                 tmem_fence_after();
                 top = fmaxf(top, tops[half ^ 1][r]) * mul;
                 if (__any_sync(0xFFFFFFFFu, top > m + 8.f)) {
@@ -365,10 +378,10 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
             if (n > 0) wait(kValues, it0 + n - 1);
             if (half) sums_sm[r] = l;
             __syncwarp();
-            asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads) : "memory");
+            pair_sync();
             tmem_fence_after();
             if (!half) sums_sm[r] = l += sums_sm[r];
-            asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads) : "memory");
+            pair_sync();
             l = sums_sm[r];
             const bool ok = *(volatile uint32_t*)&failed == 0u;
             // ---- the row's result, or its share
@@ -440,7 +453,7 @@ int launch(AttentionParams p, const ChunkPlan& pl, uint8_t* tiles, cudaStream_t 
     p.runs = pl.runs < fit * sm_count() ? pl.runs : fit * sm_count();
     p.whole = 0;
     launch_after(kern, dim3((unsigned)p.runs), dim3(kThreads), Shape::smem, st, p, tiles, pl.tiles_per_seq);
-    if (p.runs > 1) launch_after(mx_attention_join_kernel<kTile>, dim3((unsigned)(p.runs - 1), kTile / 8), dim3(128), 0, st, p);
+    if (p.runs > 1) launch_after(mx_attention_join_kernel<kTile>, dim3((unsigned)(p.runs - 1), 2), dim3(512), 0, st, p);
     return check_launch("mx_attention");
 }
 
