@@ -25,7 +25,7 @@ namespace {
 #define MPT_ATT_WARPS 4
 #define MPT_ATT_LEAST 8
 #define MPT_ATT_WHOLE 64
-#define MPT_ATT_CHUNK 40
+#define MPT_ATT_CHUNK 32
 #endif
 constexpr int kWarps = MPT_ATT_WARPS, kTok = 32, kLeast = MPT_ATT_LEAST, kWhole = MPT_ATT_WHOLE;
 
@@ -603,7 +603,7 @@ int launch_rows(AttentionParams p, const Plan& pl, cudaStream_t st) {
     p.runs = pl.runs < most ? pl.runs : most;
     p.whole = pl.row_tiles >= p.runs ? kWhole : 0;
     kern<<<(unsigned)p.runs, 32 * kWarps, bytes, st>>>(p);
-    if (p.runs > 1 && pl.most_pieces > p.whole) launch_after(mx_attention_join_kernel<kTok>, dim3((unsigned)(p.runs - 1), (unsigned)(p.tile_rows + 7) / 8), dim3(128), 0, st, p);
+    if (p.runs > 1 && pl.most_pieces > p.whole) launch_after(mx_attention_join_kernel<kTok>, dim3((unsigned)(p.runs - 1), (unsigned)(p.tile_rows + 3) / 4), dim3(128), 0, st, p);
     return check_launch("mx_attention");
 }
 

@@ -255,20 +255,34 @@ __global__ void __launch_bounds__(512) mx_attention_join_kernel(const AttentionP
     auto slot_of = [&](int k) { return 2 * k + (k == run && run * per < p0 ? 1 : 0); };
     const int warps = blockDim.x >> 5;
     for (int r = warp + warps * blockIdx.y; r < count; r += warps * gridDim.y) {
-        float top = -INFINITY;
-        for (int k = run + lane; k <= last; k += 32) top = fmaxf(top, p.stats[(slot_of(k) * p.tile_rows + r) * 2]);
+        // 32 parts at a time: a lane has the statistics of one, and the sums follow without waiting for one another
+        float top = -INFINITY, sum = 0.f, v[8] = {};
+        for (int k0 = run; k0 <= last; k0 += 32) {
+            const int k = k0 + lane;
+            float2 st = make_float2(-INFINITY, 0.f);
+            if (k <= last) st = *reinterpret_cast<const float2*>(p.stats + ((int64_t)slot_of(k) * p.tile_rows + r) * 2);
+            float here = fmaxf(top, st.x);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        float sum = 0.f, v[8] = {};
-        for (int k = run; k <= last; ++k) {
-            const int slot = slot_of(k);
-            const float* st = p.stats + (slot * p.tile_rows + r) * 2;
-            const float w = st[0] == -INFINITY ? (st[1] != st[1] ? st[1] : 0.f) : exp2_fast(st[0] - top);   // a NaN sum stays one
-            sum = fmaf(st[1], w, sum);
-            const float* from = p.partial + ((int64_t)slot * p.tile_rows + r) * dim + lane;
+            for (int o = 16; o > 0; o >>= 1) here = fmaxf(here, __shfl_xor_sync(0xFFFFFFFFu, here, o));
+            const float fade = top == -INFINITY ? (sum != sum ? sum : 0.f) : exp2_fast(top - here);
+            const float w = st.x == -INFINITY ? (st.y != st.y ? st.y : 0.f) : exp2_fast(st.x - here);       // a NaN sum stays one
+            float add = st.y * w;
 #pragma unroll
-            for (int b = 0; b < 8; ++b)
-                if (b < nb) v[b] = fmaf(from[b * 32], w, v[b]);
+            for (int o = 16; o > 0; o >>= 1) add += __shfl_xor_sync(0xFFFFFFFFu, add, o);
+            sum = k0 == run ? add : fmaf(sum, fade, add);
+            if (k0 != run)
+#pragma unroll
+                for (int b = 0; b < 8; ++b) v[b] *= fade;
+            top = here;
+            const int n = min(32, last - k0 + 1);
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) {
+                const float wj = __shfl_sync(0xFFFFFFFFu, w, j);
+                const float* from = p.partial + ((int64_t)slot_of(k0 + j) * p.tile_rows + r) * dim + lane;
+#pragma unroll
+                for (int b = 0; b < 8; ++b)
+                    if (b < nb) v[b] = fmaf(from[b * 32], wj, v[b]);
+            }
         }
         const int rr = first + r, i = rr / p.group;
         const int64_t out_row = ((int64_t)(own.x + i) * p.q_heads + at.head * p.group + rr - i * p.group) * dim;

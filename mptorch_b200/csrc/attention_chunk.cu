@@ -34,11 +34,6 @@ __device__ __forceinline__ float bf16_lo(uint32_t x) { return __uint_as_float(x 
 __device__ __forceinline__ float bf16_hi(uint32_t x) { return __uint_as_float(x & 0xFFFF0000u); }
 
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }   // the lowest n bits
-__device__ __forceinline__ uint32_t opaque(uint32_t x) {
-    asm volatile("" : "+r"(x));
-    return x;
-}
-
 // ---- expanding.  One CTA for 128 tokens of a (sequence, kv head).
 template <bool FP4>
 __global__ void __launch_bounds__(256) mx_expand_kernel(const AttentionParams p, uint8_t* __restrict__ tiles, int tiles_per_seq) {
@@ -230,25 +225,26 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
             }
             __syncwarp();
         } else if (warp == 9) {
-            if (lane == 0) {
+            {
+                const bool leader = lane == 0;
+                const uint32_t tm = uniform(tmem), q_u = uniform(q_at), k_u = uniform(k_at), v_u = uniform(v_at);
                 constexpr uint32_t score_desc = product_descriptor(128, false), value_desc = product_descriptor(DIM, true);
                 auto scores = [&](int i) -> bool {
                     const uint32_t it = it0 + i;
-                    if (!wait(kKFull, it)) return false;
+                    if (!__all_sync(0xFFFFFFFFu, wait(kKFull, it))) return false;
                     // the columns are free when the product that read the weights in them is done (the segment before is done)
-                    if (i >= NS && !wait(kValues, it - NS)) return false;
+                    if (i >= NS && !__all_sync(0xFFFFFFFFu, wait(kValues, it - NS))) return false;
                     tmem_fence_after();
-                    // (addresses are opaque to the compiler, which would keep every descriptor in registers of its own)
-                    const uint64_t q_desc = tile_descriptor(opaque(q_at), 16), k_desc = tile_descriptor(opaque(k_at), 16);
-                    const uint32_t to = tmem + (NS == 2 ? (it & 1) * 128 : 0);
+                    const uint64_t q_desc = tile_descriptor(q_u, 16), k_desc = tile_descriptor(k_u, 16);
+                    const uint32_t to = tm + (NS == 2 ? (it & 1) * 128 : 0);
 #pragma unroll
                     for (int k = 0; k < PIECES; ++k)
 #pragma unroll
                         for (int s = 0; s < DIM / 16; ++s)
                             mma_ss(to, q_desc + (((k * Shape::parts + (s >> 2)) * kPart + (s & 3) * 32) >> 4), k_desc + (((s >> 2) * kPart + (s & 3) * 32) >> 4), score_desc,
-                                   k + s > 0);
-                    mma_commit(bar(NS == 2 && (it & 1) ? kScores2 : kScores));
-                    mma_commit(bar(kKEmpty));
+                                   k + s > 0, leader);
+                    mma_commit(bar(NS == 2 && (it & 1) ? kScores2 : kScores), leader);
+                    mma_commit(bar(kKEmpty), leader);
                     return true;
                 };
                 bool ok = n == 0 || scores(0);
@@ -256,20 +252,20 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
                     const uint32_t it = it0 + i;
                     if (NS == 2 && i + 1 < n && !(ok = scores(i + 1))) break;
                     const uint32_t turn = NS == 2 ? it & 1 : 0;
-                    if (!(ok = wait(kVFull, it))) break;
-                    if (!(ok = wait(turn ? kWeights2 : kWeights, NS == 2 ? it >> 1 : it))) break;
+                    if (!(ok = __all_sync(0xFFFFFFFFu, wait(kVFull, it)))) break;
+                    if (!(ok = __all_sync(0xFFFFFFFFu, wait(turn ? kWeights2 : kWeights, NS == 2 ? it >> 1 : it)))) break;
                     tmem_fence_after();
-                    const uint64_t v_desc = tile_descriptor(opaque(v_at), kPart);
+                    const uint64_t v_desc = tile_descriptor(v_u, kPart);
 #pragma unroll
                     for (int k = 0; k < PIECES; ++k) {
-                        const uint32_t w = tmem + (k < 2 ? turn * 128 + k * 64 : Shape::more + turn * 64);
+                        const uint32_t w = tm + (k < 2 ? turn * 128 + k * 64 : Shape::more + turn * 64);
 #pragma unroll
                         for (int s = 0; s < 8; ++s)
-                            mma_ts(tmem + (PIECES == 3 && k > 0 ? Shape::small : Shape::sums), w + s * 8, v_desc + (s * 2048 >> 4), value_desc,
-                                   i > 0 || s > 0 || k > (PIECES == 3 ? 1 : 0));
+                            mma_ts(tm + (PIECES == 3 && k > 0 ? Shape::small : Shape::sums), w + s * 8, v_desc + (s * 2048 >> 4), value_desc,
+                                   i > 0 || s > 0 || k > (PIECES == 3 ? 1 : 0), leader);
                     }
-                    mma_commit(bar(kValues));
-                    mma_commit(bar(kVEmpty));
+                    mma_commit(bar(kValues), leader);
+                    mma_commit(bar(kVEmpty), leader);
                     if (NS == 1 && i + 1 < n) ok = scores(i + 1);
                 }
             }

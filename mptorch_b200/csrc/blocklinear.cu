@@ -19,7 +19,10 @@
 namespace mpt {
 namespace {
 
-constexpr int kWarps = 16, kChunk = 128, kPitch = 80, kStages = 4;          // pitch: eight rows of four words meet no bank twice
+#ifndef MPT_FEW_COLUMNS
+#define MPT_FEW_COLUMNS 16
+#endif
+constexpr int kWarps = 16, kChunk = 128, kPitch = 80, kStages = 3;          // pitch: eight rows of four words meet no bank twice
 
 __device__ __forceinline__ void cp_bytes(uint32_t dst, const void* src, int bytes) {   // 16
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes));
@@ -369,7 +372,7 @@ int launch_few(const LinearParams& p, cudaStream_t st) {
 // Few rows: at most 16 columns (a float32 row takes two), x within the shared memory beside the rings.
 bool few_rows(int64_t rows, int64_t n_in, int dtype) {
     const int64_t columns = rows * (dtype == MPT_DTYPE_F32 ? 2 : 1);
-    return columns <= 16 && n_in <= 65536 && columns * x_pitch((int)n_in) <= 112 * 1024;
+    return columns <= MPT_FEW_COLUMNS && n_in <= 65536 && columns * x_pitch((int)n_in) <= 140 * 1024;
 }
 
 }  // namespace

@@ -21,7 +21,10 @@
 namespace mpt {
 namespace {
 
-constexpr int kRowsW = 128, kBlock = 64, kSuper = 4, kWorkers = 512, kThreads = kWorkers + 64;   // codes are read in pieces of four blocks
+#ifndef MPT_TILE_WORKERS
+#define MPT_TILE_WORKERS 512
+#endif
+constexpr int kRowsW = 128, kBlock = 64, kSuper = 4, kWorkers = MPT_TILE_WORKERS, kThreads = kWorkers + 64, kRowStep = kWorkers / 8, kEach = kRowsW / kRowStep;   // codes are read in pieces of four blocks
 constexpr int kPartW = kRowsW * 128;                               // bytes of a tile of W: 128 rows of 64 weights
 
 struct TilesParams {
@@ -119,7 +122,7 @@ __device__ __noinline__ void tile_end(const TilesParams& p, uint32_t tmem, const
     const bool near = we >= -60 && we <= 60;                       // no product leaves fp32's range on the way
     const float wpow = __uint_as_float((uint32_t)(127 + (near ? we : 0)) << 23);
     float* part = p.partial + (2 * (int64_t)blockIdx.x + (begins ? 0 : 1)) * p.cols * kRowsW + rw;
-    for (int c0 = 16 * (warp >> 2); c0 < p.cols; c0 += 64) {
+    for (int c0 = 16 * (warp >> 2); c0 < p.cols; c0 += kWorkers / 8) {
         uint32_t v[16], v2[16];
         const int m_lane = ct * p.cols + c0 + (lane & 15), mine = m_lane < l.rows ? p.exponent[m_lane] : 0;
         tmem_load16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0, v);
@@ -204,38 +207,41 @@ __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_con
         }
         __syncwarp();
     } else if (warp == kWorkers / 32 + 1) {
-        if (lane == 0) {
+        {
+            const bool leader = lane == 0;
+            const uint32_t sums = uniform(tmem), ring = uniform(base);
             const int n = p.pieces * p.cols;                       // the pieces' columns side by side, sums apart
             const uint32_t desc = half_product_descriptor(n);
             int super = super0, ws = 0, wt = 0, xs = 0, xt = 0, t = 0;
             bool first = true, ok = true;
             for (int i = 0; ok && i < count; ++i) {
-                if (first && t > 1 && !(ok = bar_wait(taken(t), ((t >> 1) - 1) & 1, &failed))) break;
-                const uint32_t to = tmem + (t & 1) * (p.columns >> 1);
+                if (first && t > 1 && !(ok = __all_sync(0xFFFFFFFFu, bar_wait(taken(t), ((t >> 1) - 1) & 1, &failed)))) break;
+                const uint32_t to = sums + (t & 1) * (p.columns >> 1);
                 const int blocks = blocks_of(super);
                 for (int q = 0; q < blocks; q += PER) {
                     ok = bar_wait(x_full(xs), xt & 1, &failed) && bar_wait(w_full(ws), wt & 1, &failed);
+                    ok = __all_sync(0xFFFFFFFFu, ok);
                     if (!ok) break;
                     tmem_fence_after();
-                    uint64_t w = tile_descriptor(base + ws * PER * kPartW, 16), x = tile_descriptor(base + x_base + xs * PER * x_bytes, 16);
+                    uint64_t w = tile_descriptor(ring + ws * PER * kPartW, 16), x = tile_descriptor(ring + x_base + xs * PER * x_bytes, 16);
 #pragma unroll
                     for (int b = 0; b < PER; ++b) {
                         if (q + b < blocks) {
 #pragma unroll
-                            for (int k = 0; k < kBlock / 16; ++k) mma_ss(to, w + 2 * k, x + 2 * k, desc, !first || k > 0);
+                            for (int k = 0; k < kBlock / 16; ++k) mma_ss(to, w + 2 * k, x + 2 * k, desc, !first || k > 0, leader);
                             first = false;
                             w += kPartW >> 4;
                             x += x_bytes >> 4;
                         }
                     }
-                    mma_commit(w_empty(ws));
-                    mma_commit(x_empty(xs));
+                    mma_commit(w_empty(ws), leader);
+                    mma_commit(x_empty(xs), leader);
                     if (++ws == p.w_stages) { ws = 0; ++wt; }
                     if (++xs == p.x_stages) { xs = 0; ++xt; }
                 }
                 if (++super == p.k_supers) super = 0;
                 if (super == 0 || i + 1 == count) {
-                    mma_commit(done(t));
+                    mma_commit(done(t), leader);
                     ++t;
                     first = true;
                 }
@@ -243,56 +249,60 @@ __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_con
         }
         __syncwarp();
     } else {
-        // ---- weights: lane (c, row) takes 32 weights, half of block c / 2 of the piece, of rows r and r + 64
+        // ---- weights: lane (c, row) takes 32 weights, half of block c / 2 of the piece, of row r and those kRowStep apart
         const int c = lane >> 2, r = warp * 4 + (lane & 3), q_mine = c >> 1, half = c & 1;
         const int groups = l.n_in / (NV ? 16 : 32);
         constexpr int kAhead = 2;
-        uint4 ahead[kAhead][2] = {};
-        uint32_t ahead_s[kAhead][2] = {};
-        int next_tile = tile0, next_super = super0, next_i = 0, next_row = -1;
-        const uint8_t *codes0 = l.codes, *codes1 = l.codes, *scales0 = l.scales, *scales1 = l.scales;
+        uint4 ahead[kAhead][kEach] = {};
+        uint32_t ahead_s[kAhead][kEach] = {};
+        const int last = l.n_in / 32 - 1;                          // of a row's pieces of 32 weights
+        int next_ct = tile0 % p.col_tiles, next_rt = tile0 / p.col_tiles, next_super = super0, next_left = count;
+        const uint8_t *codes[kEach], *scales[kEach];
+        auto next_rows = [&]() {
+#pragma unroll
+            for (int v = 0; v < kEach; ++v) {
+                const int64_t n = min(next_rt * kRowsW + r + kRowStep * v, l.n_out - 1);
+                codes[v] = l.codes + n * (l.n_in >> 1);
+                scales[v] = l.scales + n * groups;
+            }
+        };
+        next_rows();
         // What lies outside the matrix is read from a place inside (and scaled by zero when it is used: a choice made here would wait
         // for the load).
-        auto fetch = [&](uint4 (&w)[2], uint32_t (&sc)[2]) {
-            if (next_i < count) {
-                const int rt = next_tile / p.col_tiles;
-                if (rt != next_row) {
-                    next_row = rt;
-                    const int64_t n0 = min(rt * kRowsW + r, l.n_out - 1), n1 = min(rt * kRowsW + r + 64, l.n_out - 1);
-                    codes0 = l.codes + n0 * (l.n_in >> 1);
-                    codes1 = l.codes + n1 * (l.n_in >> 1);
-                    scales0 = l.scales + n0 * groups;
-                    scales1 = l.scales + n1 * groups;
-                }
-                const int at = min(next_super * 8 + c, l.n_in / 32 - 1);
+        auto fetch = [&](uint4 (&w)[kEach], uint32_t (&sc)[kEach]) {
+            if (next_left > 0) {
+                const int at = min(next_super * 8 + c, last);
                 if (at >= 0) {
-                    w[0] = __ldg(reinterpret_cast<const uint4*>(codes0) + at);
-                    w[1] = __ldg(reinterpret_cast<const uint4*>(codes1) + at);
-                    if (NV) {
-                        sc[0] = __ldg(reinterpret_cast<const uint16_t*>(scales0) + at);
-                        sc[1] = __ldg(reinterpret_cast<const uint16_t*>(scales1) + at);
-                    } else {
-                        sc[0] = __ldg(scales0 + at);
-                        sc[1] = __ldg(scales1 + at);
+#pragma unroll
+                    for (int v = 0; v < kEach; ++v) {
+                        w[v] = __ldg(reinterpret_cast<const uint4*>(codes[v]) + at);
+                        if (NV) sc[v] = __ldg(reinterpret_cast<const uint16_t*>(scales[v]) + at);
+                        else sc[v] = __ldg(scales[v] + at);
                     }
                 }
-                ++next_i;
-                if (++next_super == p.k_supers) { next_super = 0; ++next_tile; }
+                --next_left;
+                if (++next_super == p.k_supers) {
+                    next_super = 0;
+                    if (++next_ct == p.col_tiles) { next_ct = 0; ++next_rt; next_rows(); }
+                }
             }
         };
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) fetch(ahead[a], ahead_s[a]);
 
-        int tile = tile0, super = super0, seg_end = min(p.k_supers - super0, count), tiles = 0, i = 0, stage = 0, turn = 0, top[2];
+        int tile = tile0, super = super0, seg_end = min(p.k_supers - super0, count), tiles = 0, i = 0, stage = 0, turn = 0, top[kEach];
         bool whole = seg_end == p.k_supers;                        // the run has all pieces of the tile
         int ended = -1;                                            // a tile whose sums have not been read yet
         bool ended_whole = false;
+        int ct = tile0 % p.col_tiles, rt = tile0 / p.col_tiles;
+        bool live[kEach];
         auto begin_rows = [&](int t) {
-            const int n = tile / p.col_tiles * kRowsW + r;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (t == 0 || tile % p.col_tiles == 0) top[h] = row_top<NV>(p, n + 64 * h, c);     // otherwise the same rows again
-                if (!NV && c == 0) top_e[t & 1][r + 64 * h] = top[h];
+            for (int h = 0; h < kEach; ++h) {
+                const int n = rt * kRowsW + r + kRowStep * h;
+                live[h] = n < l.n_out;
+                if (t == 0 || ct == 0) top[h] = row_top<NV>(p, n, c);          // otherwise the same rows again
+                if (!NV && c == 0) top_e[t & 1][r + kRowStep * h] = top[h];
             }
         };
         auto end_tile = [&]() {                                    // tile `tiles - 1` of the run
@@ -317,13 +327,13 @@ __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_con
                     }
                     if (PER > 1 || q_mine < blocks) {
                         if (t > 0) bar_wait(w_empty(s), (t - 1) & 1, &failed);
-                        const bool inside = super * 8 + c < l.n_in / 32;
-                        const int n = tile / p.col_tiles * kRowsW + r;
+                        __syncwarp(__activemask());            // the lanes wait for different places, and go on together
+                        const bool inside = super * 8 + c <= last;
 #pragma unroll
-                        for (int v = 0; v < 2; ++v) {
+                        for (int v = 0; v < kEach; ++v) {
                             const uint4 w = ahead[a][v];
                             const uint32_t sc = ahead_s[a][v];
-                            const bool on = inside && n + 64 * v < l.n_out;
+                            const bool on = inside && live[v];
                             uint32_t h[16], f[2];
                             e2m1x8_to_half(w.x, *reinterpret_cast<uint32_t(*)[4]>(h));
                             e2m1x8_to_half(w.y, *reinterpret_cast<uint32_t(*)[4]>(h + 4));
@@ -342,7 +352,7 @@ __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_con
                                 const __half2 x = __hmul2(*reinterpret_cast<__half2*>(&h[q]), *reinterpret_cast<__half2*>(&f[q >> 3]));
                                 h[q] = *reinterpret_cast<const uint32_t*>(&x);
                             }
-                            const int row = r + 64 * v;
+                            const int row = r + kRowStep * v;
                             uint8_t* to = smem + (PER == 1 ? s : s * PER + q_mine) * kPartW + row * 128;
 #pragma unroll
                             for (int q = 0; q < 4; ++q)
@@ -367,6 +377,7 @@ __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_con
                         seg_end = min(i + p.k_supers, count);
                         whole = seg_end - i == p.k_supers;
                         ++tile;
+                        if (++ct == p.col_tiles) { ct = 0; ++rt; }
                         begin_rows(tiles);
                     } else {
                         seg_end = -1;
