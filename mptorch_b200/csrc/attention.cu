@@ -15,6 +15,7 @@
 // moved only when a tile exceeds it.
 //
 // Measured figures stand at the launch rule below.
+#define MPT_DEFINE_JOIN
 #include "attention.cuh"
 #include "attention_chunk.cuh"
 
@@ -540,8 +541,9 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_att
         }
     }
     __syncthreads();
-    run.advance(p, take);
+    run.advance(p, take, pieces);
     }
+    run.end(p);
 }
 
 // How a call is cut: columns of a tile, and CTAs.
@@ -567,7 +569,7 @@ Plan make_plan(const CacheView& c, int q_heads, int dtype, int window, int sinks
     pl.row_tiles = tiles * c.heads;
     pl.most_pieces = pieces;
     pl.partial_floats = (size_t)2 * pl.runs * pl.tile_rows * c.dim;
-    pl.stats_floats = (size_t)2 * pl.runs * pl.tile_rows * 2;
+    pl.stats_floats = (size_t)2 * pl.runs * pl.tile_rows * 2 + (size_t)pl.runs * (sizeof(Cut) / 4);      // and the cuts
     return pl;
 }
 
@@ -603,7 +605,7 @@ int launch_rows(AttentionParams p, const Plan& pl, cudaStream_t st) {
     p.runs = pl.runs < most ? pl.runs : most;
     p.whole = pl.row_tiles >= p.runs ? kWhole : 0;
     kern<<<(unsigned)p.runs, 32 * kWarps, bytes, st>>>(p);
-    if (p.runs > 1 && pl.most_pieces > p.whole) launch_after(mx_attention_join_kernel<kTok>, dim3((unsigned)(p.runs - 1), (unsigned)(p.tile_rows + 3) / 4), dim3(128), 0, st, p);
+    if (p.runs > 1 && pl.most_pieces > p.whole) launch_after(mx_attention_join_kernel, dim3((unsigned)(p.runs - 1), (unsigned)(p.tile_rows + 3) / 4), dim3(128), 0, st, p);
     return check_launch("mx_attention");
 }
 
@@ -670,11 +672,13 @@ int mpt_mx_attention(const mpt_mx_cache* cache, const mpt_mx_batch* batch, const
     if (call.chunk) {
         p.partial = reinterpret_cast<float*>(ws + call.chunks.tile_bytes);
         p.stats = p.partial + call.chunks.partial_floats;
+        p.cuts = reinterpret_cast<Cut*>(p.stats + call.chunks.stats_floats - (size_t)call.chunks.runs * (sizeof(Cut) / 4));
         return launch_chunk(p, call.chunks, ws, fp4, st);
     }
     p.tile_rows = call.rows.tile_rows; p.least = kLeast;
     p.partial = reinterpret_cast<float*>(ws);
     p.stats = p.partial + call.rows.partial_floats;
+    p.cuts = reinterpret_cast<Cut*>(p.stats + (size_t)4 * call.rows.runs * call.rows.tile_rows);
     return fp4 ? launch_rows<true>(p, call.rows, st) : launch_rows<false>(p, call.rows, st);
 }
 

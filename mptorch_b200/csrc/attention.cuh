@@ -20,7 +20,11 @@ struct AttentionParams {
     int runs, least;                   // CTAs, and pieces of tokens that one takes at least
     int whole;                         // row tiles of at most so many pieces are not cut
     float *partial, *stats;            // of row tiles that two or more CTAs share: sums [slot, row, dim], and {maximum, sum} of each row
+    struct Cut* cuts;                  // for each run, the row tile that it has the first but not the last pieces of
 };
+
+// A row tile that runs `run` to `last` share: the first one's slot, and two for each of the others, of which they use the first.
+struct Cut { int seq, head, tile, slot, last; };           // seq: -1 for none
 
 // New rows of sequence s, clamped to the rows there are.
 __device__ __forceinline__ int2 rows_of(const CacheView& c, int s) {
@@ -211,14 +215,15 @@ __device__ __forceinline__ float exp2_fast(float x) {       // relative error 2^
 template <int STEP>
 struct RunOf {
     Place at;
-    int64_t left;
-    bool begins = true;                        // the segment stands at the beginning of the run
+    int64_t left, pos, per;                    // pieces left, number of the piece at `at` among all, pieces of a run
+    bool begins = true, told = false;          // the segment stands at the beginning of the run; its cut has been written
     __device__ __forceinline__ RunOf(const AttentionParams& p, int64_t* sm) {
-        int64_t per;
         const int64_t total = find_place<STEP>(p, blockIdx.x, per, at, sm);
-        left = min(per, total - blockIdx.x * per);
+        pos = blockIdx.x * per;
+        left = min(per, total - pos);
         if (left > 0 && at.piece > 0 && at.w.pieces(at.tile) <= p.whole) {
             left += at.piece;
+            pos -= at.piece;
             at.piece = 0;
         }
     }
@@ -227,32 +232,35 @@ struct RunOf {
         const int rest = pieces - at.piece;
         return left >= rest ? rest : left <= 0 || pieces <= p.whole ? 0 : (int)left;
     }
-    __device__ __forceinline__ void advance(const AttentionParams& p, int took) {
+    __device__ __forceinline__ void advance(const AttentionParams& p, int took, int pieces) {
+        if (threadIdx.x == 0 && at.piece == 0 && took < pieces) {
+            p.cuts[blockIdx.x] = Cut{at.seq, at.head, at.tile, 2 * (int)blockIdx.x + (begins ? 0 : 1), (int)((pos + pieces - 1) / per)};
+            told = true;
+        }
         left -= took;
+        pos += took;
         begins = false;
         if (left > 0) at.template next_tile<STEP>(p);
     }
+    __device__ __forceinline__ void end(const AttentionParams& p) {
+        if (threadIdx.x == 0 && !told) p.cuts[blockIdx.x].seq = -1;
+    }
 };
 
-// Joins the row tiles that runs end in: CTAs (x, .) look at the end of run x, where run x + 1 begins.  A warp
-// takes a row.
-template <int STEP>
+// Joins the row tiles that are cut: CTAs (x, .) that of which run x has the first pieces.  A warp takes a row.
+__global__ void __launch_bounds__(512) mx_attention_join_kernel(const AttentionParams p);
+
+#ifdef MPT_DEFINE_JOIN
 __global__ void __launch_bounds__(512) mx_attention_join_kernel(const AttentionParams p) {
     const CacheView& c = p.c;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = c.dim, nb = dim >> 5;
-    __shared__ int64_t place_sm[kPlaceWords];
-    Place at;
-    int64_t per;
-    const int run = blockIdx.x;
-    const int64_t total = find_place<STEP>(p, run + 1, per, at, place_sm), cut = (run + 1) * per;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = c.dim, nb = dim >> 5, run = blockIdx.x;
     wait_for_previous();                                           // whatever follows: this kernel is not done before the one it follows
-    if (cut >= total || at.piece == 0 || at.w.pieces(at.tile) <= p.whole) return;       // nothing is cut here
-    const int64_t p0 = cut - at.piece, p1 = p0 + at.w.pieces(at.tile);
-    if (run * per > p0) return;                                    // an earlier CTA joins this one
-    const int last = (int)((p1 - 1) / per);
+    const Cut at = p.cuts[run];
+    if (at.seq < 0) return;
+    const int last = at.last;
     const int2 own = rows_of(c, at.seq);
     const int first = at.tile * p.tile_rows, count = min(p.tile_rows, own.y * p.group - first);
-    auto slot_of = [&](int k) { return 2 * k + (k == run && run * per < p0 ? 1 : 0); };
+    auto slot_of = [&](int k) { return k == run ? at.slot : 2 * k; };
     const int warps = blockDim.x >> 5;
     for (int r = warp + warps * blockIdx.y; r < count; r += warps * gridDim.y) {
         // 32 parts at a time: a lane has the statistics of one, and the sums follow without waiting for one another
@@ -292,5 +300,6 @@ __global__ void __launch_bounds__(512) mx_attention_join_kernel(const AttentionP
             if (b < nb) store_value(p.out, p.dtype, out_row + b * 32 + lane, v[b] * inv_sum);
     }
 }
+#endif
 
 }  // namespace mpt

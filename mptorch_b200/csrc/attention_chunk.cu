@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
     zero_outside(p);
     RunOf<kTile> run(p, place_sm);
     if (run.left <= 0) {
+        run.end(p);
         wait_for_previous();                                      // no CTA is done before the kernel that this one follows
         return;
     }
@@ -428,8 +429,9 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
         tmem_fence_after();
         if (failed) break;
         it0 += n;
-        run.advance(p, take);
+        run.advance(p, take, pieces);
     }
+    run.end(p);
     if (failed && warp == 8 && lane == 0) {                       // copies on the way write to this CTA's memory
         failed = 0u;
         wait(kKFull, 0); wait(kKFull, 1);
@@ -449,7 +451,7 @@ int launch(AttentionParams p, const ChunkPlan& pl, uint8_t* tiles, cudaStream_t 
     p.runs = pl.runs < fit * sm_count() ? pl.runs : fit * sm_count();
     p.whole = 0;
     launch_after(kern, dim3((unsigned)p.runs), dim3(kThreads), Shape::smem, st, p, tiles, pl.tiles_per_seq);
-    if (p.runs > 1) launch_after(mx_attention_join_kernel<kTile>, dim3((unsigned)(p.runs - 1), 2), dim3(512), 0, st, p);
+    if (p.runs > 1) launch_after(mx_attention_join_kernel, dim3((unsigned)(p.runs - 1), 2), dim3(512), 0, st, p);
     return check_launch("mx_attention");
 }
 
@@ -485,7 +487,7 @@ ChunkPlan chunk_plan(const CacheView& c, int q_heads) {
     const int64_t row_tiles = c.rows * group / kTile + c.seqs, want = row_tiles * c.heads * (pl.tiles_per_seq + 1), most = 2 * (int64_t)sm_count();
     pl.runs = (int)(want < 1 ? 1 : want > most ? most : want);
     pl.partial_floats = (size_t)2 * pl.runs * kTile * c.dim;
-    pl.stats_floats = (size_t)2 * pl.runs * kTile * 2;
+    pl.stats_floats = (size_t)2 * pl.runs * kTile * 2 + (size_t)pl.runs * (sizeof(Cut) / 4);      // and the cuts
     return pl;
 }
 
