@@ -363,7 +363,8 @@ enum { MPT_BLOCK_MXFP4 = 0, MPT_BLOCK_NVFP4 = 1 };
 /* y[rows, n_out] = x[rows, n_in] W^T + bias, W [n_out, n_in] as packed E2M1 codes ([n_out, n_in / 2] bytes,
  * element 2i in the low nibble) with MXFP4 scales (E8M0, [n_out, n_in / 32]) or NVFP4 scales (E4M3,
  * [n_out, n_in / 16], times the fp32 scale at the device address `global_scale`, 1 where it is NULL).  n_in is a
- * multiple of 32; `codes` begins at a multiple of 16 bytes; x and y are contiguous; `bias` may be NULL.
+ * multiple of 32; `codes` begins at a multiple of 16 bytes, NVFP4 `scales` at an even address; x and y are contiguous;
+ * `bias` may be NULL.
  * `workspace`: mpt_block_linear_workspace_bytes() bytes at a multiple of 256, of this call alone until it is done. */
 MPT_API size_t mpt_block_linear_workspace_bytes(int64_t rows, int64_t n_out, int64_t n_in, int format, int dtype);
 MPT_API int mpt_block_linear(const void *x, const uint8_t *codes, const uint8_t *scales, const float *global_scale,
@@ -372,7 +373,8 @@ MPT_API int mpt_block_linear(const void *x, const uint8_t *codes, const uint8_t 
 
 /* A cache of K and V in MX format, in pages: codes [num_pages, heads, page, dim] bytes (E4M3) or
  * [num_pages, heads, page, dim / 2] (E2M1), scales [num_pages, heads, page, dim / 32] E8M0 bytes.  dim is a multiple
- * of 32 up to 256, page a power of two from 8 to 256; codes begin at a multiple of 16 bytes. */
+ * of 32 up to 256, page a power of two from 8 to 256; codes begin at a multiple of 16 bytes, scales at one of 8.  A code
+ * that is a NaN (0x7F, 0xFF) stands only in blocks whose scale is 0xFF, as mpt_mx_cache_write leaves them. */
 typedef struct {
     uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
     int64_t num_pages;

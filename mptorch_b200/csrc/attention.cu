@@ -664,7 +664,8 @@ int mpt_mx_attention(const mpt_mx_cache* cache, const mpt_mx_batch* batch, const
     p.out_vec = ((uintptr_t)out & 15u) == 0;
     p.q_heads = q_heads; p.group = q_heads / c.heads;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634);
-    p.window = window; p.sinks = sinks;
+    p.window = window < (1 << 30) ? window : 1 << 30;          // so that no position leaves 32 bits
+    p.sinks = sinks < (1 << 30) ? sinks : 1 << 30;
     p.out = out; p.zero_tail = zero_tail;
     cudaStream_t st = as_stream(stream);
     const bool fp4 = cache->elem_format == MPT_ELEM_E2M1;

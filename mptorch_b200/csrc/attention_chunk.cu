@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(256) mx_expand_kernel(const AttentionParams p,
 
 // ---- attention
 constexpr int kRowThreads = 256, kThreads = kRowThreads + 64;     // two threads a row, each with half of the tokens; a warp that copies, one that issues products
-enum { kKFull, kKEmpty, kVFull, kVEmpty, kScores, kScores2, kWeights, kWeights2, kValues, kBars };
+enum { kKFull, kKEmpty, kVFull, kVEmpty, kScores, kScores2, kWeights, kWeights2, kValues, kValues2, kBars };
 
 template <int DIM, int PIECES, int NS>
 struct ChunkShape {
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
     __shared__ int64_t place_sm[kPlaceWords];
     __shared__ __align__(8) uint64_t bars[kBars];
     __shared__ uint32_t tmem_slot, failed;
-    __shared__ float tops[2][kTile], sums_sm[kTile];
+    __shared__ float tops[2][2][kTile], sums_sm[kTile];           // of alternate pieces: with two sets of scores one warp may be a piece ahead
 
     next_may_start();
     zero_outside(p);
@@ -150,6 +150,10 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
 
     auto bar = [&](int i) { return smem_at(&bars[i]); };
     auto wait = [&](int i, uint32_t parity) { return bar_wait(bar(i), parity & 1u, &failed); };
+    // A wait for a phase is only sound where the phase before it is known to be over.  With two sets of scores a row's weights may be
+    // ready while the product with the piece before is under way, so each set has barriers of its own.
+    auto values_bar = [&](uint32_t it) { return NS == 2 && (it & 1) ? kValues2 : kValues; };
+    auto wait_values = [&](uint32_t it) { return wait(values_bar(it), NS == 2 ? it >> 1 : it); };
     if (threadIdx.x == 0) {
         for (int i = 0; i < kBars; ++i) bar_init(bar(i), i == kWeights || i == kWeights2 ? kRowThreads : 1);
         failed = 0u;
@@ -234,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
                     const uint32_t it = it0 + i;
                     if (!__all_sync(0xFFFFFFFFu, wait(kKFull, it))) return false;
                     // the columns are free when the product that read the weights in them is done (the segment before is done)
-                    if (i >= NS && !__all_sync(0xFFFFFFFFu, wait(kValues, it - NS))) return false;
+                    if (i >= NS && !__all_sync(0xFFFFFFFFu, wait_values(it - NS))) return false;
                     tmem_fence_after();
                     const uint64_t q_desc = tile_descriptor(q_u, 16), k_desc = tile_descriptor(k_u, 16);
                     const uint32_t to = tm + (NS == 2 ? (it & 1) * 128 : 0);
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
                             mma_ts(tm + (PIECES == 3 && k > 0 ? Shape::small : Shape::sums), w + s * 8, v_desc + (s * 2048 >> 4), value_desc,
                                    i > 0 || s > 0 || k > (PIECES == 3 ? 1 : 0), leader);
                     }
-                    mma_commit(bar(kValues), leader);
+                    mma_commit(bar(values_bar(it)), leader);
                     mma_commit(bar(kVEmpty), leader);
                     if (NS == 1 && i + 1 < n) ok = scores(i + 1);
                 }
@@ -316,17 +320,17 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
                 }
                 top = fmaxf(top, top2);
                 // the other half's; from here on the scores' columns are free
-                tops[half][r] = top;
+                tops[it & 1][half][r] = top;
                 tmem_fence_before();
                 pair_sync();
                 tmem_fence_after();
-                top = fmaxf(top, tops[half ^ 1][r]) * mul;
+                top = fmaxf(top, tops[it & 1][half ^ 1][r]) * mul;
                 if (__any_sync(0xFFFFFFFFu, top > m + 8.f)) {
                     const float next = fmaxf(m, top), fade = next == -INFINITY ? 1.f : exp2_fast(m - next);
                     m = next;
                     l *= fade;
                     if (i > 0) {
-                        wait(kValues, it - 1);
+                        wait_values(it - 1);
                         __syncwarp();
                         tmem_fence_after();
                         // the halves take blocks of 16 columns in turn; few registers are free here
@@ -372,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
                 tmem_fence_before();
                 bar_arrive(bar(turn ? kWeights2 : kWeights));
             }
-            if (n > 0) wait(kValues, it0 + n - 1);
+            if (n > 0) wait_values(it0 + n - 1);
             if (half) sums_sm[r] = l;
             __syncwarp();
             pair_sync();
@@ -450,7 +454,9 @@ int launch(AttentionParams p, const ChunkPlan& pl, uint8_t* tiles, cudaStream_t 
     if (!allow_shared<kern>(Shape::smem)) return check_launch("mx_attention");
     p.runs = pl.runs < fit * sm_count() ? pl.runs : fit * sm_count();
     p.whole = 0;
-    launch_after(kern, dim3((unsigned)p.runs), dim3(kThreads), Shape::smem, st, p, tiles, pl.tiles_per_seq);
+    // (without tokens nothing was expanded, and the kernel before this one is none of this call's)
+    if (pl.tiles_per_seq > 0) launch_after(kern, dim3((unsigned)p.runs), dim3(kThreads), Shape::smem, st, p, tiles, pl.tiles_per_seq);
+    else kern<<<(unsigned)p.runs, kThreads, Shape::smem, st>>>(p, tiles, pl.tiles_per_seq);
     if (p.runs > 1) launch_after(mx_attention_join_kernel, dim3((unsigned)(p.runs - 1), 2), dim3(512), 0, st, p);
     return check_launch("mx_attention");
 }

@@ -326,6 +326,8 @@ __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_con
                         if (s >= p.w_stages) { s -= p.w_stages; ++t; }
                     }
                     if (PER > 1 || q_mine < blocks) {
+                        // (a lane does not use a place each turn, but its blocks are at most seven apart and the ring has seven places
+                        // at least: the phase before the one that it waits for is over)
                         if (t > 0) bar_wait(w_empty(s), (t - 1) & 1, &failed);
                         __syncwarp(__activemask());            // the lanes wait for different places, and go on together
                         const bool inside = super * 8 + c <= last;
@@ -436,6 +438,7 @@ TilesPlan tiles_plan(int64_t rows, int64_t n_out, int64_t n_in, int dtype) {
     pl.x_stages = pl.ring_blocks > 1 ? 2 : x_bytes <= 16 * 1024 ? 4 : 3;
     pl.w_stages = (room - pl.x_stages * pl.ring_blocks * x_bytes) / (pl.ring_blocks * kPartW);
     if (pl.w_stages > kMaxStages) pl.w_stages = kMaxStages;
+    // (single blocks: 7 places with 32 kB of x, more with less)
     // equal runs, one for each SM; or whole tiles, where their number leaves hardly an SM idle
     const int64_t tiles = (int64_t)pl.row_tiles * pl.col_tiles, sms = sm_count(), rounds = (tiles + sms - 1) / sms;
     pl.k_supers = (pl.k_blocks + kSuper - 1) / kSuper;

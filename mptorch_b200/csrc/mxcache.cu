@@ -30,12 +30,14 @@ bool convert_cache(const char* who, const mpt_mx_cache* c, const mpt_mx_batch* b
     if (b->rows != 0 && (!c->k_codes || !c->k_scales || !c->v_codes || !c->v_scales) && c->num_pages != 0) { set_error("%s: null pointer", who); return false; }
     if (b->rows != 0 && b->seqs != 0 && (!b->lens || (!b->pages && b->width != 0))) { set_error("%s: null pointer", who); return false; }
     if (((uintptr_t)c->k_codes | (uintptr_t)c->v_codes) & 15u) { set_error("%s: the codes must begin at a multiple of 16 bytes", who); return false; }
+    if (((uintptr_t)c->k_scales | (uintptr_t)c->v_scales) & 7u) { set_error("%s: the scales must begin at a multiple of 8 bytes", who); return false; }
     out->k_codes = c->k_codes; out->k_scales = c->k_scales; out->v_codes = c->v_codes; out->v_scales = c->v_scales;
     out->heads = c->heads; out->dim = c->dim;
     out->page_shift = 31 - __builtin_clz((unsigned)c->page);
     out->num_pages = (int)c->num_pages;
     out->pages = b->pages; out->lens = b->lens; out->starts = b->starts;
-    out->seqs = b->seqs; out->width = b->width;
+    out->seqs = b->seqs;
+    out->width = c->num_pages ? b->width : 0;      // without pages there are no tokens
     out->new_rows = b->starts == nullptr && b->seqs > 0 ? (int)(b->rows / b->seqs) : 1;
     out->rows = b->rows;
     return true;

@@ -196,6 +196,20 @@ def test_linear_shapes_strides_and_quantizers(q):
     assert torch.equal(q.mx_linear(x, codes, scales), q.mx_linear(x, codes, scales))
 
 
+@pytest.mark.parametrize("rows", [1, 5, 12, 40, 200])
+def test_linear_slices_of_a_weight_and_no_inputs(q, rows):
+    """Rows of a packed weight (scales that begin anywhere), one output, and no inputs at all."""
+    g = gen(rows)
+    for fmt, k in (("mxfp4", 96), ("mxfp4", 1120), ("nvfp4", 96), ("nvfp4", 544)):
+        codes, scales, glob, w = pack(300, k, fmt, g)
+        x = torch.randn(rows, k, device="cuda", generator=g)
+        for lo, hi in ((1, 2), (7, 140), (131, 300)):
+            check_linear(linear(q, x, codes[lo:hi], scales[lo:hi], glob), x, w[lo:hi])
+    bias = torch.randn(9, device="cuda", generator=g)
+    none = torch.zeros(9, 0, device="cuda", dtype=torch.uint8)
+    assert torch.equal(q.mx_linear(torch.zeros(rows, 0, device="cuda"), none, none, bias), bias.expand(rows, 9))
+
+
 # ---------------------------------------------------------------------------------- the cache
 def place(lens, page, g, extra=2):
     """A page table over pages in random order (-1 behind the last one) and the number of pages."""
@@ -370,6 +384,22 @@ def test_attention_chunks(q, elem, dtype, case, window, sinks):
     check_attention(got, want, tol)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,group", [(64, 1), (96, 2), (128, 1), (192, 1), (256, 1)])
+def test_attention_chunks_over_long_contexts(q, dtype, dim, group):
+    """Many pieces of tokens for each row tile, in row tiles that are cut and in whole ones, twice the same bits."""
+    lens, new = [2000, 1000, 333, 2600], [250, 300, 100, 129]
+    qry, cache, pages, ln, starts = setup(q, lens, new, 4, group, dim, 16, "e4m3", dtype, dim)
+    got = q.mx_attention(qry, cache, pages, ln, starts, scale=0.05)
+    want, tol = reference(qry, cache, pages, lens, new, dim, 0.05)
+    check_attention(got, want, tol)
+    # errors of random sign: their norm stays well below the bound on each
+    norm = ((got.double() - want).norm() / want.norm()).item()
+    assert norm < (4e-6 if dtype == torch.float32 else 2 * half_ulp(dtype))
+    for _ in range(3):
+        assert torch.equal(q.mx_attention(qry, cache, pages, ln, starts, scale=0.05), got)
+
+
 FORMS = [([70, 33], [1, 1], 1, 4), ([70, 33, 260], [9, 20, 130], 1, 2), ([190], [180], 2, 2)]
 
 
@@ -441,6 +471,46 @@ def test_attention_rows_that_see_nothing(q, dtype, new):
     assert q.mx_attention(flat, cache, pages, ln, starts, out=mine) is mine or True
     assert torch.equal(mine[:new + 1], got[:new + 1]) and (mine[new + 1:] == 7).all()
     assert q.mx_attention(flat[:0], cache, pages, ln, cumulative([0] * 4)).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("new", [1, 40, 150])
+def test_attention_extreme_arguments(q, new):
+    """A window and sinks of any size beside rows that stand nowhere, an empty cache, a table without places."""
+    lens = [new + 200, max(new - 20, 0), new]
+    qry, cache, pages, ln, _ = setup(q, [max(n, 1) for n in lens], [new] * 3, 2, 2, 64, 16, "e4m3", torch.float32, new, uniform=True)
+    ln = i32(lens)
+    plain = q.mx_attention(qry, cache, pages, ln)
+    most = 2 ** 31 - 1
+    assert torch.equal(q.mx_attention(qry, cache, pages, ln, window=most), plain)
+    assert torch.equal(q.mx_attention(qry, cache, pages, ln, window=most, sinks=most), plain)
+    got = q.mx_attention(qry, cache, pages, ln, window=7, sinks=most)
+    want, tol = reference(qry.flatten(0, 1), cache, pages, lens, [new] * 3, 64, 1 / 8)
+    check_attention(got.flatten(0, 1), want, tol)
+    none = q.MXCache(*(t[:0] for t in cache))
+    assert not q.mx_attention(qry, none, pages, ln).any() and not q.mx_cache_read(none, pages, ln, new)[0].any()
+    q.mx_cache_write(qry[:, :, :2], qry[:, :, 2:], none, pages, ln)
+    assert not q.mx_attention(qry, cache, pages[:, :0].contiguous(), ln).any()
+    ragged = q.mx_attention(qry.flatten(0, 1), cache, pages[:0], ln[:0], i32([0]))   # no sequences: every row is behind the last
+    assert not ragged.any()
+
+
+def test_two_streams_at_once(q):
+    """Calls that run at the same time share nothing: each stream gets the bits that it gets alone."""
+    g = gen(4)
+    codes, scales, glob, _ = pack(700, 512, "nvfp4", g)
+    sets = [setup(q, [n + 900, n], [n] * 2, 2, 4, 128, 32, "e4m3", torch.bfloat16, n, uniform=True) + (torch.randn(n, 512, device="cuda", generator=g),) for n in (1, 7, 90, 300)]
+    call = lambda s: (q.mx_attention(*s[:4]), q.nvfp4_linear(s[5], codes, scales, glob))  # noqa: E731
+    alone = [call(s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[] for _ in sets]
+    for _ in range(6):
+        for i, (s, st) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(call(s))
+    torch.cuda.synchronize()
+    for want, results in zip(alone, got):
+        assert all(torch.equal(x, y) for r in results for x, y in zip(r, want))
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -107,6 +107,8 @@ def test_c_abi_refuses_before_any_launch():
     assert "bad extents" in err("mpt_block_linear", one, one, one, None, None, one, -1, 8, 64, 0, 0, None, 0, None)
     assert "null pointer" in err("mpt_block_linear", None, one, one, None, None, one, 1, 8, 64, 0, 0, None, 0, None)
     assert "16 bytes" in err("mpt_block_linear", one, ctypes.c_void_p(264), one, None, None, one, 1, 8, 64, 0, 0, None, 0, None)
+    assert "even address" in err("mpt_block_linear", one, one, ctypes.c_void_p(257), None, None, one, 1, 8, 64, 1, 0, None, 0, None)
+    assert L.mpt_block_linear(one, one, one, None, None, one, 40, 8, 64, 0, 0, None, 0, None) == 3 and b"workspace" in L.mpt_last_error()
     assert L.mpt_block_linear(None, None, None, None, None, None, 0, 8, 64, 0, 0, None, 0, None) == 0
 
     def cache(**kw):
@@ -121,7 +123,8 @@ def test_c_abi_refuses_before_any_launch():
     att = lambda c, b, heads=2, win=0, sinks=0, q=one, out=one: err("mpt_mx_attention", c, b, q, 0, strides, heads, 1.0, win, sinks, out, 1, None, 0, None)  # noqa: E731
     for bad, text in ((dict(dim=48), "head_dim"), (dict(dim=512), "head_dim"), (dict(page=24), "page size"), (dict(page=512), "page size"),
                       (dict(elem_format=3), "element format"), (dict(heads=0), "kv heads"), (dict(num_pages=-1), "number of pages"),
-                      (dict(k_codes=None), "null pointer"), (dict(v_codes=264), "16 bytes")):
+                      (dict(k_codes=None), "null pointer"), (dict(v_codes=264), "16 bytes"), (dict(k_scales=260), "8 bytes"),
+                      (dict(v_scales=258), "8 bytes")):
         assert text in att(cache(**bad), rows())
         assert text in err("mpt_mx_cache_write", cache(**bad), rows(), one, one, 0, strides, strides, None)
         assert text in err("mpt_mx_cache_read", cache(**bad), rows(), one, one, 0, None)
@@ -129,6 +132,7 @@ def test_c_abi_refuses_before_any_launch():
                       (dict(pages=None), "null pointer")):
         assert text in att(cache(), rows(**bad))
     assert "null descriptor" in att(None, rows())
+    assert L.mpt_mx_attention(cache(), rows(), one, 0, strides, 2, 1.0, 0, 0, one, 1, None, 0, None) == 3 and b"workspace" in L.mpt_last_error()
     assert "do not divide" in att(cache(), rows(), heads=3)
     assert "negative" in att(cache(), rows(), win=-1)
     assert "null pointer" in att(cache(), rows(), q=None)
