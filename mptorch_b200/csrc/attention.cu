@@ -14,7 +14,10 @@
 // first leaves (22 bits).  p 2^15 is rounded to binary16 (11 bits) in one piece, for float32 in two.  The running maximum is
 // moved only when a tile exceeds it.
 //
-// Measured figures stand at the launch rule below.
+// Measured on a B200 (the bytes at the measured bandwidth in brackets): one token each over 16 contexts up to 32768, 32 heads on 8 of
+// 128, E4M3, bfloat16 140 us (97.9: the issue of conversions and the latency of products hold it to seven tenths of the bandwidth);
+// over a window of 1024 with 4 sinks, 96 sequences, 24 heads on 8 of 96, E2M1, float16 60 us (11.8: an element is half a byte, and
+// the conversions are twice as many a byte); four sequences up to 1024, 12 heads of 64, float32 18.4 us (0.6: host time, two launches).
 #define MPT_DEFINE_JOIN
 #include "attention.cuh"
 #include "attention_chunk.cuh"
@@ -22,13 +25,9 @@
 namespace mpt {
 namespace {
 
-#ifndef MPT_ATT_WARPS
-#define MPT_ATT_WARPS 4
-#define MPT_ATT_LEAST 8
-#define MPT_ATT_WHOLE 64
-#define MPT_ATT_CHUNK 32
-#endif
-constexpr int kWarps = MPT_ATT_WARPS, kTok = 32, kLeast = MPT_ATT_LEAST, kWhole = MPT_ATT_WHOLE;
+// kLeast, pieces of 32 tokens that a run has at least: with 8 four sequences of 1024 tokens take 18.4 us, with 16 22.5.
+// kWhole, pieces up to which a row tile is not cut where there are as many tiles as CTAs: windows of 1024 take 59.4 us whole and 69.4 cut.
+constexpr int kWarps = 4, kTok = 32, kLeast = 8, kWhole = 64;
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(live ? 16 : 0));
@@ -558,6 +557,8 @@ Plan make_plan(const CacheView& c, int q_heads, int dtype, int window, int sinks
     const int group = q_heads / c.heads;
     pl.pieces = dtype == MPT_DTYPE_F32 ? 2 : 1;
     const int64_t per_seq = c.starts == nullptr ? (int64_t)c.new_rows * group : (c.seqs ? (c.rows * group + c.seqs - 1) / c.seqs : 0);
+    // more than eight columns: a tile of 16 reads the cache once (16 sequences, four rows of 32 heads on 8 of 128 over 8192: 95 us, 109 in
+    // two tiles of eight; over 1024 tokens of four sequences, where latency counts, 24 and 20)
     pl.nt = per_seq * pl.pieces > 8 ? 2 : 1;
     pl.tile_rows = 8 * pl.nt / pl.pieces;
     // at most four CTAs on each SM, and no more than there is work for if every sequence is as long as its row of the page table
@@ -573,7 +574,12 @@ Plan make_plan(const CacheView& c, int q_heads, int dtype, int window, int sinks
     return pl;
 }
 
-// Which kernel a call takes, and the workspace it needs.
+// Which kernel a call takes, and the workspace it needs.  The chunk kernel from kChunkRows rows of q for a sequence and kv head on, on
+// average.  It against this file's, by rows: head_dim 128, bfloat16, 16 sequences of 2048: 16 rows 62 and 66 us, 32 rows 68 and 89,
+// 64 rows 79 and 164; four of 4096: 32 rows 52 and 55, 64 rows 63 and 60, 256 rows 92 and 128.  head_dim 64, float32, 16 sequences:
+// 16 rows 78 and 51, 32 rows 80 and 93; four: 32 rows 47 and 43, 64 rows 52 and 62.  Where the expanded cache would pass 4 GB this
+// file's kernel takes the call, which needs no such workspace.
+constexpr int kChunkRows = 32;
 struct CallShape {
     bool chunk;
     Plan rows;
@@ -586,7 +592,7 @@ struct CallShape {
 CallShape shape_of(const CacheView& c, int q_heads, int dtype, int window, int sinks) {
     CallShape s{};
     const int64_t per_seq = c.seqs ? c.rows * (q_heads / c.heads) / c.seqs : 0;
-    if (per_seq >= MPT_ATT_CHUNK && chunk_kernel_exists(c.dim, dtype)) {
+    if (per_seq >= kChunkRows && chunk_kernel_exists(c.dim, dtype)) {
         s.chunks = chunk_plan(c, q_heads);
         s.chunk = s.chunks.tile_bytes <= ((size_t)4 << 30);
     }

@@ -11,7 +11,10 @@
 // Accuracy.  bfloat16 queries are one operand; float16 and float32 ones are the sum of two and three bfloat16 pieces (16 and 24
 // bits), and so are their weights p; sums are fp32 throughout.
 //
-// Measured figures stand at the launch rule below.
+// Measured on a B200: 1024-token chunks of two sequences over 8192, 32 heads on 8 of 128, E4M3, bfloat16 310 us (115.5 for the
+// products at the measured rate of bfloat16; 610 TFLOP/s).  The expansion takes 20 us of it and the join of cut tiles some 10; what bounds
+// the rest is the chain of a tile, product, softmax, product, two CTAs on an SM hiding each other's.  Six ragged chunks up to 300 over
+// 2000, 12 heads of 64, float32: 81 us (2.9), three pieces of q and of p each, and runs of a few tiles.
 #include "attention.cuh"
 #include "attention_chunk.cuh"
 #include "tcgen05.cuh"
@@ -461,6 +464,9 @@ int launch(AttentionParams p, const ChunkPlan& pl, uint8_t* tiles, cudaStream_t 
     return check_launch("mx_attention");
 }
 
+// One set of scores where two CTAs fit an SM (bfloat16 up to 128), two sets where one CTA has the tensor memory for itself.  This choice
+// and the other, 1024-token chunks of two sequences over 8192, 16 heads on 8: bfloat16 of 128 198 and 233 us, of 64 151 and 177; float32
+// of 64 287 and 308, of 32 253 and 283.
 template <int DIM>
 int launch(const AttentionParams& p, const ChunkPlan& pl, uint8_t* tiles, cudaStream_t st) {
     if (p.dtype == MPT_DTYPE_BF16) {

@@ -12,16 +12,15 @@
 // fp32 as they are.  MXFP4: the scale of a block multiplies the fp32 sum of its 32 products, relative to an exponent that is kept
 // for each row of W and raised when a block exceeds it by 2^60, so that no range of scales overflows.
 //
-// Measured figures stand at the launch rule below.
+// Measured on a B200 (weights' bytes at the measured bandwidth in brackets): one bfloat16 row of 8192 by 28672 NVFP4 weights 39 us
+// (20.2); three float32 rows of 768 by 50257 MXFP4 weights 14.4 us (3.2); one of 768 by 2304 9.7 us (0.1: host time and a launch).
+// Some 39 instructions for 512 weights bound the largest, not the memory: copies of twice the depth changed nothing.
 #include "blocklinear.cuh"
 #include "launch.cuh"
 
 namespace mpt {
 namespace {
 
-#ifndef MPT_FEW_COLUMNS
-#define MPT_FEW_COLUMNS 16
-#endif
 constexpr int kWarps = 16, kChunk = 128, kPitch = 80, kStages = 3;          // pitch: eight rows of four words meet no bank twice
 
 __device__ __forceinline__ void cp_bytes(uint32_t dst, const void* src, int bytes) {   // 16
@@ -56,14 +55,16 @@ inline int few_smem(int n_in, int columns, bool nv, int nt) {
     return columns * x_pitch(n_in) + ring + sums;
 }
 
-// GROUPS: one or two columns only.  The other columns of the products are used to keep the scale groups apart: column c has x where its
-// group is c and zeros elsewhere, so that a column's sum over a piece of 128 is that of one group, and the scales multiply eight sums
-// a row and piece instead of 128 weights.  NVFP4: eight groups of 16, a second column of x takes products of its own.  MXFP4: four
-// blocks of 32 in columns 0 to 3, and in 4 to 7 those of the second column.
+// GROUPS: one column (NVFP4), one or two (MXFP4).  The other columns of the products are used to keep the scale groups apart: column c
+// has x where its group is c and zeros elsewhere, so that a column's sum over a piece of 128 is that of one group, and the scales
+// multiply eight sums a row and piece instead of 128 weights.  NVFP4: eight groups of 16.  MXFP4: four blocks of 32 in columns 0 to 3,
+// and in 4 to 7 those of the second column.  With and without, 8192 by 28672: NVFP4 40 and 44 us for one column (48 and 46 for two,
+// which would need products of their own), MXFP4 50 and 61 for one, 51 and 63 for two.
 template <bool NV, int PIECES, int NT, bool GROUPS>
 __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const LinearParams p, int tiles, int share) {
-    constexpr int kColumns = GROUPS ? NT : 8 * NT;                        // (GROUPS: NT counts columns)
+    constexpr int kColumns = GROUPS ? NT : 8 * NT;                        // (GROUPS: NT counts columns; NVFP4 has one)
     constexpr int kScaleRow = NV ? 8 : 4;                                 // bytes of scales of a row in a piece of 128
+    static_assert(!GROUPS || !NV || NT == 1);
     extern __shared__ __align__(16) uint8_t smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, tig = lane & 3;
     const int pitch = x_pitch(p.n_in), columns = p.rows * PIECES, row_bytes = p.n_in >> 1, scale_row = p.n_in / (NV ? 16 : 32);
@@ -180,27 +181,16 @@ __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const 
             const uint8_t* w = ring + stage * stage_bytes(NV);
             const uint8_t* sc = w + 16 * kPitch;
             if constexpr (GROUPS) {
-                constexpr int kSets = NV ? NT : 1;
-                float c[kSets][4];
-#pragma unroll
-                for (int n = 0; n < kSets; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) c[n][i] = 0.f;
-                uint4 xv[kSets];
-#pragma unroll
-                for (int n = 0; n < kSets; ++n)
-                    xv[n] = *reinterpret_cast<const uint4*>(smem + (NV ? min(n, columns - 1) : my_column) * pitch + (chunk * kChunk + my_block * 32 + tig * 8) * 2);
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint4 xv = *reinterpret_cast<const uint4*>(smem + my_column * pitch + (chunk * kChunk + my_block * 32 + tig * 8) * 2);
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     uint32_t a[4], d[4];
                     e2m1x8_to_half(*reinterpret_cast<const uint32_t*>(w + g * kPitch + b * 16 + tig * 4), a);
                     e2m1x8_to_half(*reinterpret_cast<const uint32_t*>(w + (g + 8) * kPitch + b * 16 + tig * 4), d);
                     const bool here = mine && b == my_block;
-#pragma unroll
-                    for (int n = 0; n < kSets; ++n) {
-                        mma(c[n], a[0], d[0], a[1], d[1], here ? xv[n].x : 0u, here ? xv[n].y : 0u);
-                        mma(c[n], a[2], d[2], a[3], d[3], here ? xv[n].z : 0u, here ? xv[n].w : 0u);
-                    }
+                    mma(c, a[0], d[0], a[1], d[1], here ? xv.x : 0u, here ? xv.y : 0u);
+                    mma(c, a[2], d[2], a[3], d[3], here ? xv.z : 0u, here ? xv.w : 0u);
                 }
                 // sums of row g (and g + 8) in this lane: groups 2 tig and 2 tig + 1 (MXFP4: modulo four)
                 const int at = NV ? 2 * tig : 2 * (tig & 1);
@@ -228,11 +218,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const 
                     f0 = make_float2(x0 == 255 ? nan : relative_power(x0, ref0), y0 == 255 ? nan : relative_power(y0, ref0));
                     f1 = make_float2(x1 == 255 ? nan : relative_power(x1, ref1), y1 == 255 ? nan : relative_power(y1, ref1));
                 }
-#pragma unroll
-                for (int n = 0; n < kSets; ++n) {
-                    acc[n][0] = fmaf(c[n][0], f0.x, fmaf(c[n][1], f0.y, acc[n][0]));
-                    acc[n][1] = fmaf(c[n][2], f1.x, fmaf(c[n][3], f1.y, acc[n][1]));
-                }
+                acc[0][0] = fmaf(c[0], f0.x, fmaf(c[1], f0.y, acc[0][0]));
+                acc[0][1] = fmaf(c[2], f1.x, fmaf(c[3], f1.y, acc[0][1]));
             } else {
                 uint2 s0, s1;
                 if (NV) {
@@ -316,7 +303,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const 
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float v = acc[NV ? n : 0][i];
+                    float v = acc[0][i];
                     v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
                     if (NV) v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
                     if (NV ? tig == 0 : tig == 2 * n) sums[(warp * NT + n) * 16 + g + 8 * i] = v;
@@ -357,7 +344,9 @@ int launch_few(const LinearParams& p, cudaStream_t st) {
     const int bytes = few_smem(p.n_in, p.rows * PIECES, NV, NT), tiles = (p.n_out + 15) / 16;
     constexpr auto kern = block_linear_few_kernel<NV, PIECES, NT, GROUPS>;
     if (!allow_shared<kern>(220 * 1024)) return check_launch("block_linear");
-    // One CTA on each SM.  As many warps share a tile as take the least time: rounds of tiles times pieces of a warp, with two for the end.
+    // One CTA on each SM.  As many warps share a tile as take the least time: rounds of tiles times pieces of a warp, with two for the
+    // end.  One row, MXFP4: 4096 by 4096 takes 10 us with eight that share, 19 where none do and 11 where all sixteen do; 768 by 50257
+    // 14, 14 and 46; 8192 by 28672 50, 50 and 64.
     const int chunks = (p.n_in + kChunk - 1) / kChunk;
     int share = 1;
     int64_t least = -1;
@@ -369,10 +358,12 @@ int launch_few(const LinearParams& p, cudaStream_t st) {
     return check_launch("block_linear");
 }
 
-// Few rows: at most 16 columns (a float32 row takes two), x within the shared memory beside the rings.
+// Few rows: at most 16 columns (a float32 row takes two), x within the shared memory beside the rings.  This kernel against the tiles',
+// 4096 by 11008, NVFP4, bfloat16: one row 13 and 28 us, eight 19 and 30, sixteen 28 and 32; MXFP4, float32, eight rows 28 and 35.
+// More columns would need another set of sums for each eight, and 24 rows take the tiles 33.
 bool few_rows(int64_t rows, int64_t n_in, int dtype) {
     const int64_t columns = rows * (dtype == MPT_DTYPE_F32 ? 2 : 1);
-    return columns <= MPT_FEW_COLUMNS && n_in <= 65536 && columns * x_pitch((int)n_in) <= 140 * 1024;
+    return columns <= 16 && n_in <= 65536 && columns * x_pitch((int)n_in) <= 140 * 1024;
 }
 
 }  // namespace
@@ -404,12 +395,12 @@ int mpt_block_linear(const void* x, const uint8_t* codes, const uint8_t* scales,
         const bool nv = format == MPT_BLOCK_NVFP4;
         const int columns = (int)rows * (dtype == MPT_DTYPE_F32 ? 2 : 1);
         if (dtype == MPT_DTYPE_F32) {
-            if (columns == 2) return nv ? launch_few<true, 2, 2, true>(p, st) : launch_few<false, 2, 2, true>(p, st);
+            if (columns == 2 && !nv) return launch_few<false, 2, 2, true>(p, st);
             if (columns <= 8) return nv ? launch_few<true, 2, 1, false>(p, st) : launch_few<false, 2, 1, false>(p, st);
             return nv ? launch_few<true, 2, 2, false>(p, st) : launch_few<false, 2, 2, false>(p, st);
         }
         if (columns == 1) return nv ? launch_few<true, 1, 1, true>(p, st) : launch_few<false, 1, 1, true>(p, st);
-        if (columns == 2) return nv ? launch_few<true, 1, 2, true>(p, st) : launch_few<false, 1, 2, true>(p, st);
+        if (columns == 2 && !nv) return launch_few<false, 1, 2, true>(p, st);
         if (columns <= 8) return nv ? launch_few<true, 1, 1, false>(p, st) : launch_few<false, 1, 1, false>(p, st);
         return nv ? launch_few<true, 1, 2, false>(p, st) : launch_few<false, 1, 2, false>(p, st);
     }

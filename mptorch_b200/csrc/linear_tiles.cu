@@ -13,7 +13,10 @@
 //      Sums are fp32 in tensor memory, those of float32's second pieces apart, and the powers of two are put back at the end.
 //   3. A tile that a run ends in is left in parts, which are added up in order.
 //
-// Measured figures stand at the launch rule below.
+// Measured on a B200 (bf16 products at the measured rate and bytes at the measured bandwidth in brackets): 37 x 4096 by 11008 NVFP4
+// weights, float16, 36.8 us (4.1 of bytes: x's tiles, the parts of cut tiles and three kernels' starts are most of it); 1024 x 4096 by
+// 4096 MXFP4 weights, float32, 120 us (42 of products, two pieces each); 1024 x 4096 by 11008 NVFP4, bfloat16, 176 us (56).  What bounds
+// it is the instruction issue of the warps that turn codes into weights, once for every 256 columns of x.
 #include "blocklinear.cuh"
 #include "launch.cuh"
 #include "tcgen05.cuh"
@@ -21,10 +24,8 @@
 namespace mpt {
 namespace {
 
-#ifndef MPT_TILE_WORKERS
-#define MPT_TILE_WORKERS 512
-#endif
-constexpr int kRowsW = 128, kBlock = 64, kSuper = 4, kWorkers = MPT_TILE_WORKERS, kThreads = kWorkers + 64, kRowStep = kWorkers / 8, kEach = kRowsW / kRowStep;   // codes are read in pieces of four blocks
+// Sixteen warps for the weights: 1024 x 4096 by 4096 MXFP4, float32, took 130 us with eight and takes 120 with sixteen.
+constexpr int kRowsW = 128, kBlock = 64, kSuper = 4, kWorkers = 512, kThreads = kWorkers + 64, kRowStep = kWorkers / 8, kEach = kRowsW / kRowStep;   // codes are read in pieces of four blocks
 constexpr int kPartW = kRowsW * 128;                               // bytes of a tile of W: 128 rows of 64 weights
 
 struct TilesParams {
@@ -329,7 +330,6 @@ __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_con
                         // (a lane does not use a place each turn, but its blocks are at most seven apart and the ring has seven places
                         // at least: the phase before the one that it waits for is over)
                         if (t > 0) bar_wait(w_empty(s), (t - 1) & 1, &failed);
-                        __syncwarp(__activemask());            // the lanes wait for different places, and go on together
                         const bool inside = super * 8 + c <= last;
 #pragma unroll
                         for (int v = 0; v < kEach; ++v) {
@@ -431,15 +431,16 @@ TilesPlan tiles_plan(int64_t rows, int64_t n_out, int64_t n_in, int dtype) {
     pl.col_tiles = (int)((rows + pl.cols - 1) / pl.cols);
     pl.row_tiles = (int)((n_out + kRowsW - 1) / kRowsW);
     pl.k_blocks = n_in > 0 ? (int)((n_in + kBlock - 1) / kBlock) : 1;
-    // rings: where x's tiles are small, places of four blocks; else single blocks, x's ring covering the latency of a copy with three, the
-    // rest being W's (four blocks at least, a piece of which is written before it is waited for)
+    // Rings: where x's tiles are small, places of four blocks (24 rows of 4096 by 11008 NVFP4, bfloat16: 33 us, 40 with single blocks; 64
+    // rows: 41 and 48); else single blocks, since two places of four would not fit.  x's ring covers the latency of a copy with three
+    // places or four, the rest is W's: seven places at least, which the wait of a worker's lane counts on.
     const int x_bytes = pl.pieces * pl.cols * 128, room = 219 * 1024;
     pl.ring_blocks = x_bytes <= 8 * 1024 ? kSuper : 1;
     pl.x_stages = pl.ring_blocks > 1 ? 2 : x_bytes <= 16 * 1024 ? 4 : 3;
     pl.w_stages = (room - pl.x_stages * pl.ring_blocks * x_bytes) / (pl.ring_blocks * kPartW);
     if (pl.w_stages > kMaxStages) pl.w_stages = kMaxStages;
-    // (single blocks: 7 places with 32 kB of x, more with less)
-    // equal runs, one for each SM; or whole tiles, where their number leaves hardly an SM idle
+    // Equal runs, one for each SM; or whole tiles, where their number leaves at most a sixteenth of the SMs' time idle: no parts and no
+    // third kernel (1024 x 768 by 50257 MXFP4, bfloat16: 263 us, 303 in equal runs).
     const int64_t tiles = (int64_t)pl.row_tiles * pl.col_tiles, sms = sm_count(), rounds = (tiles + sms - 1) / sms;
     pl.k_supers = (pl.k_blocks + kSuper - 1) / kSuper;
     pl.units = tiles * pl.k_supers;

@@ -468,7 +468,7 @@ def test_attention_rows_that_see_nothing(q, dtype, new):
     got = q.mx_attention(flat, cache, pages, ln, starts)
     assert not got[new + 1:].any()
     mine = torch.full_like(flat, 7)
-    assert q.mx_attention(flat, cache, pages, ln, starts, out=mine) is mine or True
+    q.mx_attention(flat, cache, pages, ln, starts, out=mine)
     assert torch.equal(mine[:new + 1], got[:new + 1]) and (mine[new + 1:] == 7).all()
     assert q.mx_attention(flat[:0], cache, pages, ln, cumulative([0] * 4)).shape == (0, 4, 64)
 
