@@ -9,7 +9,7 @@
 // m is moved, and O multiplied, only when a row's maximum has grown by more than 2^8 over it; p is at most 2^8 then.
 //
 // Accuracy.  bfloat16 queries are one operand; float16 and float32 ones are the sum of two and three bfloat16 pieces (16 and 24
-// bits), and so are their weights p; sums are fp32 throughout.
+// bits), and so are their weights p; sums are fp32 throughout, and short ones where three pieces are worth it (kFold).
 //
 // Measured on a B200: 1024-token chunks of two sequences over 8192, 32 heads on 8 of 128, E4M3, bfloat16 310 us (115.5 for the
 // products at the measured rate of bfloat16; 610 TFLOP/s).  The expansion takes 20 us of it and the join of cut tiles some 10; what bounds
@@ -23,6 +23,10 @@ namespace mpt {
 namespace {
 
 constexpr int kTile = 128, kPart = 128 * 128;                     // tokens and rows of a tile; bytes of 128 rows of 64 values
+// Three pieces: the tensor cores cut their sums off instead of rounding them, an error that grows with the context.  After every fourth
+// tile the sums are added to fp32 sums in registers and begun again.  384 rows over 3438, head_dim 128: 2.9e-6 of the result without,
+// 1.3e-6 with every eighth, 8e-7 with every fourth (fp32 arithmetic as torch has it 1.6e-6), all of them in 220 us.
+constexpr int kFold = 4;
 constexpr int kTrailer = 256;                                     // there[4], any V block NaN, -, -, -, then a byte of blocks for each token
 
 __host__ __device__ constexpr int parts_for(int dim) { return (dim + 63) / 64; }
@@ -246,11 +250,11 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
                     const uint64_t q_desc = tile_descriptor(q_u, 16), k_desc = tile_descriptor(k_u, 16);
                     const uint32_t to = tm + (NS == 2 ? (it & 1) * 128 : 0);
 #pragma unroll
-                    for (int k = 0; k < PIECES; ++k)
+                    for (int k = PIECES - 1; k >= 0; --k)             // the smallest first, while the sums are small
 #pragma unroll
                         for (int s = 0; s < DIM / 16; ++s)
                             mma_ss(to, q_desc + (((k * Shape::parts + (s >> 2)) * kPart + (s & 3) * 32) >> 4), k_desc + (((s >> 2) * kPart + (s & 3) * 32) >> 4), score_desc,
-                                   k + s > 0, leader);
+                                   k < PIECES - 1 || s > 0, leader);
                     mma_commit(bar(NS == 2 && (it & 1) ? kScores2 : kScores), leader);
                     mma_commit(bar(kKEmpty), leader);
                     return true;
@@ -270,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
 #pragma unroll
                         for (int s = 0; s < 8; ++s)
                             mma_ts(tm + (PIECES == 3 && k > 0 ? Shape::small : Shape::sums), w + s * 8, v_desc + (s * 2048 >> 4), value_desc,
-                                   i > 0 || s > 0 || k > (PIECES == 3 ? 1 : 0), leader);
+                                   (PIECES == 3 ? i % kFold > 0 : i > 0) || s > 0 || k > (PIECES == 3 ? 1 : 0), leader);
                     }
                     mma_commit(bar(values_bar(it)), leader);
                     mma_commit(bar(kVEmpty), leader);
@@ -285,8 +289,24 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
             const int pos = r < count ? pos0 + (first + r) / p.group : -1;
             float m = -INFINITY, l = 0.f;
             uint32_t poison = 0u;
+            constexpr int kTotal = PIECES == 3 ? DIM / 32 : 1;    // blocks of 16 columns, which the halves take in turn
+            float total[kTotal][16] = {};
             for (int i = 0; i < n; ++i) {
                 const uint32_t it = it0 + i, turn = NS == 2 ? it & 1 : 0, set = turn * 128;
+                if (PIECES == 3 && i > 0 && i % kFold == 0) {
+                    wait_values(it - 1);
+                    __syncwarp();
+                    tmem_fence_after();
+#pragma unroll
+                    for (int j = 0; j < kTotal; ++j) {
+                        uint32_t o[16], o2[16];
+                        tmem_load16(mine + Shape::sums + 16 * half + 32 * j, o);
+                        tmem_load16(mine + Shape::small + 16 * half + 32 * j, o2);
+                        tmem_wait_load();
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) total[j][k] += __uint_as_float(o[k]) + __uint_as_float(o2[k]);
+                    }
+                }
                 wait(turn ? kScores2 : kScores, NS == 2 ? it >> 1 : it);
                 __syncwarp();
                 tmem_fence_after();
@@ -332,7 +352,13 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
                     const float next = fmaxf(m, top), fade = next == -INFINITY ? 1.f : exp2_fast(m - next);
                     m = next;
                     l *= fade;
-                    if (i > 0) {
+                    if (PIECES == 3) {
+#pragma unroll
+                        for (int j = 0; j < kTotal; ++j)
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) total[j][k] *= fade;
+                    }
+                    if (PIECES == 3 ? i % kFold > 0 : i > 0) {
                         wait_values(it - 1);
                         __syncwarp();
                         tmem_fence_after();
@@ -393,8 +419,8 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
             const int64_t out_row = ((int64_t)(own.x + tok) * p.q_heads + head * p.group + rr - tok * p.group) * DIM;
             const int share = 2 * blockIdx.x + (run.begins ? 0 : 1);
             const float times = !ok ? __uint_as_float(0x7FC00000u) : finished ? (l == 0.f ? 0.f : __frcp_rn(l)) : 1.f;
-#pragma unroll 1
-            for (int b = 16 * half; b < DIM; b += 32) {           // the halves take blocks of 16 columns in turn
+#pragma unroll(PIECES == 3 ? kTotal : 1)
+            for (int b = 16 * half, j = 0; j < DIM / 32; b += 32, ++j) {      // the halves take blocks of 16 columns in turn
                 uint32_t o[16];
                 tmem_load16(mine + Shape::sums + b, o);
                 tmem_wait_load();
@@ -403,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
                     tmem_load16(mine + Shape::small + b, o2);
                     tmem_wait_load();
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) + __uint_as_float(o2[k]));
+                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(total[j][k] + (__uint_as_float(o[k]) + __uint_as_float(o2[k])));
                 }
                 if (r < count) {
                     const bool bad = (poison >> (b >> 5)) & 1u;
