@@ -374,9 +374,8 @@ using namespace mpt;
 extern "C" {
 
 size_t mpt_block_linear_workspace_bytes(int64_t rows, int64_t n_out, int64_t n_in, int format, int dtype) {
-    (void)format;
     if (rows <= 0 || n_out <= 0 || n_in < 0 || rows > 0x7FFFFFFF || n_out > 0x7FFFFFFF || n_in > 0x7FFFFFFF || few_rows(rows, n_in, dtype)) return 0;
-    return tiles_plan(rows, n_out, n_in, dtype).bytes;
+    return tiles_plan(rows, n_out, n_in, format, dtype).bytes;
 }
 
 int mpt_block_linear(const void* x, const uint8_t* codes, const uint8_t* scales, const float* global_scale, const void* bias, void* y,
@@ -404,7 +403,7 @@ int mpt_block_linear(const void* x, const uint8_t* codes, const uint8_t* scales,
         if (columns <= 8) return nv ? launch_few<true, 1, 1, false>(p, st) : launch_few<false, 1, 1, false>(p, st);
         return nv ? launch_few<true, 1, 2, false>(p, st) : launch_few<false, 1, 2, false>(p, st);
     }
-    const TilesPlan pl = tiles_plan(rows, n_out, n_in, dtype);
+    const TilesPlan pl = tiles_plan(rows, n_out, n_in, format, dtype);
     if (workspace_bytes < pl.bytes || !workspace || ((uintptr_t)workspace & 255u)) {
         set_error("block_linear: a workspace of %zu bytes at a multiple of 256 is needed", pl.bytes);
         return MPT_ERR_WORKSPACE;

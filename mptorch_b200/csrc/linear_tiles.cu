@@ -26,6 +26,12 @@ namespace {
 
 // Sixteen warps for the weights: 1024 x 4096 by 4096 MXFP4, float32, took 130 us with eight and takes 120 with sixteen.
 constexpr int kRowsW = 128, kBlock = 64, kSuper = 4, kWorkers = 512, kThreads = kWorkers + 64, kRowStep = kWorkers / 8, kEach = kRowsW / kRowStep;   // codes are read in pieces of four blocks
+// FOLD, float32 rows and NVFP4: the tensor cores cut their sums off instead of rounding them, an error that grows with the sum's length,
+// so after every kFold pieces (1536 of the sum) what there is is added to fp32 sums in memory and begun again.  1024 x 4096 by 4096:
+// 3.3e-6 of the result without, 1.7e-6 with 8, 1.1e-6 with 6, 8.1e-7 with 4 (fp32 arithmetic as torch has it 1.1e-6), in 110, 128, 145 and
+// 155 us.  MXFP4's sums lose less (1.3e-6 there, 1.7e-6 with 8128) and take 120 us without and 177 with 8, since the kernel has no
+// registers left.  bfloat16 and float16 round the result far more coarsely.
+constexpr int kFold = 6;
 constexpr int kPartW = kRowsW * 128;                               // bytes of a tile of W: 128 rows of 64 weights
 
 struct TilesParams {
@@ -36,6 +42,8 @@ struct TilesParams {
     const uint8_t* image;              // x: [column tile][block of 64][piece][cols][128 bytes]
     int* exponent;                     // of each row of x
     float* partial;                    // of tiles that are cut: [slot][column][128]
+    int fold;                          // pieces after which sums are added up in memory and begun again
+    float* kept;                       // there: [run][column][128]
 };
 
 // ---- x into tiles: a CTA for a row
@@ -110,9 +118,11 @@ __device__ __forceinline__ int row_top(const TilesParams& p, int n, int c) {
     return top;
 }
 
-// A tile's sums, or a run's part of them: a thread has one row of W; the warps of each quarter of rows take every fourth 16 columns.
-template <bool NV>
-__device__ __noinline__ void tile_end(const TilesParams& p, uint32_t tmem, const int* top_e, int tile, bool whole, bool begins, bool ok) {
+// A tile's sums, or a run's part of them, or (`more`) those of some pieces of it, which are kept for the next ones (`carry`): a thread has one row of W; the warps of each quarter of rows take every fourth 16 columns.
+constexpr uint32_t kEnded = 1u, kWhole = 2u, kCarry = 4u, kMore = 8u, kNext = 16u;     // kNext: the run's next piece is another tile's
+template <bool NV, bool FOLD>
+__device__ __noinline__ void tile_end(const TilesParams& p, uint32_t tmem, const int* top_e, int tile, uint32_t what, bool begins, bool ok) {
+    const bool whole = what & kWhole, carry = FOLD && (what & kCarry), more = FOLD && (what & kMore);
     const LinearParams& l = p.l;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rt = tile / p.col_tiles, ct = tile - rt * p.col_tiles;
     tmem_fence_after();
@@ -123,8 +133,12 @@ __device__ __noinline__ void tile_end(const TilesParams& p, uint32_t tmem, const
     const bool near = we >= -60 && we <= 60;                       // no product leaves fp32's range on the way
     const float wpow = __uint_as_float((uint32_t)(127 + (near ? we : 0)) << 23);
     float* part = p.partial + (2 * (int64_t)blockIdx.x + (begins ? 0 : 1)) * p.cols * kRowsW + rw;
+    float* kept = p.kept + (int64_t)blockIdx.x * p.cols * kRowsW + rw;
     for (int c0 = 16 * (warp >> 2); c0 < p.cols; c0 += kWorkers / 8) {
         uint32_t v[16], v2[16];
+        float before[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) before[k] = carry && ct * p.cols + c0 + k < l.rows ? kept[(c0 + k) * kRowsW] : 0.f;
         const int m_lane = ct * p.cols + c0 + (lane & 15), mine = m_lane < l.rows ? p.exponent[m_lane] : 0;
         tmem_load16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0, v);
         if (p.pieces == 2) tmem_load16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + p.cols + c0, v2);
@@ -138,8 +152,10 @@ __device__ __noinline__ void tile_end(const TilesParams& p, uint32_t tmem, const
                 if (near) y = y * wpow * __uint_as_float((uint32_t)(127 - xe) << 23);
                 else y = scale_by_power(y, we - xe);
                 y *= glob;
+                if (carry) y += before[k];
                 if (!ok) y = __uint_as_float(0x7FC00000u);
-                if (!whole) part[(c0 + k) * kRowsW] = y;
+                if (more) kept[(c0 + k) * kRowsW] = y;
+                else if (!whole) part[(c0 + k) * kRowsW] = y;
                 else if (n < l.n_out) write_value(l.y, l.dtype, (int64_t)m * l.n_out + n, y + bias);
             }
         }
@@ -150,7 +166,7 @@ __device__ __noinline__ void tile_end(const TilesParams& p, uint32_t tmem, const
 
 // PER: blocks of a place in the rings, one or (where x's tiles are small) the four of a piece: what is waited for and handed on costs some
 // hundred clocks each time.
-template <bool NV, int PER>
+template <bool NV, int PER, bool FOLD>
 __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_constant__ TilesParams p) {
     next_may_start();
     extern __shared__ uint8_t smem_raw[];
@@ -213,7 +229,7 @@ __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_con
             const uint32_t sums = uniform(tmem), ring = uniform(base);
             const int n = p.pieces * p.cols;                       // the pieces' columns side by side, sums apart
             const uint32_t desc = half_product_descriptor(n);
-            int super = super0, ws = 0, wt = 0, xs = 0, xt = 0, t = 0;
+            int super = super0, fold = p.fold - super0 % p.fold, ws = 0, wt = 0, xs = 0, xt = 0, t = 0;
             bool first = true, ok = true;
             for (int i = 0; ok && i < count; ++i) {
                 if (first && t > 1 && !(ok = __all_sync(0xFFFFFFFFu, bar_wait(taken(t), ((t >> 1) - 1) & 1, &failed)))) break;
@@ -241,10 +257,11 @@ __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_con
                     if (++xs == p.x_stages) { xs = 0; ++xt; }
                 }
                 if (++super == p.k_supers) super = 0;
-                if (super == 0 || i + 1 == count) {
+                if (super == 0 || (FOLD && --fold == 0) || i + 1 == count) {
                     mma_commit(done(t), leader);
                     ++t;
                     first = true;
+                    fold = p.fold;
                 }
             }
         }
@@ -291,35 +308,36 @@ __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_con
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) fetch(ahead[a], ahead_s[a]);
 
-        int tile = tile0, super = super0, seg_end = min(p.k_supers - super0, count), tiles = 0, i = 0, stage = 0, turn = 0, top[kEach];
-        bool whole = seg_end == p.k_supers;                        // the run has all pieces of the tile
-        int ended = -1;                                            // a tile whose sums have not been read yet
-        bool ended_whole = false;
+        // Sums are read `ends` times in all: at the end of each tile, and after every p.fold pieces of one.
+        int tile = tile0, super = super0, ends = 0, i = 0, stage = 0, turn = 0, fold = p.fold - super0 % p.fold, top[kEach];
+        uint32_t ended = 0u;                                       // sums that have not been read yet, and of what they are
+        uint32_t carry = 0u;                                       // kCarry, if there are kept sums of this tile
         int ct = tile0 % p.col_tiles, rt = tile0 / p.col_tiles;
         bool live[kEach];
-        auto begin_rows = [&](int t) {
+        auto begin_rows = [&](int t, bool next) {
 #pragma unroll
             for (int h = 0; h < kEach; ++h) {
                 const int n = rt * kRowsW + r + kRowStep * h;
                 live[h] = n < l.n_out;
-                if (t == 0 || ct == 0) top[h] = row_top<NV>(p, n, c);          // otherwise the same rows again
+                if (t == 0 || (next && ct == 0)) top[h] = row_top<NV>(p, n, c);          // otherwise the same rows again
                 if (!NV && c == 0) top_e[t & 1][r + kRowStep * h] = top[h];
             }
         };
-        auto end_tile = [&]() {                                    // tile `tiles - 1` of the run
-            bar_wait(done(tiles - 1), ((tiles - 1) >> 1) & 1, &failed);
-            if (tiles == 1) wait_for_previous();                   // the exponents of x
+        auto end_tile = [&]() {                                    // time `ends - 1`
+            bar_wait(done(ends - 1), ((ends - 1) >> 1) & 1, &failed);
+            if (ends == 1) wait_for_previous();                   // the exponents of x
             asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory");      // and every thread's part of top_e
-            tile_end<NV>(p, tmem + ((tiles - 1) & 1) * (p.columns >> 1), top_e[(tiles - 1) & 1], ended, ended_whole, tiles == 1, *(volatile uint32_t*)&failed == 0u);
-            bar_arrive(taken(tiles - 1));
-            ended = -1;
+            tile_end<NV, FOLD>(p, tmem + ((ends - 1) & 1) * (p.columns >> 1), top_e[(ends - 1) & 1], tile - (ended & kNext ? 1 : 0), ended, tile - (ended & kNext ? 1 : 0) == tile0, *(volatile uint32_t*)&failed == 0u);
+            bar_arrive(taken(ends - 1));
+            ended = 0u;
             asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory");      // top_e has been read
         };
-        begin_rows(0);
-        while (i < count || ended >= 0) {
+        begin_rows(0, true);
+        while (i < count || ended) {
 #pragma unroll
             for (int a = 0; a < kAhead; ++a) {
-                if (i < count) {
+                const bool worked = i < count;
+                if (worked) {
                     const int blocks = blocks_of(super);
                     int s = stage, t = turn;
                     if (PER == 1) {
@@ -368,23 +386,23 @@ __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_con
                     if (stage >= p.w_stages) { stage -= p.w_stages; ++turn; }
                     if (++super == p.k_supers) super = 0;
                     ++i;
+                    --fold;
                 }
                 // the sums of a tile are read when the first piece of the next one is under way
-                if (ended >= 0) end_tile();
-                if (i == seg_end) {
-                    ended = tile;
-                    ended_whole = whole;
-                    ++tiles;
-                    if (i < count) {
-                        seg_end = min(i + p.k_supers, count);
-                        whole = seg_end - i == p.k_supers;
+                if (ended) end_tile();
+                if (worked && (super == 0 || (FOLD && fold == 0) || i == count)) {
+                    const bool more = FOLD && super != 0 && i < count;     // pieces of this tile
+                    ended = kEnded | carry | (more ? kMore : 0u) | (super == 0 && i >= p.k_supers ? kWhole : 0u);
+                    carry = more ? kCarry : 0u;
+                    fold = p.fold;
+                    ++ends;
+                    if (!more) {
                         ++tile;
+                        ended |= kNext;
                         if (++ct == p.col_tiles) { ct = 0; ++rt; }
-                        begin_rows(tiles);
-                    } else {
-                        seg_end = -1;
-                        end_tile();
                     }
+                    if (i < count) begin_rows(ends, !more);
+                    else end_tile();
                 }
             }
         }
@@ -421,7 +439,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const TilesParams p) {
 
 }  // namespace
 
-TilesPlan tiles_plan(int64_t rows, int64_t n_out, int64_t n_in, int dtype) {
+TilesPlan tiles_plan(int64_t rows, int64_t n_out, int64_t n_in, int format, int dtype) {
     TilesPlan pl;
     pl.pieces = dtype == MPT_DTYPE_F32 ? 2 : 1;
     const int64_t most = 256 / pl.pieces;
@@ -451,7 +469,9 @@ TilesPlan tiles_plan(int64_t rows, int64_t n_out, int64_t n_in, int dtype) {
     pl.columns = used <= 16 ? 32 : used <= 32 ? 64 : used <= 64 ? 128 : used <= 128 ? 256 : 512;      // two sets of sums
     pl.image_bytes = (size_t)pl.col_tiles * pl.k_blocks * pl.pieces * pl.cols * 128;
     pl.partial_bytes = pl.runs > 1 && pl.per % pl.k_supers ? (size_t)2 * pl.runs * pl.cols * kRowsW * 4 : 0;
-    pl.bytes = pl.image_bytes + ((size_t)rows * 4 + 255) / 256 * 256 + pl.partial_bytes;
+    pl.fold = format == MPT_BLOCK_NVFP4 && pl.pieces == 2 && pl.k_supers > kFold ? kFold : pl.k_supers;
+    pl.kept_bytes = pl.fold < pl.k_supers ? (size_t)pl.runs * pl.cols * kRowsW * 4 : 0;
+    pl.bytes = pl.image_bytes + ((size_t)rows * 4 + 255) / 256 * 256 + pl.partial_bytes + pl.kept_bytes;
     return pl;
 }
 
@@ -462,6 +482,8 @@ int launch_tiles(const LinearParams& l, const TilesPlan& pl, int format, uint8_t
     p.image = workspace;
     p.exponent = reinterpret_cast<int*>(workspace + pl.image_bytes);
     p.partial = reinterpret_cast<float*>(workspace + pl.image_bytes + ((size_t)l.rows * 4 + 255) / 256 * 256);
+    p.fold = pl.fold;
+    p.kept = p.partial + pl.partial_bytes / 4;
     linear_split_kernel<<<(unsigned)l.rows, 256, 0, st>>>(p, workspace);
     const int bytes = 1024 + pl.ring_blocks * (pl.w_stages * kPartW + pl.x_stages * pl.pieces * pl.cols * 128);
     const bool nv = format == MPT_BLOCK_NVFP4, single = pl.ring_blocks == 1;
@@ -471,10 +493,13 @@ int launch_tiles(const LinearParams& l, const TilesPlan& pl, int format, uint8_t
         launch_after(kern, dim3((unsigned)pl.runs), dim3(kThreads), bytes, st, p);
         return true;
     };
-    const bool fine = nv ? (single ? launch(linear_tiles_kernel<true, 1>, allow_shared<linear_tiles_kernel<true, 1>>(most))
-                                   : launch(linear_tiles_kernel<true, kSuper>, allow_shared<linear_tiles_kernel<true, kSuper>>(most)))
-                         : (single ? launch(linear_tiles_kernel<false, 1>, allow_shared<linear_tiles_kernel<false, 1>>(most))
-                                   : launch(linear_tiles_kernel<false, kSuper>, allow_shared<linear_tiles_kernel<false, kSuper>>(most)));
+    const bool fold = pl.fold < pl.k_supers;
+    const bool fine = nv ? (fold ? (single ? launch(linear_tiles_kernel<true, 1, true>, allow_shared<linear_tiles_kernel<true, 1, true>>(most))
+                                           : launch(linear_tiles_kernel<true, kSuper, true>, allow_shared<linear_tiles_kernel<true, kSuper, true>>(most)))
+                                 : (single ? launch(linear_tiles_kernel<true, 1, false>, allow_shared<linear_tiles_kernel<true, 1, false>>(most))
+                                           : launch(linear_tiles_kernel<true, kSuper, false>, allow_shared<linear_tiles_kernel<true, kSuper, false>>(most))))
+                         : (single ? launch(linear_tiles_kernel<false, 1, false>, allow_shared<linear_tiles_kernel<false, 1, false>>(most))
+                                   : launch(linear_tiles_kernel<false, kSuper, false>, allow_shared<linear_tiles_kernel<false, kSuper, false>>(most)));
     if (!fine) {
         check_launch("block_linear");
         set_error("block_linear: the kernel does not fit this device");

@@ -121,6 +121,21 @@ def test_linear(q, fmt, dtype, rows, n, k):
 
 
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,n,k", [(24, 20000, 1568), (33, 130, 1536), (40, 700, 6400), (130, 2600, 3232), (200, 4000, 1792), (260, 200, 9632), (300, 9000, 2048)])
+def test_linear_long_sums(q, fmt, dtype, rows, n, k):
+    """Sums that are added up in memory piece by piece, in tiles that are cut and in whole ones, twice the same bits."""
+    g = gen(rows + n + k)
+    codes, scales, glob, w = pack(n, k, fmt, g)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(dtype)
+    bias = torch.randn(n, device="cuda", generator=g).to(dtype)
+    y = linear(q, x, codes, scales, glob, bias)
+    check_linear(y, x, w, bias)
+    for _ in range(2):
+        assert torch.equal(linear(q, x, codes, scales, glob, bias), y)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
 @pytest.mark.parametrize("rows", [1, 3, 24, 200])
 def test_linear_range_of_x(q, fmt, rows):
     """Values of x over many orders of magnitude, within a row and between rows, keep fp32's accuracy."""
