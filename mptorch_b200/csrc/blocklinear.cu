@@ -14,7 +14,8 @@
 //
 // Measured on a B200 (weights' bytes at the measured bandwidth in brackets): one bfloat16 row of 8192 by 28672 NVFP4 weights 39 us
 // (20.2); three float32 rows of 768 by 50257 MXFP4 weights 14.4 us (3.2); one of 768 by 2304 9.7 us (0.1: host time and a launch).
-// Some 39 instructions for 512 weights bound the largest, not the memory: copies of twice the depth changed nothing.
+// The largest has its issue slots 55 % busy and DRAM 43 %: four warps a scheduler do not cover the fixed latency between an instruction
+// and the next that needs it (39 of them for 512 weights).  Copies of twice the depth changed nothing.
 #include "blocklinear.cuh"
 #include "launch.cuh"
 

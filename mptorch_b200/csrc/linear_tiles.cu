@@ -16,7 +16,8 @@
 // Measured on a B200 (bf16 products at the measured rate and bytes at the measured bandwidth in brackets): 37 x 4096 by 11008 NVFP4
 // weights, float16, 36.8 us (4.1 of bytes: x's tiles, the parts of cut tiles and three kernels' starts are most of it); 1024 x 4096 by
 // 4096 MXFP4 weights, float32, 120 us (42 of products, two pieces each); 1024 x 4096 by 11008 NVFP4, bfloat16, 176 us (56).  What bounds
-// it is the instruction issue of the warps that turn codes into weights, once for every 256 columns of x.
+// it is the warps that turn codes into weights, again for every 256 columns of x (128 rows of float32): they wait for places in the
+// ring and for codes on the way, with the issue slots 35 % busy and the tensor cores 37 % in the second of these.
 #include "blocklinear.cuh"
 #include "launch.cuh"
 #include "tcgen05.cuh"
