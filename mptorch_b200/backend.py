@@ -927,7 +927,7 @@ def mx_attention(q, cache, pages, lens, starts=None, scale=1.0, window=0, sinks=
         raise RuntimeError("%s: window and sinks must not be negative" % who)
     if out is not None:
         _whole(who, "out", out, q.dtype, tuple(q.shape))
-    _no_gradient(who, q)
+    _no_gradient(who, q, *([out] if out is not None else []))
     _on_device(who, q, out=out, k_codes=cache[0], k_scales=cache[1], v_codes=cache[2], v_scales=cache[3], pages=pages, lens=lens, starts=starts)
     with torch.cuda.device(q.device):
         q = q if q.stride(-1) == 1 else q.contiguous()

@@ -16,8 +16,8 @@ template <auto Kern>
 bool allow_shared(int bytes) {
     static std::atomic<uint64_t> asked{0};
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
-    const uint64_t bit = (uint64_t)1 << dev;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;       // (devices behind the 64th are asked each time)
     if (asked.load(std::memory_order_relaxed) & bit) return true;
     if (cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
     asked.fetch_or(bit, std::memory_order_relaxed);

@@ -575,6 +575,7 @@ at::Tensor mx_attention(at::Tensor q_in, std::vector<at::Tensor> cache, at::Tens
         TORCH_CHECK(out_in->sizes() == q_in.sizes() && out_in->scalar_type() == q_in.scalar_type() && out_in->is_contiguous(), who,
                     ": out must be contiguous with the shape and type of q");
     no_gradient(who, q_in);
+    if (out_in) no_gradient(who, *out_in);
     TORCH_CHECK(q_in.is_cuda(), who, ": q must be a CUDA tensor");
     if (out_in) same_device(who, "out", *out_in, q_in);
     serving_devices(who, q_in, cache, pages, lens, starts);

@@ -79,6 +79,7 @@ def test_cache_and_attention():
     refused("negative", q.mx_attention, k, cache, p, n, window=4, sinks=-1)
     refused("out", q.mx_attention, k, cache, p, n, out=torch.zeros(2, 1, 2, 32))
     refused("out", q.mx_attention, k, cache, p, n, out=torch.zeros(2, 1, 2, 64, dtype=torch.half))
+    refused("backward", q.mx_attention, k, cache, p, n, out=torch.zeros(2, 1, 2, 64, requires_grad=True))
     refused("CUDA", q.mx_cache_read, cache, p, n, 1)
     refused("negative", q.mx_cache_read, cache, p, n, -1)
 
