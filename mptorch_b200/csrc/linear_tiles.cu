@@ -18,6 +18,8 @@
 // 4096 MXFP4 weights, float32, 120 us (42 of products, two pieces each); 1024 x 4096 by 11008 NVFP4, bfloat16, 176 us (56).  What bounds
 // it is the warps that turn codes into weights, again for every 256 columns of x (128 rows of float32): they wait for places in the
 // ring and for codes on the way, with the issue slots 35 % busy and the tensor cores 37 % in the second of these.
+#include <type_traits>
+
 #include "blocklinear.cuh"
 #include "launch.cuh"
 #include "tcgen05.cuh"
@@ -27,12 +29,13 @@ namespace {
 
 // Sixteen warps for the weights: 1024 x 4096 by 4096 MXFP4, float32, took 130 us with eight and takes 120 with sixteen.
 constexpr int kRowsW = 128, kBlock = 64, kSuper = 4, kWorkers = 512, kThreads = kWorkers + 64, kRowStep = kWorkers / 8, kEach = kRowsW / kRowStep;   // codes are read in pieces of four blocks
-// FOLD, float32 rows and NVFP4: the tensor cores cut their sums off instead of rounding them, an error that grows with the sum's length,
-// so after every kFold pieces (1536 of the sum) what there is is added to fp32 sums in memory and begun again.  1024 x 4096 by 4096:
-// 3.3e-6 of the result without, 1.7e-6 with 8, 1.1e-6 with 6, 8.1e-7 with 4 (fp32 arithmetic as torch has it 1.1e-6), in 110, 128, 145 and
-// 155 us.  MXFP4's sums lose less (1.3e-6 there, 1.7e-6 with 8128) and take 120 us without and 177 with 8, since the kernel has no
-// registers left.  bfloat16 and float16 round the result far more coarsely.
-constexpr int kFold = 6;
+// FOLD, float32 rows: the tensor cores cut their sums off instead of rounding them, an error that grows with the sum's length, so after
+// every kFoldNv or kFoldMx pieces (1536 and 4096 of the sum) what there is is added to fp32 sums in memory and begun again.  NVFP4, 1024
+// x 4096 by 4096: 3.3e-6 of the result without, 1.7e-6 with 8, 1.1e-6 with 6, 8.1e-7 with 4 (fp32 arithmetic as torch has it 1.1e-6), in
+// 110, 128, 145 and 155 us.  MXFP4 loses less: 33 x 4096 by 18889 1.7e-6 without, 9152 4.4e-6 without and 1.5e-6 with 16 (torch's 1.1e-6
+// and 1.6e-6), the last in 151 us; it pays more for it, since that kernel has no registers left (1024 x 4096 by 4096: 120 us without,
+// 177 with 8).  bfloat16 and float16 round the result far more coarsely.
+constexpr int kFoldNv = 6, kFoldMx = 16;
 constexpr int kPartW = kRowsW * 128;                               // bytes of a tile of W: 128 rows of 64 weights
 
 struct TilesParams {
@@ -470,7 +473,8 @@ TilesPlan tiles_plan(int64_t rows, int64_t n_out, int64_t n_in, int format, int 
     pl.columns = used <= 16 ? 32 : used <= 32 ? 64 : used <= 64 ? 128 : used <= 128 ? 256 : 512;      // two sets of sums
     pl.image_bytes = (size_t)pl.col_tiles * pl.k_blocks * pl.pieces * pl.cols * 128;
     pl.partial_bytes = pl.runs > 1 && pl.per % pl.k_supers ? (size_t)2 * pl.runs * pl.cols * kRowsW * 4 : 0;
-    pl.fold = format == MPT_BLOCK_NVFP4 && pl.pieces == 2 && pl.k_supers > kFold ? kFold : pl.k_supers;
+    const int fold = format == MPT_BLOCK_NVFP4 ? kFoldNv : kFoldMx;
+    pl.fold = pl.pieces == 2 && pl.k_supers > fold ? fold : pl.k_supers;
     pl.kept_bytes = pl.fold < pl.k_supers ? (size_t)pl.runs * pl.cols * kRowsW * 4 : 0;
     pl.bytes = pl.image_bytes + ((size_t)rows * 4 + 255) / 256 * 256 + pl.partial_bytes + pl.kept_bytes;
     return pl;
@@ -495,12 +499,14 @@ int launch_tiles(const LinearParams& l, const TilesPlan& pl, int format, uint8_t
         return true;
     };
     const bool fold = pl.fold < pl.k_supers;
-    const bool fine = nv ? (fold ? (single ? launch(linear_tiles_kernel<true, 1, true>, allow_shared<linear_tiles_kernel<true, 1, true>>(most))
-                                           : launch(linear_tiles_kernel<true, kSuper, true>, allow_shared<linear_tiles_kernel<true, kSuper, true>>(most)))
-                                 : (single ? launch(linear_tiles_kernel<true, 1, false>, allow_shared<linear_tiles_kernel<true, 1, false>>(most))
-                                           : launch(linear_tiles_kernel<true, kSuper, false>, allow_shared<linear_tiles_kernel<true, kSuper, false>>(most))))
-                         : (single ? launch(linear_tiles_kernel<false, 1, false>, allow_shared<linear_tiles_kernel<false, 1, false>>(most))
-                                   : launch(linear_tiles_kernel<false, kSuper, false>, allow_shared<linear_tiles_kernel<false, kSuper, false>>(most)));
+    auto choose = [&](auto nv_c, auto fold_c) {
+        constexpr bool kNv = decltype(nv_c)::value, kFolds = decltype(fold_c)::value;
+        return single ? launch(linear_tiles_kernel<kNv, 1, kFolds>, allow_shared<linear_tiles_kernel<kNv, 1, kFolds>>(most))
+                      : launch(linear_tiles_kernel<kNv, kSuper, kFolds>, allow_shared<linear_tiles_kernel<kNv, kSuper, kFolds>>(most));
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    const bool fine = nv ? (fold ? choose(Yes{}, Yes{}) : choose(Yes{}, No{})) : (fold ? choose(No{}, Yes{}) : choose(No{}, No{}));
     if (!fine) {
         check_launch("block_linear");
         set_error("block_linear: the kernel does not fit this device");
