@@ -14,7 +14,7 @@
 // Measured on a B200: 1024-token chunks of two sequences over 8192, 32 heads on 8 of 128, E4M3, bfloat16 310 us (115.5 for the
 // products at the measured rate of bfloat16; 610 TFLOP/s).  The expansion takes 20 us of it and the join of cut tiles some 10; what bounds
 // the rest is the chain of a tile, product, softmax, product, two CTAs on an SM hiding each other's.  Six ragged chunks up to 300 over
-// 2000, 12 heads of 64, float32: 81 us (2.9), three pieces of q and of p each, and runs of a few tiles.
+// 2000, 12 heads of 64, float32: 84 us (2.9), three pieces of q and of p each, and runs of a few tiles.
 #include "attention.cuh"
 #include "attention_chunk.cuh"
 #include "tcgen05.cuh"
