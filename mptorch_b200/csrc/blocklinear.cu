@@ -51,10 +51,10 @@ __device__ __forceinline__ float relative_power(int e, int ref) {
 
 __host__ __device__ constexpr int stage_bytes(bool nv) { return 16 * kPitch + 16 * (nv ? 8 : 4); }
 __host__ __device__ inline int x_pitch(int n_in) { return (n_in + kChunk - 1) / kChunk * kChunk * 2 + 64; }   // whole pieces; 64 bytes behind a multiple of 128
-inline int few_smem(int n_in, int columns, bool nv, int nt) {
-    const int ring = kWarps * kStages * stage_bytes(nv), sums = kWarps * 16 * 8 * nt * 4;
-    return columns * x_pitch(n_in) + ring + sums;
-}
+constexpr int few_smem(int x_bytes, bool nv, int nt) { return x_bytes + kWarps * kStages * stage_bytes(nv) + kWarps * 16 * 8 * nt * 4; }   // x, rings, sums
+// What few_rows admits of x, and the shared memory that the kernel is allowed: whatever is admitted can be launched.
+constexpr int kMostX = 140 * 1024, kMostShared = few_smem(kMostX, true, 2);
+static_assert(kMostShared + 2 * 1024 <= 227 * 1024, "2 kB for the kernel's static shared memory");
 
 // GROUPS: one column (NVFP4), one or two (MXFP4).  The other columns of the products are used to keep the scale groups apart: column c
 // has x where its group is c and zeros elsewhere, so that a column's sum over a piece of 128 is that of one group, and the scales
@@ -342,9 +342,9 @@ __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const 
 
 template <bool NV, int PIECES, int NT, bool GROUPS>
 int launch_few(const LinearParams& p, cudaStream_t st) {
-    const int bytes = few_smem(p.n_in, p.rows * PIECES, NV, NT), tiles = (p.n_out + 15) / 16;
+    const int bytes = few_smem(p.rows * PIECES * x_pitch(p.n_in), NV, NT), tiles = (p.n_out + 15) / 16;
     constexpr auto kern = block_linear_few_kernel<NV, PIECES, NT, GROUPS>;
-    if (!allow_shared<kern>(220 * 1024)) return check_launch("block_linear");
+    if (!allow_shared<kern>(kMostShared)) return check_launch("block_linear");
     // One CTA on each SM.  As many warps share a tile as take the least time: rounds of tiles times pieces of a warp, with two for the
     // end.  One row, MXFP4: 4096 by 4096 takes 10 us with eight that share, 19 where none do and 11 where all sixteen do; 768 by 50257
     // 14, 14 and 46; 8192 by 28672 50, 50 and 64.
@@ -364,7 +364,7 @@ int launch_few(const LinearParams& p, cudaStream_t st) {
 // More columns would need another set of sums for each eight, and 24 rows take the tiles 33.
 bool few_rows(int64_t rows, int64_t n_in, int dtype) {
     const int64_t columns = rows * (dtype == MPT_DTYPE_F32 ? 2 : 1);
-    return columns <= 16 && n_in <= 65536 && columns * x_pitch((int)n_in) <= 140 * 1024;
+    return columns <= 16 && n_in <= 65536 && columns * x_pitch((int)n_in) <= kMostX;
 }
 
 }  // namespace

@@ -668,3 +668,18 @@ def test_another_device_than_the_current_one(q):
     assert there.device == dev and torch.equal(there.cpu(), want.cpu())
     with pytest.raises(RuntimeError, match="expected"):
         q.mx_attention(qry.to(dev), cache, pages, ln, starts)
+
+
+# ---------------------------------------------------------------------------------- few rows of the products
+@pytest.mark.parametrize("dtype,rows,k", [(torch.bfloat16, 10, 6944), (torch.bfloat16, 10, 7040), (torch.bfloat16, 10, 7072), (torch.float16, 11, 6304),
+                                          (torch.float16, 11, 6400), (torch.float16, 11, 6432), (torch.bfloat16, 12, 5888), (torch.bfloat16, 12, 5920),
+                                          (torch.bfloat16, 15, 4640), (torch.bfloat16, 15, 4736), (torch.bfloat16, 15, 4768), (torch.float32, 5, 7040),
+                                          (torch.float32, 5, 7072), (torch.float32, 6, 5888), (torch.float32, 6, 5920), (torch.bfloat16, 16, 4384),
+                                          (torch.bfloat16, 1, 65536), (torch.bfloat16, 2, 35840), (torch.bfloat16, 9, 7808)])
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_linear_as_much_of_x_as_shared_memory_holds(q, fmt, dtype, rows, k):
+    """Sizes on both sides of what the kernel for a few rows takes."""
+    g = gen(rows + k)
+    codes, scales, glob, w = pack(40, k, fmt, g)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(dtype)
+    check_linear(linear(q, x, codes, scales, glob), x, w)
