@@ -8,8 +8,9 @@
 //
 // x is scaled for each row by a power of two to a largest value in [2^14, 2^15) and held as binary16: bfloat16 and float16 in one
 // column (exact unless a value is 2^-29 of the largest or less), float32 in two, the second 2^11 times what the first leaves (22
-// bits).  NVFP4: a code times its E4M3 scale is exact in binary16 (six bits), so the weights are scaled and the products summed in
-// fp32 as they are.  MXFP4: the scale of a block multiplies the fp32 sum of its 32 products, relative to an exponent that is kept
+// bits).  NVFP4: a code times its E4M3 scale is exact in binary16 (six bits), so the weights are scaled and the products of a piece of
+// 128 summed by the tensor cores; pieces are added up in fp32 registers, since the tensor cores cut their sums off instead of rounding
+// them (two float32 rows of 9600 by 33000: 2.4e-7 of the result, 1.1e-5 with sums that run through).  MXFP4: the scale of a block multiplies the fp32 sum of its 32 products, relative to an exponent that is kept
 // for each row of W and raised when a block exceeds it by 2^60, so that no range of scales overflows.
 //
 // Measured on a B200 (weights' bytes at the measured bandwidth in brackets): one bfloat16 row of 8192 by 28672 NVFP4 weights 39 us
@@ -246,6 +247,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const 
                     }
                 }
                 const int k0 = chunk * kChunk;
+                float part[NT][4];                                         // NVFP4: of this piece
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     uint32_t a[4], d[4];
@@ -266,8 +268,9 @@ __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const 
                         }
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            mma(acc[n], a[0], d[0], a[1], d[1], x[n].x, x[n].y);
-                            mma(acc[n], a[2], d[2], a[3], d[3], x[n].z, x[n].w);
+                            if (b == 0) mma_first(part[n], a[0], d[0], a[1], d[1], x[n].x, x[n].y);
+                            else mma(part[n], a[0], d[0], a[1], d[1], x[n].x, x[n].y);
+                            mma(part[n], a[2], d[2], a[3], d[3], x[n].z, x[n].w);
                         }
                     } else {
                         const int e0 = (s0.x >> (8 * b)) & 255u, e1 = (s1.x >> (8 * b)) & 255u;
@@ -284,6 +287,12 @@ __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const 
                             acc[n][3] = fmaf(c[3], f1, acc[n][3]);
                         }
                     }
+                }
+                if (NV) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[n][i] += part[n][i];
                 }
             }
             __syncwarp();

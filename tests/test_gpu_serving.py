@@ -683,3 +683,25 @@ def test_linear_as_much_of_x_as_shared_memory_holds(q, fmt, dtype, rows, k):
     codes, scales, glob, w = pack(40, k, fmt, g)
     x = torch.randn(rows, k, device="cuda", generator=g).to(dtype)
     check_linear(linear(q, x, codes, scales, glob), x, w)
+
+
+# Accuracy of long float32 sums.  The tensor cores cut their running sums off, by up to 2^-23 of the sum for each 16 products.  A kernel
+# that adds partial sums of S products up in fp32 is off by at most (S / 16) 2^-23 of the sum of magnitudes for the cut sums, always in
+# the same direction, and by roundings of random sign, sqrt(K / S) 2^-24, for the rest.  Of one sign, where nothing cancels, that is the
+# result's relative error; 2^-21 comes on top for x and the weights of a softmax in two binary16 pieces.
+def cut_off_bound(part, length):
+    return (part / 16) * 2.0 ** -23 + (math.sqrt(length / part) + 4) * 2.0 ** -24 + 2.0 ** -21
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("rows,n,k", [(1, 33000, 9600), (2, 33000, 9600), (5, 4000, 6880), (7, 20000, 4096), (8, 40, 8160), (1, 300, 32768)])
+def test_linear_few_rows_sums_of_one_sign(q, fmt, rows, n, k):
+    """No longer sums than 128 products are left to the tensor cores; sums that ran through were up to 4.5e-5 off."""
+    g = gen(rows + n)
+    codes, scales, glob, _ = pack(n, k, fmt, g)
+    codes &= 0x77
+    w = torch.stack([field_value(codes & 15, 2, 1), field_value(codes >> 4, 2, 1)], -1).flatten(-2)
+    w = w * (e8m0_value(scales).repeat_interleave(32, -1) if glob is None else e4m3_value(scales).repeat_interleave(16, -1) * glob.double())
+    x = torch.randn(rows, k, device="cuda", generator=g).abs()
+    want = x.double() @ w.t()
+    assert ((linear(q, x, codes, scales, glob).double() - want).norm() / want.norm()).item() <= cut_off_bound(128, k)
