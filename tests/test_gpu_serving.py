@@ -705,3 +705,23 @@ def test_linear_few_rows_sums_of_one_sign(q, fmt, rows, n, k):
     x = torch.randn(rows, k, device="cuda", generator=g).abs()
     want = x.double() @ w.t()
     assert ((linear(q, x, codes, scales, glob).double() - want).norm() / want.norm()).item() <= cut_off_bound(128, k)
+
+
+@pytest.mark.parametrize("lens,heads,group,dim", [([20000] * 64, 8, 1, 64), ([20000] * 16, 4, 2, 128), ([30000, 20000], 1, 1, 256), ([9000] * 40, 8, 3, 96)])
+def test_attention_tokens_over_long_contexts_of_one_sign(q, lens, heads, group, dim):
+    """V of one sign, float32: no longer sums than 32 tokens are left to the tensor cores.  The weights are off by what the scores
+    are: 2^-21 of sum |q k| for q in two pieces, and 2^-22 for the exponential; their error is of both signs and fades in the sum."""
+    qry, cache, pages, ln, _ = setup(q, lens, [1] * len(lens), heads, group, dim, 64, "e4m3", torch.float32, dim, uniform=True)
+    cache.v_codes.bitwise_and_(127)
+    got = q.mx_attention(qry, cache, pages, ln, scale=0.02)
+    off = norm = 0.0
+    for s in range(0, len(lens), max(1, len(lens) // 4)):
+        t = torch.arange(lens[s], device="cuda")
+        slot = pages[s].long()[t // 64]
+        for h in range(heads):
+            k, v = (values(cache[i][slot, h, t % 64], cache[i + 1][slot, h, t % 64], dim) for i in (0, 2))
+            rows = slice(h * group, (h + 1) * group)
+            o = torch.softmax((qry[s, 0, rows].double() @ k.t()) * 0.02, -1) @ v
+            off += (got[s, 0, rows].double() - o).square().sum().item()
+            norm += o.square().sum().item()
+    assert math.sqrt(off / norm) <= cut_off_bound(32, max(lens))
