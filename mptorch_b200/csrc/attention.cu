@@ -8,11 +8,12 @@
 //   s[t, r] = sum_b 2^e[t,b] sum_{d in b} c_k[t,d] q[r,d]        o[d, r] = sum_t c_v[t,d] (2^e[t,b(d)] p[t,r])
 // Codes are exact in binary16, so both inner sums run on m16n8k16 tensor-core products of codes as they are (one conversion per two
 // elements) with fp32 sums: K as the 16 x 16 operand and q^T as the 16 x 8 one, then V^T and p^T.  The scale of K multiplies a
-// block's partial sums; the scale of V multiplies p, relative to the block's largest so far (which moves like the running maximum
-// of the softmax), and that is put back at the end.  q is scaled by a power of two to a largest value in [2^14, 2^15) and held as binary16: bfloat16 and float16 in
-// one piece, exact unless a value is 2^-29 of the row's largest or less; float32 in two columns, the second 2^11 times what the
-// first leaves (22 bits).  p 2^15 is rounded to binary16 (11 bits) in one piece, for float32 in two.  The running maximum is
-// moved only when a tile exceeds it.  The sums of 32 tokens are added up in fp32 registers: the tensor cores cut their running sums off
+// block's partial sums; the scale of V multiplies p, relative to a reference that moves when a scale is above it or more than 2^14 below
+// it; tokens of one piece that are further apart than that are taken in two passes or more, so that neither a large V with a small weight
+// nor one that a row does not see takes bits from the others.  q is scaled by a power of two to a largest value in [2^14, 2^15) and held
+// as binary16: bfloat16 and float16 in one piece, exact unless a value is 2^-29 of the row's largest or less; float32 in two columns, the
+// second 2^11 times what the first leaves (22 bits).  p 2^15 is rounded to binary16 (11 bits) in one piece, for float32 in two.  The
+// running maximum is moved only when a tile exceeds it.  The sums of 32 tokens are added up in fp32 registers: the tensor cores cut their running sums off
 // instead of rounding them, which after 20000 tokens of float32 had come to 3.9e-6 of the result, 1.5e-5 where V has one sign; now
 // 3.8e-7 and 1.4e-7.
 //
@@ -54,9 +55,11 @@ __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_
 __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
     return half2_bits(__hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b)));
 }
-__device__ __forceinline__ uint32_t half_power(int down) {   // 2^-down as binary16, zero below 2^-24
-    return down < 15 ? (uint32_t)(15 - down) << 10 : (down < 25 ? 1u << (24 - down) : 0u);
-}
+// 2^-down as binary16 where down is 0 to kLevel, zero elsewhere
+constexpr int kLevel = 14, kNone = -1 - kLevel;           // kNone: a reference that no exponent is in reach of
+__device__ __forceinline__ uint32_t half_power(int down) { return (unsigned)down <= (unsigned)kLevel ? (uint32_t)(15 - down) << 10 : 0u; }
+// 2^(ref - 127 - 15), the 15 for the weights; nothing is in reach of a negative ref
+__device__ __forceinline__ float sum_power(int ref) { return __uint_as_float(ref > 15 ? (uint32_t)(ref - 15) << 23 : 1u << max(ref + 7, 0)); }
 
 // Bytes of a token in shared memory.  A warp's reads meet no bank twice when eight K rows of four words (E2M1), four K rows of
 // four double words (E4M3) and four V rows two apart fall into different quarters of the banks.
@@ -70,7 +73,7 @@ struct Layout {
         scales = kTok * (k_pitch > v_pitch ? k_pitch : v_pitch);
         half = scales + kTok * nb;             // K or V of 32 tokens
         q_pitch = (nb | 1) * 64;
-        expand = nb * kTok * 4 + kTok / 2 * ((nb + 3) & ~3) * 4 * 2;
+        expand = nb * kTok * 4 + kTok / 2 * ((nb + 3) & ~3) * 4;
     }
 };
 __host__ __device__ __forceinline__ int smem_bytes(int dim, bool fp4, int nt) {
@@ -110,7 +113,6 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_att
     float* k_scale = reinterpret_cast<float*>(ring + 3 * lay.half);                       // [block][token]
     uint32_t* v_scale = reinterpret_cast<uint32_t*>(k_scale + nb * kTok);                       // [pair of tokens][block, of four]
     constexpr int nb4 = (nb + 3) & ~3;
-    uint32_t* v_scale2 = v_scale + kTok / 2 * nb4;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
 
     // ---- the warp's ring
@@ -219,9 +221,9 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_att
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[b][j][n][i] = 0.f;
 
-    int v_top[NB];                            // the exponent that the sums of a block are relative to, the largest so far
+    int v_ref[NB];                            // the exponent that scales of V are taken relative to
 #pragma unroll
-    for (int b = 0; b < NB; ++b) v_top[b] = 0;
+    for (int b = 0; b < NB; ++b) v_ref[b] = kNone;
     // The ring has three places: while K of a tile is used, V of it and K of the warp's next tile are on the way.
     int slot = 0;
     for (int j = j_lo + warp; j < j_hi; j += kWarps) {
@@ -349,62 +351,55 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_att
                 }
                 pw[i >> 1][n][i & 1] = transpose8x8(w);
             }
-        // ---- scales of V: each lane those of its token, relative to the largest so far, as binary16 powers of two
+        // ---- scales of V: each lane those of its token, relative to a reference, as binary16 powers of two
         issue(c.v_codes, c.v_scales, lay.v_pitch, j + kWarps, slot, page_put);
         asm volatile("cp.async.wait_group 2;\n" ::);
         __syncwarp();
-        bool bad = false, higher_v = false;
-        int ev[NB];
+        const bool mine = (there >> lane) & 1u;
+        auto exponent = [&](int b) -> int { return mine ? (int)v_sm[lay.scales + lane * nb + b] : v_ref[b]; };
+        auto zero_block = [&](int b) {
+            uint32_t any = 0u;
+            for (int i = 0; i < (FP4 ? 4 : 8); ++i) any |= reinterpret_cast<const uint32_t*>(v_sm + lane * lay.v_pitch)[b * (FP4 ? 4 : 8) + i];
+            return (any & (FP4 ? 0x77777777u : 0x7F7F7F7Fu)) == 0u;
+        };
+        bool beyond = false;                    // a scale is above its reference or more than 2^kLevel below it
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            ev[b] = ((there >> lane) & 1u) ? v_sm[lay.scales + lane * nb + b] : 0;
-            bad |= ev[b] == 255;
-            higher_v |= ev[b] > v_top[b];
-        }
-        if (__any_sync(0xFFFFFFFFu, higher_v)) {
-            if (__any_sync(0xFFFFFFFFu, bad)) {
-                // a block scale of 0xFF: NaN for the rows that see the token, and nothing for those that do not
-                uint32_t blocks_v = 0u;
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    if (ev[b] == 255) {
-                        blocks_v |= 1u << b;
-                        ev[b] = 0;
-                        for (int i = 0; i < (FP4 ? 4 : 8); ++i) reinterpret_cast<uint32_t*>(v_sm + lane * lay.v_pitch)[b * (FP4 ? 4 : 8) + i] = 0u;
-                    }
-                for (uint32_t some = __ballot_sync(0xFFFFFFFFu, blocks_v != 0u); some; some &= some - 1) {
-                    const int t = __ffs(some) - 1;
-                    const uint32_t blocks = __shfl_sync(0xFFFFFFFFu, blocks_v, t);
-#pragma unroll
-                    for (int r = 0; r < kMine; ++r)
-                        if (sees(p, pos[r], t0 + t)) poison[r] |= blocks;
-                }
-            }
+        for (int b = 0; b < NB; ++b) beyond |= (unsigned)(v_ref[b] - exponent(b)) > (unsigned)kLevel;
+        bool levels = __any_sync(0xFFFFFFFFu, beyond);
+        if (levels) {
+            // a block scale of 0xFF: NaN for the rows that see the token, and nothing for those that do not
+            uint32_t blocks_v = 0u;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
-                {
-                    const int top = max(v_top[b], (int)__reduce_max_sync(0xFFFFFFFFu, (uint32_t)ev[b]));
-                    const float fade = top - v_top[b] > 126 ? 0.f : __uint_as_float((uint32_t)(127 - top + v_top[b]) << 23);
-                    v_top[b] = top;
-#pragma unroll
-                    for (int jj = 0; jj < 2; ++jj)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) o[b][jj][n][i] *= fade;
+                if (exponent(b) == 255) {
+                    blocks_v |= 1u << b;
+                    for (int i = 0; i < (FP4 ? 4 : 8); ++i) reinterpret_cast<uint32_t*>(v_sm + lane * lay.v_pitch)[b * (FP4 ? 4 : 8) + i] = 0u;
                 }
-        }
-        bool far = false;
+            for (uint32_t some = __ballot_sync(0xFFFFFFFFu, blocks_v != 0u); some; some &= some - 1) {
+                const int t = __ffs(some) - 1;
+                const uint32_t blocks = __shfl_sync(0xFFFFFFFFu, blocks_v, t);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            ev[b] = v_top[b] - ev[b];
-            far |= ev[b] > 14 && ((there >> lane) & 1u);
+                for (int r = 0; r < kMine; ++r)
+                    if (sees(p, pos[r], t0 + t)) poison[r] |= blocks;
+            }
+            // new references: the largest so far where all scales are in its reach, else the largest of these
+            levels = false;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const int e = mine && !((blocks_v >> b) & 1u) ? exponent(b) : kNone;
+                const int top = __reduce_max_sync(0xFFFFFFFFu, e);
+                const int low = __reduce_min_sync(0xFFFFFFFFu, e == kNone || (e < top - kLevel && zero_block(b)) ? 255 : e), high = max(v_ref[b], top);
+                v_ref[b] = high - low <= kLevel ? high : top;
+                levels |= low < top - kLevel;
+            }
         }
-        far = __any_sync(0xFFFFFFFFu, far);
+        // Scales too far apart for one set of binary16 factors are taken in levels of 2^kLevel, the largest first: what a row adds up does
+        // not depend on the scales of tokens that it does not see.
+        do {
         uint32_t h[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            h[b] = far ? half_power(min(ev[b], 24)) : (uint32_t)(15 - min(ev[b], 14)) << 10;
+            h[b] = half_power(v_ref[b] - exponent(b));
             h[b] |= __shfl_down_sync(0xFFFFFFFFu, h[b], 1) << 16;              // whole in the even lanes
         }
         if (!(lane & 1)) {
@@ -412,14 +407,6 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_att
             for (int b = 0; b < NB; b += 4)
                 *reinterpret_cast<uint4*>(v_scale + (lane >> 1) * nb4 + b) =
                     make_uint4(h[b], h[b + 1 < NB ? b + 1 : b], h[b + 2 < NB ? b + 2 : b], h[b + 3 < NB ? b + 3 : b]);
-        }
-        if (far) {                              // binary16 has no power below 2^-24: scales further apart take a second factor
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                uint32_t x = half_power(max(ev[b] - 24, 0));
-                x |= __shfl_down_sync(0xFFFFFFFFu, x, 1) << 16;
-                if (!(lane & 1)) v_scale2[(lane >> 1) * nb4 + b] = x;
-            }
         }
         __syncwarp();
 
@@ -437,11 +424,6 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_att
                         const uint32_t sc = v_scale[pair * nb4 + b];
 #pragma unroll
                         for (int n = 0; n < NT; ++n) pb[n][i] = mul_half2(pw[mt][n][i], sc);
-                        if (far) {
-                            const uint32_t sc2 = v_scale2[pair * nb4 + b];
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) pb[n][i] = mul_half2(pb[n][i], sc2);
-                        }
                     }
                     uint32_t a[2][4];                                               // [half of the block's 4 g .. 4 g + 3][register]
                     const uint8_t* row = v_sm + (mt * 16 + 2 * tig) * lay.v_pitch;
@@ -474,14 +456,25 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_att
                         }
                 }
             }
+            const float up = sum_power(v_ref[b]);
 #pragma unroll
             for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[b][jj][n][i] += part[jj][n][i];
+                    for (int i = 0; i < 4; ++i) o[b][jj][n][i] = fmaf(part[jj][n][i], up, o[b][jj][n][i]);
         }
         __syncwarp();
+        if (levels) {
+            levels = false;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const int e = mine ? exponent(b) : 255;
+                v_ref[b] = __reduce_max_sync(0xFFFFFFFFu, e < v_ref[b] - kLevel && !zero_block(b) ? e : kNone);
+                levels |= v_ref[b] != kNone;
+            }
+        }
+        } while (levels);
         slot = slot_k;
         there = __ballot_sync(0xFFFFFFFFu, page_put >= 0);
         page_put = page_of(j + 2 * kWarps);
@@ -507,15 +500,14 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_att
         for (int b = 0; b < NB; ++b)
             {
                 float* to = sums + (warp * kRows + at) * dim + b * 32 + 4 * g;
-                const float up = e8m0_value(v_top[b]);             // after the 2^15 of the weights, so that no large V overflows
 #pragma unroll
                 for (int jj = 0; jj < 2; ++jj) {
                     if (PIECES == 1) {
-                        to[2 * jj] = up * (0x1p-15f * o[b][jj][r >> 1][r & 1]);
-                        to[2 * jj + 1] = up * (0x1p-15f * o[b][jj][r >> 1][2 + (r & 1)]);
+                        to[2 * jj] = o[b][jj][r >> 1][r & 1];
+                        to[2 * jj + 1] = o[b][jj][r >> 1][2 + (r & 1)];
                     } else {
-                        to[2 * jj] = up * (0x1p-15f * fmaf(o[b][jj][r][1], 0x1p-11f, o[b][jj][r][0]));
-                        to[2 * jj + 1] = up * (0x1p-15f * fmaf(o[b][jj][r][3], 0x1p-11f, o[b][jj][r][2]));
+                        to[2 * jj] = fmaf(o[b][jj][r][1], 0x1p-11f, o[b][jj][r][0]);
+                        to[2 * jj + 1] = fmaf(o[b][jj][r][3], 0x1p-11f, o[b][jj][r][2]);
                     }
                 }
             }

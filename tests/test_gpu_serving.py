@@ -725,3 +725,53 @@ def test_attention_tokens_over_long_contexts_of_one_sign(q, lens, heads, group, 
             off += (got[s, 0, rows].double() - o).square().sum().item()
             norm += o.square().sum().item()
     assert math.sqrt(off / norm) <= cut_off_bound(32, max(lens))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("elem", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("new,window,dim,group", [(1, 50, 64, 1), (1, 50, 128, 4), (6, 50, 96, 2), (20, 0, 64, 1), (20, 33, 256, 1), (160, 0, 192, 1), (160, 40, 256, 2)])
+def test_attention_large_values_in_masked_places(q, elem, dtype, new, window, dim, group):
+    """V that a row does not see takes no bits from what it sees, however large it is: the row is as near to 64-bit arithmetic without
+    those tokens as if they were not there.  A weight is held to 2^-26 of the row's largest where V's scales are up to 2^14 apart
+    (binary16 has a step of 2^-24, and weights are scaled by 2^15 before and 2^-14 after), so that of each token's |v| is allowed."""
+    length = new + 200
+    qry, cache, pages, ln, _ = setup(q, [length], [new], 1, group, dim, 16, elem, dtype, 5 + dim, uniform=True)
+    want, tol = reference(qry[0], cache, pages, [length], [new], dim, 1 / math.sqrt(dim), window)
+    t = torch.arange(length, device="cuda")
+    where = (pages[0].long()[t // 16], torch.zeros_like(t), t % 16)
+    v = values(cache.v_codes[where], cache.v_scales[where], dim).abs()
+    hidden = [length - 1] if new > 1 else []                       # by causality from all rows but the last
+    if window:
+        hidden += [length - new - window - 3, length - new - window]    # too old for every row
+    for scale in (140, 200, 246):
+        bad = q.MXCache(*(x.clone() for x in cache))
+        for h in hidden:
+            bad.v_scales[pages[0, h // 16], 0, h % 16] = scale
+        got = q.mx_attention(qry, bad, pages, ln, window=window)
+        rows = slice(0, new - 1 if new > 1 else 1)
+        check_attention(got[0, rows], want[rows], tol[rows] + 2.0 ** -26 * v.sum(0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [1, 12])
+def test_attention_large_values_with_small_weights(q, dtype, new):
+    """Tokens with tiny weights and V from 2^-27 to 2^127, all in one piece of 32 tokens, beside tokens with large weights and small V."""
+    dim, length = 64, new + 70
+    qry, cache, pages, ln, starts = setup(q, [length], [new], 1, 2, dim, 16, "e4m3", dtype, 3)
+    qry.fill_(0.25)
+    cache.k_scales.fill_(127)
+    cache.k_codes.fill_(0xD0)                                      # -8: a score of -16 where it stays
+    for i, t in enumerate((5, 11, 40, 62)):
+        cache.k_codes[pages[0, t // 16], 0, t % 16] = 0x38 if i % 2 else 0x30         # 1 and 1/2
+    g = gen(9)
+    cache.v_scales.copy_(torch.randint(100, 240, cache.v_scales.shape, device="cuda", generator=g, dtype=torch.uint8))
+    scale = 64.0                                                   # the other weights are e^-9216 and less: nothing, whatever V is
+    for t in (5, 11, 40, 62):
+        cache.v_scales[pages[0, t // 16], 0, t % 16] = 107
+    got = q.mx_attention(qry, cache, pages, ln, starts, scale=scale)
+    t = torch.tensor([11, 62], device="cuda")                      # score 1024, the halves 512
+    slot = pages[0].long()[t // 16]
+    v = values(cache.v_codes[slot, 0, t % 16], cache.v_scales[slot, 0, t % 16], dim)
+    want = v.mean(0).expand(got.shape)
+    tol = (2.0 ** -26 + 2.0 ** -20 + half_ulp(dtype)) * v.abs().sum(0) + (2.0 ** -24 if dtype == torch.float16 else 0.0)
+    check_attention(got, want, tol.expand(got.shape))
