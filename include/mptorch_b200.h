@@ -374,7 +374,8 @@ MPT_API int mpt_block_linear(const void *x, const uint8_t *codes, const uint8_t 
 /* A cache of K and V in MX format, in pages: codes [num_pages, heads, page, dim] bytes (E4M3) or
  * [num_pages, heads, page, dim / 2] (E2M1), scales [num_pages, heads, page, dim / 32] E8M0 bytes.  dim is a multiple
  * of 32 up to 256, page a power of two from 8 to 256; codes begin at a multiple of 16 bytes, scales at one of 8.  A code
- * that is a NaN (0x7F, 0xFF) stands only in blocks whose scale is 0xFF, as mpt_mx_cache_write leaves them. */
+ * that is a NaN (0x7F, 0xFF) stands only in blocks whose scale is 0xFF, and a code times its scale does not pass fp32's
+ * range, as mpt_mx_cache_write leaves them (a value that does counts as a large one, and only where it is seen). */
 typedef struct {
     uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
     int64_t num_pages;

@@ -40,6 +40,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 __device__ __forceinline__ float bf16_lo(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t x) { return __uint_as_float(x & 0xFFFF0000u); }
 
+constexpr float kMostBf16 = 0x1.FEp127f;
+
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }   // the lowest n bits
 // ---- expanding.  One CTA for 128 tokens of a (sequence, kv head).
 template <bool FP4>
@@ -94,18 +96,25 @@ __global__ void __launch_bounds__(256) mx_expand_kernel(const AttentionParams p,
                     vs = __ldg(c.v_scales + at * nb + (ch >> 2));
                 }
                 uint8_t* to = out + (ch >> 3) * kPart + tok * 128 + (((ch & 7) ^ (tok & 7)) << 4);
-                auto put = [&](uint2 w, float s, uint8_t* to) {
+                auto put = [&](uint2 w, float s, bool bound, uint8_t* to) {
                     float x[8];
                     decode8<FP4>(w, x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] *= s;
+                    if (bound) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = fminf(fmaxf(x[e], -kMostBf16), kMostBf16);
+                    }
                     uint4 v;
-                    v.x = pack_bf16(x[0] * s, x[1] * s); v.y = pack_bf16(x[2] * s, x[3] * s);
-                    v.z = pack_bf16(x[4] * s, x[5] * s); v.w = pack_bf16(x[6] * s, x[7] * s);
+                    v.x = pack_bf16(x[0], x[1]); v.y = pack_bf16(x[2], x[3]);
+                    v.z = pack_bf16(x[4], x[5]); v.w = pack_bf16(x[6], x[7]);
                     *reinterpret_cast<uint4*>(to) = v;
                 };
-                put(kw, e8m0_value(ks), to);
+                put(kw, e8m0_value(ks), false, to);
                 // a block of V that is NaN takes no part in the product; its rows are told at the end
                 if (vs == 255u) vw = make_uint2(0u, 0u);
-                put(vw, vs == 255u ? 0.f : e8m0_value(vs), to + side_bytes);
+                // (a code of 2^8 or 2^2 with a scale this large passes fp32's range; an infinity would reach rows that do not see the token)
+                put(vw, vs == 255u ? 0.f : e8m0_value(vs), vs >= 247u, to + side_bytes);
             }
         }
         uint32_t* tail = reinterpret_cast<uint32_t*>(out + 2 * parts_for(c.dim) * kPart);

@@ -43,7 +43,7 @@ def nvfp4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, glo
 class MXCache(NamedTuple):
     """K and V of one layer in pages, quantized along head_dim in blocks of 32 (MXFP8 or MXFP4): codes and E8M0 scale bytes of
     each.  The functions below also take a plain tuple of the four tensors.  Codes that are NaN stand in blocks whose scale byte is
-    0xFF, as ``mx_cache_write`` leaves them."""
+    0xFF, and codes times their scales do not pass float32's range, as ``mx_cache_write`` leaves them."""
     k_codes: torch.Tensor
     k_scales: torch.Tensor
     v_codes: torch.Tensor

@@ -775,3 +775,24 @@ def test_attention_large_values_with_small_weights(q, dtype, new):
     want = v.mean(0).expand(got.shape)
     tol = (2.0 ** -26 + 2.0 ** -20 + half_ulp(dtype)) * v.abs().sum(0) + (2.0 ** -24 if dtype == torch.float16 else 0.0)
     check_attention(got, want, tol.expand(got.shape))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("elem", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("new,window", [(1, 0), (20, 0), (20, 25), (200, 0), (200, 64)])
+def test_attention_values_beyond_fp32_in_masked_places(q, elem, dtype, new, window):
+    """Scale bytes up to 254, with codes that take their values out of fp32's range, where a row does not see them."""
+    length, dim = new + 90, 64
+    qry, cache, pages, ln, _ = setup(q, [length], [new], 1, 2, dim, 16, elem, dtype, 12, uniform=True)
+    want, tol = reference(qry[0], cache, pages, [length], [new], dim, 1 / 8, window)
+    bad = q.MXCache(*(x.clone() for x in cache))
+    for h in ([length - 1] if new > 1 else []) + ([length - new - window - 2] if window else []):
+        for scales, codes in ((bad.k_scales, bad.k_codes), (bad.v_scales, bad.v_codes)):
+            scales[pages[0, h // 16], 0, h % 16] = 254
+            codes[pages[0, h // 16], 0, h % 16] = 0x7E if elem == "e4m3" else 0x77
+    got = q.mx_attention(qry, bad, pages, ln, window=window)
+    rows = slice(0, new - 1 if new > 1 else 1)
+    t = torch.arange(length, device="cuda")
+    where = (pages[0].long()[t // 16], torch.zeros_like(t), t % 16)
+    v = values(cache.v_codes[where], cache.v_scales[where], dim).abs()
+    check_attention(got[0, rows], want[rows], tol[rows] + 2.0 ** -26 * v.sum(0))      # as above
