@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_att
                 x[b] = load_value(p.q, p.dtype, off + (head * p.group + rr - i * p.group) * p.q_head + b * 32 + lane);
                 const float a = fabsf(x[b]);
                 if (a < INFINITY) top = fmaxf(top, a);
+                else x[b] = __uint_as_float(0x7FC00000u);      // an infinity gives scores of infinities and NaN alone: the row is NaN
             }
         }
         const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top));
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_by_registers(NB, NT)) mx_att
                 *to = hi;
                 if (PIECES == 2) {
                     const float left = (v - __half2float(hi)) * 2048.f;
-                    to[lay.q_pitch / 2] = fabsf(v) < INFINITY ? __float2half_rn(left) : __float2half_rn(0.f);
+                    to[lay.q_pitch / 2] = __float2half_rn(left);
                 }
             }
         }

@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
                 else load8(static_cast<const __nv_bfloat16*>(p.q) + off, p.q_vec, x);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= sign;
+            for (int e = 0; e < 8; ++e) x[e] = fabsf(x[e]) < INFINITY ? x[e] * sign : __uint_as_float(0x7FC00000u);      // (an infinity: the row is NaN)
 #pragma unroll
             for (int k = 0; k < PIECES; ++k) {
                 uint32_t w[4];

@@ -796,3 +796,27 @@ def test_attention_values_beyond_fp32_in_masked_places(q, elem, dtype, new, wind
     where = (pages[0].long()[t // 16], torch.zeros_like(t), t % 16)
     v = values(cache.v_codes[where], cache.v_scales[where], dim).abs()
     check_attention(got[0, rows], want[rows], tol[rows] + 2.0 ** -26 * v.sum(0))      # as above
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [1, 40, 200])
+@pytest.mark.parametrize("x", [math.inf, -math.inf, math.nan])
+def test_attention_infinite_rows_of_q(q, dtype, new, x):
+    """Scores that are all minus infinity are no empty row: their softmax is NaN, as that of plus infinity.  A row that sees nothing
+    gives zeros, whatever it holds."""
+    qry, cache, pages, ln, _ = setup(q, [new], [new], 1, 2, 64, 16, "e4m3", dtype, 5, uniform=True)
+    clean = q.mx_attention(qry, cache, pages, ln)
+    cache.k_codes[pages[0, 0], 0, 0] = 0x38                        # the first token's K: ones
+    cache.k_scales[pages[0, 0], 0, 0] = 127
+    same = q.mx_attention(qry, cache, pages, ln)
+    for where in (slice(None), 3):                                 # every element, or one beside finite ones
+        bad = qry.clone()
+        bad[0, 0, 0, where] = x
+        bad[0, -1, 1, where] = x
+        got = q.mx_attention(bad, cache, pages, ln)
+        assert got[0, 0, 0].isnan().all() and got[0, -1, 1].isnan().all()
+        got[0, 0, 0], got[0, -1, 1] = same[0, 0, 0], same[0, -1, 1]
+        assert torch.equal(got, same)
+    assert clean.isfinite().all()
+    bad = torch.full_like(qry, x)
+    assert not q.mx_attention(bad, cache, torch.full_like(pages, -1), ln).any()
