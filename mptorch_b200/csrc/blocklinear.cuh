@@ -43,7 +43,7 @@ __device__ __forceinline__ void read8(const void* p, int dtype, bool vec, int64_
 struct TilesPlan {
     int cols, pieces, row_tiles, col_tiles, k_blocks, k_supers, runs, ring_blocks, w_stages, x_stages, columns, fold;
     int64_t units, per;
-    size_t image_bytes, partial_bytes, kept_bytes, bytes;
+    size_t image_bytes, partial_bytes, kept_bytes, far_bytes, bytes;
 };
 TilesPlan tiles_plan(int64_t rows, int64_t n_out, int64_t n_in, int format, int dtype);
 int launch_tiles(const LinearParams& p, const TilesPlan& pl, int format, uint8_t* workspace, cudaStream_t st);

@@ -9,7 +9,8 @@
 //      copies x's tiles, a warp issues products, and sixteen warps turn codes into binary16 weights in shared memory, four blocks of
 //      64 at a time (a warp then reads 128 bytes of each of four rows), two pieces ahead in registers: one conversion and one
 //      multiplication for two weights.  NVFP4: a code times its E4M3 scale is exact (six bits).  MXFP4: a code times
-//      2^(13 + e - E), E the row's largest exponent, is exact down to e = E - 36; smaller blocks count less than 2^-36 of the largest.
+//      2^(13 + e - E), E the row's largest exponent, is exact down to e = E - 36; rows with smaller blocks that are not all zeros are
+//      found here and computed by a kernel at the end, in fp32 (rare, and slow: 1024 x 4096 by 4096 takes 120 us without, 197 with 40 such rows, 6.6 ms with nothing else).
 //      Sums are fp32 in tensor memory, those of float32's second pieces apart, and the powers of two are put back at the end.
 //   3. A tile that a run ends in is left in parts, which are added up in order.
 //
@@ -48,6 +49,7 @@ struct TilesParams {
     float* partial;                    // of tiles that are cut: [slot][column][128]
     int fold;                          // pieces after which sums are added up in memory and begun again
     float* kept;                       // there: [run][column][128]
+    uint8_t* far_rows;                 // MXFP4: 1 for the rows of W that linear_far_kernel computes
 };
 
 // ---- x into tiles: a CTA for a row
@@ -92,21 +94,39 @@ __global__ void __launch_bounds__(256) linear_split_kernel(const TilesParams p, 
 // fp32 sums of binary16 products, M = 128
 __device__ __forceinline__ uint32_t half_product_descriptor(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | (8u << 24); }
 
-// 2^(13 - d) as binary16, zero below 2^-24
-__device__ __forceinline__ uint32_t half_weight_power(int d) { return d <= 27 ? (uint32_t)(28 - d) << 10 : d <= 37 ? 1u << (37 - d) : 0u; }
+// 2^(13 - d) as binary16, zero where its half, the smallest code's, is below 2^-24
+constexpr int kReach = 36;
+__device__ __forceinline__ uint32_t half_weight_power(int d) { return d <= 27 ? (uint32_t)(28 - d) << 10 : d <= kReach ? 1u << (37 - d) : 0u; }
 
 constexpr int kMaxStages = 12;                                      // of W's ring; x's has at most eight
 
-// MXFP4: the largest exponent of row n of W, found by the eight lanes c of a row (255 is a NaN and no exponent); bytes up to an aligned
-// word, then words.
+// MXFP4: whether row n of W has blocks that are out of its largest exponent's reach and not all zeros
+__device__ __noinline__ bool far_blocks(const LinearParams& l, int n, int c, int top, int low) {
+    const int groups = l.n_in / 32;
+    bool far = false;
+    if (top - low > kReach)
+        for (int k = c; k < groups; k += 8)
+            if (top - (int)__ldg(l.scales + (int64_t)n * groups + k) > kReach) {
+                const uint4 w = __ldg(reinterpret_cast<const uint4*>(l.codes + (int64_t)n * (l.n_in >> 1)) + k);
+                far |= ((w.x | w.y | w.z | w.w) & 0x77777777u) != 0u;
+            }
+    const unsigned some = __ballot_sync(0xFFFFFFFFu, far);         // the lanes of a row are four apart
+    return ((some >> (threadIdx.x & 3)) & 0x11111111u) != 0u;
+}
+
+// MXFP4: the largest exponent of row n of W, found by the eight lanes c of a row (255 is a NaN and no exponent), and whether the row is
+// left to linear_far_kernel; bytes up to an aligned word, then words.
 template <bool NV>
 __device__ __forceinline__ int row_top(const TilesParams& p, int n, int c) {
     if (NV) return 0;
-    int top = 0;
+    int top = 0, low = 255;
     const int groups = p.l.n_in / 32;
     if (n < p.l.n_out) {
         const uint8_t* sc = p.l.scales + (int64_t)n * groups;
-        auto take = [&](uint32_t e) { top = max(top, e == 255u ? 0 : (int)e); };
+        auto take = [&](uint32_t e) {
+            top = max(top, e == 255u ? 0 : (int)e);
+            low = min(low, (int)e);
+        };
         const int head = min((int)((4 - (reinterpret_cast<uintptr_t>(sc) & 3)) & 3), groups), words = (groups - head) >> 2;
         if (c < head) take(__ldg(sc + c));
         const uint32_t* from = reinterpret_cast<const uint32_t*>(sc + head);
@@ -118,7 +138,12 @@ __device__ __forceinline__ int row_top(const TilesParams& p, int n, int c) {
         if (head + 4 * words + c < groups) take(__ldg(sc + head + 4 * words + c));
     }
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    for (int o = 4; o < 32; o <<= 1) {
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        low = min(low, __shfl_xor_sync(0xFFFFFFFFu, low, o));
+    }
+    const bool far = __any_sync(0xFFFFFFFFu, top - low > kReach) && far_blocks(p.l, n, c, top, low);
+    if (c == 0 && n < p.l.n_out) p.far_rows[n] = far;
     return top;
 }
 
@@ -420,8 +445,68 @@ __global__ void __launch_bounds__(kThreads) linear_tiles_kernel(const __grid_con
     if (warp == kWorkers / 32 + 1) tmem_free(tmem, p.columns);
 }
 
+// MXFP4: the rows of W that are marked, in fp32.  CTAs (x, .) look at rows 4096 x and on and share what there is to do: four rows of x for
+// each warp and row of W at a time.
+constexpr int kFarRows = 4096, kFarCols = 4;
+__global__ void __launch_bounds__(256) linear_far_kernel(const TilesParams p) {
+    const LinearParams& l = p.l;
+    __shared__ uint16_t rows[kFarRows];                            // in order, so that all CTAs count alike
+    __shared__ int of_warp[8];
+    const int lane = threadIdx.x & 31, groups = l.n_in / 32, n0 = blockIdx.x * kFarRows, mine = n0 + 16 * threadIdx.x;
+    wait_for_previous();
+    uint32_t f[4] = {}, marked = 0u;
+    if (mine < l.n_out) *reinterpret_cast<uint4*>(f) = *reinterpret_cast<const uint4*>(p.far_rows + mine);       // (the marks end at a multiple of 16 bytes)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) marked |= mine + i < l.n_out && (f[i >> 2] >> (8 * (i & 3)) & 1u) ? 1u << i : 0u;
+    int upto = __popc(marked);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) of_warp[threadIdx.x >> 5] = upto;
+    if (!__syncthreads_or(marked != 0u)) return;
+    int count = 0, at = upto - __popc(marked);
+    for (int w = 0; w < 8; ++w) {
+        if (w < (int)(threadIdx.x >> 5)) at += of_warp[w];
+        count += of_warp[w];
+    }
+    for (; marked; marked &= marked - 1) rows[at++] = (uint16_t)(16 * threadIdx.x + __ffs(marked) - 1);
+    __syncthreads();
+    const int each = (l.rows + 8 * kFarCols - 1) / (8 * kFarCols);
+    for (int64_t item = blockIdx.y; item < (int64_t)count * each; item += gridDim.y) {
+        const int64_t n = n0 + rows[item / each];
+        const int m0 = ((int)(item % each) * 8 + (threadIdx.x >> 5)) * kFarCols;
+        if (m0 >= l.rows) continue;
+        const uint8_t *codes = l.codes + n * (l.n_in >> 1), *scales = l.scales + n * groups;
+        const float bias = l.bias != nullptr ? read_value(l.bias, l.dtype, n) : 0.f;
+        float sum[kFarCols] = {};
+        for (int k = lane; k < l.n_in / 8; k += 32) {
+            float w[8], x[kFarCols][8];
+            decode8<true>(make_uint2(__ldg(reinterpret_cast<const uint32_t*>(codes) + k), 0u), w);
+            const float scale = e8m0_value(__ldg(scales + (k >> 2)));
+#pragma unroll
+            for (int j = 0; j < kFarCols; ++j) read8(l.x, l.dtype, l.x_vec, (int64_t)min(m0 + j, l.rows - 1) * l.n_in + 8 * (int64_t)k, x[j]);
+#pragma unroll
+            for (int j = 0; j < kFarCols; ++j) {
+                float here = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) here = fmaf(w[i], x[j][i], here);
+                sum[j] = fmaf(here, scale, sum[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kFarCols; ++j) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum[j] += __shfl_xor_sync(0xFFFFFFFFu, sum[j], o);
+            if (lane == 0 && m0 + j < l.rows) write_value(l.y, l.dtype, (m0 + j) * (int64_t)l.n_out + n, sum[j] + bias);
+        }
+    }
+}
+
 // Adds up the tiles that runs end in: CTAs (x, .) look at the end of run x.
 __global__ void __launch_bounds__(256) linear_join_kernel(const TilesParams p) {
+    next_may_start();
     const LinearParams& l = p.l;
     const int64_t cut = (blockIdx.x + 1) * p.per;
     wait_for_previous();
@@ -476,7 +561,8 @@ TilesPlan tiles_plan(int64_t rows, int64_t n_out, int64_t n_in, int format, int 
     const int fold = format == MPT_BLOCK_NVFP4 ? kFoldNv : kFoldMx;
     pl.fold = pl.pieces == 2 && pl.k_supers > fold ? fold : pl.k_supers;
     pl.kept_bytes = pl.fold < pl.k_supers ? (size_t)pl.runs * pl.cols * kRowsW * 4 : 0;
-    pl.bytes = pl.image_bytes + ((size_t)rows * 4 + 255) / 256 * 256 + pl.partial_bytes + pl.kept_bytes;
+    pl.far_bytes = format == MPT_BLOCK_MXFP4 ? ((size_t)n_out + 15) / 16 * 16 : 0;
+    pl.bytes = pl.image_bytes + ((size_t)rows * 4 + 255) / 256 * 256 + pl.partial_bytes + pl.kept_bytes + pl.far_bytes;
     return pl;
 }
 
@@ -489,6 +575,7 @@ int launch_tiles(const LinearParams& l, const TilesPlan& pl, int format, uint8_t
     p.partial = reinterpret_cast<float*>(workspace + pl.image_bytes + ((size_t)l.rows * 4 + 255) / 256 * 256);
     p.fold = pl.fold;
     p.kept = p.partial + pl.partial_bytes / 4;
+    p.far_rows = pl.far_bytes ? reinterpret_cast<uint8_t*>(p.kept) + pl.kept_bytes : nullptr;
     linear_split_kernel<<<(unsigned)l.rows, 256, 0, st>>>(p, workspace);
     const int bytes = 1024 + pl.ring_blocks * (pl.w_stages * kPartW + pl.x_stages * pl.pieces * pl.cols * 128);
     const bool nv = format == MPT_BLOCK_NVFP4, single = pl.ring_blocks == 1;
@@ -513,6 +600,10 @@ int launch_tiles(const LinearParams& l, const TilesPlan& pl, int format, uint8_t
         return MPT_ERR_CUDA;
     }
     if (pl.partial_bytes) launch_after(linear_join_kernel, dim3((unsigned)(pl.runs - 1), 4), dim3(256), 0, st, p);
+    if (pl.far_bytes) {
+        const int groups = (int)(((int64_t)l.n_out + kFarRows - 1) / kFarRows), parts = 2 * sm_count() / groups;
+        launch_after(linear_far_kernel, dim3((unsigned)groups, (unsigned)(parts < 1 ? 1 : parts)), dim3(256), 0, st, p);
+    }
     return check_launch("block_linear");
 }
 

@@ -820,3 +820,38 @@ def test_attention_infinite_rows_of_q(q, dtype, new, x):
     assert clean.isfinite().all()
     bad = torch.full_like(qry, x)
     assert not q.mx_attention(bad, cache, torch.full_like(pages, -1), ln).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,k", [(1, 70, 96), (5, 70, 1120), (24, 300, 1024), (33, 1000, 2080), (40, 129, 6400), (200, 4000, 512), (300, 20000, 96)])
+def test_linear_blocks_of_very_different_size(q, dtype, rows, n, k):
+    """MXFP4 blocks far below their row's largest count in full, whatever the number of rows: x that is zero where the large ones are
+    reads them out exactly, and together with others sums keep the bound of `test_linear`."""
+    g = gen(rows + n + k)
+    codes, scales, _, _ = pack(n, k, "mxfp4", g)
+    some = torch.rand(n, 1, device="cuda", generator=g) < 0.3                     # rows with such blocks
+    at = torch.randint(0, 2, scales.shape, device="cuda", generator=g).bool() & some
+    at[:, 0], at[:, 1] = False, some[:, 0]
+    low = (scales.int() - torch.randint(33, 100, scales.shape, device="cuda", generator=g)).clamp(min=0).to(torch.uint8)
+    scales = torch.where(at, low, scales)
+    zero = torch.rand(n, k // 32, device="cuda", generator=g) < 0.05               # and blocks of zeros, whose scale is the smallest
+    scales = torch.where(zero, 0, scales).to(torch.uint8)
+    codes = torch.where(zero.repeat_interleave(16, -1), 0, codes).to(torch.uint8)
+    v = torch.stack([field_value(codes & 15, 2, 1), field_value(codes >> 4, 2, 1)], -1).flatten(-2)
+    w = v * e8m0_value(scales).repeat_interleave(32, -1)
+    x = torch.randn(rows, k, device="cuda", generator=g).to(dtype)
+    bias = torch.randn(n, device="cuda", generator=g).to(dtype)
+    check_linear(q.mx_linear(x, codes, scales, bias), x, w, bias)
+    far = x.clone()
+    far[:, :32] = 0
+    far[:, 64:] = 0                                                               # the second block alone
+    y = q.mx_linear(far, codes, scales)
+    want, mag = far.double() @ w.t(), far.double().abs() @ w.abs().t()
+    # float16 results have a step of 2^-24 at the least, float32 and bfloat16 sums one of 2^-149
+    low = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -133 if dtype == torch.bfloat16 else 2.0 ** -148
+    assert ((y.double() - want).abs() <= (2.0 ** -21 + 36 * 2.0 ** -24) * mag + half_ulp(dtype) * want.abs() + low).all()
+    unit = torch.zeros(rows, k, device="cuda", dtype=torch.float32)
+    unit[:, 40] = 1
+    assert torch.equal(q.mx_linear(unit, codes, scales).double(), w[:, 40].expand(rows, n))
+    part = q.mx_linear(x, codes[17:60], scales[17:60], bias[17:60])
+    check_linear(part, x, w[17:60], bias[17:60])
