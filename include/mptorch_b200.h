@@ -411,6 +411,9 @@ MPT_API size_t mpt_mx_attention_workspace_bytes(const mpt_mx_cache *cache, const
 MPT_API int mpt_mx_attention(const mpt_mx_cache *cache, const mpt_mx_batch *batch, const void *q, int dtype,
                              const int64_t *q_strides, int q_heads, float scale, int window, int sinks, void *out,
                              int zero_tail, void *workspace, size_t workspace_bytes, void *stream);
+/* For tests of what happens when a wait inside the attention of chunks runs out (the rows concerned become NaN): in later calls one
+ * is taken to have done so at the given part of each CTA's work.  -1, the state at the start: none. */
+MPT_API void mpt_test_attention_wait_runs_out(int part);
 
 /* ---- quantized optimizer steps and tensor scaling -----------------------------------------------------
  * One launch updates many tensors in place (up to 40 per launch; more are split over launches).  The

@@ -116,6 +116,7 @@ def lib() -> C.CDLL:
             fn.restype = i32
             fn.argtypes = args
         L.mpt_block_linear_workspace_bytes.argtypes, L.mpt_block_linear_workspace_bytes.restype = [i64, i64, i64, i32, i32], sz
+        L.mpt_test_attention_wait_runs_out.argtypes, L.mpt_test_attention_wait_runs_out.restype = [i32], None
         L.mpt_mx_attention_workspace_bytes.argtypes, L.mpt_mx_attention_workspace_bytes.restype = [p, p, i32, i32, i32, i32], sz
         _lib = L
     return _lib

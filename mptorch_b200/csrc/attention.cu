@@ -644,7 +644,13 @@ int launch_rows(const AttentionParams& p, const Plan& pl, cudaStream_t st) {
 
 using namespace mpt;
 
+namespace {
+std::atomic<int> fail_at{-1};
+}
+
 extern "C" {
+
+void mpt_test_attention_wait_runs_out(int part) { fail_at.store(part, std::memory_order_relaxed); }
 
 size_t mpt_mx_attention_workspace_bytes(const mpt_mx_cache* cache, const mpt_mx_batch* batch, int q_heads, int dtype, int window, int sinks) {
     CacheView c;
@@ -678,6 +684,7 @@ int mpt_mx_attention(const mpt_mx_cache* cache, const mpt_mx_batch* batch, const
     p.window = window < (1 << 30) ? window : 1 << 30;          // so that no position leaves 32 bits
     p.sinks = sinks < (1 << 30) ? sinks : 1 << 30;
     p.out = out; p.zero_tail = zero_tail;
+    p.fail_at = fail_at.load(std::memory_order_relaxed);
     cudaStream_t st = as_stream(stream);
     const bool fp4 = cache->elem_format == MPT_ELEM_E2M1;
     uint8_t* ws = static_cast<uint8_t*>(workspace);

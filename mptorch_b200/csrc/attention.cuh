@@ -21,6 +21,7 @@ struct AttentionParams {
     int whole;                         // row tiles of at most so many pieces are not cut
     float *partial, *stats;            // of row tiles that two or more CTAs share: sums [slot, row, dim], and {maximum, sum} of each row
     struct Cut* cuts;                  // for each run, the row tile that it has the first but not the last pieces of
+    int fail_at;                       // chunks: the part of a run at which a wait is taken to have run out (-1: none; tests alone set it)
 };
 
 // A row tile that runs `run` to `last` share: the first one's slot, and two for each of the others, of which they use the first.

@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(256) mx_expand_kernel(const AttentionParams p,
 
 // ---- attention
 constexpr int kRowThreads = 256, kThreads = kRowThreads + 64;     // two threads a row, each with half of the tokens; a warp that copies, one that issues products
-enum { kKFull, kKEmpty, kVFull, kVEmpty, kScores, kScores2, kWeights, kWeights2, kValues, kValues2, kBars };
+enum { kKFull, kKEmpty, kVFull, kVEmpty, kScores, kScores2, kWeights, kWeights2, kValues, kValues2, kLast, kBars };
 
 template <int DIM, int PIECES, int NS>
 struct ChunkShape {
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
     auto wait_values = [&](uint32_t it) { return wait(values_bar(it), NS == 2 ? it >> 1 : it); };
     if (threadIdx.x == 0) {
         for (int i = 0; i < kBars; ++i) bar_init(bar(i), i == kWeights || i == kWeights2 ? kRowThreads : 1);
-        failed = 0u;
+        failed = p.fail_at == 0;
         fence_barrier_init();
     }
     if (warp == 9) tmem_alloc(smem_at(&tmem_slot), Shape::columns);
@@ -183,8 +183,11 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
 
     const float sign = p.scale_log2 > 0.f ? 1.f : p.scale_log2 < 0.f ? -1.f : 0.f;      // of q, so that the largest score is of the largest sum
     const float mul = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
-    uint32_t it0 = 0;                                             // pieces before this segment
-    while (run.left > 0) {
+    uint32_t it0 = 0, k_copies = 0, v_copies = 0;                 // pieces before this segment; copies begun (by the thread that copies)
+    for (int segment = 0; run.left > 0; ++segment) {
+        // Once a wait has run out nothing more is computed: all that is left of the run gives NaN, whole row tiles and shares alike.  (Read
+        // between two barriers: no wait is under way here.)
+        const bool dead = *(volatile uint32_t*)&failed != 0u;
         const int seq = run.at.seq, head = run.at.head, pieces = run.at.w.pieces(run.at.tile), take = run.take(p, pieces);
         if (take == 0) break;
         const int2 own = rows_of(c, seq);
@@ -193,11 +196,11 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
         const int low_pos = pos0 + first / p.group, high_pos = pos0 + (first + count - 1) / p.group;
         const TokenTiles<kTile> tt(p, low_pos, high_pos);
         const bool finished = take == pieces;
-        const int j_lo = min(run.at.piece, tt.tiles), n = min(run.at.piece + take, tt.tiles) - j_lo;
+        const int j_lo = min(run.at.piece, tt.tiles), n = dead ? 0 : min(run.at.piece + take, tt.tiles) - j_lo;
 
         // ---- q, in pieces
 #pragma unroll 1
-        for (int i = threadIdx.x; i < kTile * (DIM / 8); i += kThreads) {
+        for (int i = dead ? kTile * (DIM / 8) : threadIdx.x; i < kTile * (DIM / 8); i += kThreads) {
             const int r = i / (DIM / 8), ch = i - r * (DIM / 8);
             float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             if (r < count) {
@@ -236,10 +239,12 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
                     const uint32_t it = it0 + i;
                     const uint8_t* src = from + (int64_t)(tt.start(j_lo + i) / kTile) * tile_bytes(DIM);
                     if (it > 0 && !wait(kKEmpty, it - 1)) break;
+                    ++k_copies;
                     bar_expect(bar(kKFull), Shape::side + kTrailer);
                     bulk_load(k_at, src, Shape::side, bar(kKFull));
                     bulk_load(tail_at + (it & 3) * kTrailer, src + 2 * Shape::side, kTrailer, bar(kKFull));
                     if (it > 0 && !wait(kVEmpty, it - 1)) break;
+                    ++v_copies;
                     bar_expect(bar(kVFull), Shape::side);
                     bulk_load(v_at, src + Shape::side, Shape::side, bar(kVFull));
                 }
@@ -427,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
             const int rr = first + r, tok = rr / p.group;
             const int64_t out_row = ((int64_t)(own.x + tok) * p.q_heads + head * p.group + rr - tok * p.group) * DIM;
             const int share = 2 * blockIdx.x + (run.begins ? 0 : 1);
-            const float times = !ok ? __uint_as_float(0x7FC00000u) : finished ? (l == 0.f ? 0.f : __frcp_rn(l)) : 1.f;
+            const float times = finished ? (l == 0.f ? 0.f : __frcp_rn(l)) : 1.f;
 #pragma unroll(PIECES == 3 ? kTotal : 1)
             for (int b = 16 * half, j = 0; j < DIM / 32; b += 32, ++j) {      // the halves take blocks of 16 columns in turn
                 uint32_t o[16];
@@ -446,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
                     for (int k = 0; k < 16; k += 8) {
                         float v[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = bad ? __uint_as_float(0x7FC00000u) : n > 0 ? __uint_as_float(o[k + e]) * times : 0.f;
+                        for (int e = 0; e < 8; ++e) v[e] = bad || !ok ? __uint_as_float(0x7FC00000u) : n > 0 ? __uint_as_float(o[k + e]) * times : 0.f;
                         if (!finished) {
                             store8(p.partial + ((int64_t)share * kTile + r) * DIM + b + k, v);
                         } else if (p.out_vec) {
@@ -467,17 +472,24 @@ __global__ void __launch_bounds__(kThreads, NS == 1 && PIECES == 1 ? 2 : 1) mx_a
             }
             tmem_fence_before();
         }
+        if (threadIdx.x == 0 && segment + 1 == p.fail_at) failed = 1u;
         __syncthreads();
         tmem_fence_after();
-        if (failed) break;
         it0 += n;
         run.advance(p, take, pieces);
     }
     run.end(p);
-    if (failed && warp == 8 && lane == 0) {                       // copies on the way write to this CTA's memory
-        failed = 0u;
-        wait(kKFull, 0); wait(kKFull, 1);
-        wait(kVFull, 0); wait(kVFull, 1);
+    if (*(volatile uint32_t*)&failed) {                           // copies and products on the way use this CTA's memory
+        __syncthreads();
+        if (threadIdx.x == 0) failed = 0u;
+        __syncthreads();
+        if (warp == 8 && lane == 0) {
+            if (k_copies) wait(kKFull, k_copies - 1);
+            if (v_copies) wait(kVFull, v_copies - 1);
+        } else if (warp == 9) {
+            mma_commit(bar(kLast), lane == 0);
+            wait(kLast, 0);
+        }
     }
     __syncthreads();
     if (warp == 9) tmem_free(tmem, Shape::columns);

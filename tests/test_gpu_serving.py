@@ -855,3 +855,29 @@ def test_linear_blocks_of_very_different_size(q, dtype, rows, n, k):
     assert torch.equal(q.mx_linear(unit, codes, scales).double(), w[:, 40].expand(rows, n))
     part = q.mx_linear(x, codes[17:60], scales[17:60], bias[17:60])
     check_linear(part, x, w[17:60], bias[17:60])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,group", [(64, 1), (128, 4)])
+def test_attention_chunks_after_a_wait_that_ran_out(q, dtype, dim, group):
+    """Nothing is left unwritten or joined from old shares: what was computed before is right, all else is NaN.  (The library is told
+    that a wait ran out; none does.)"""
+    from mptorch_b200 import _cabi
+
+    lens, new = [2000, 1000, 333, 2600, 150], [250, 300, 100, 129, 1]
+    qry, cache, pages, ln, starts = setup(q, lens, new, 8, group, dim, 16, "e4m3", dtype, dim)
+    clean = q.mx_attention(qry, cache, pages, ln, starts)
+    assert clean.isfinite().all()
+    held = []
+    try:
+        for part in (0, 1, 2):
+            _cabi.lib().mpt_test_attention_wait_runs_out(part)
+            out = torch.full_like(qry, 7)
+            q.mx_attention(qry, cache, pages, ln, starts, out=out)
+            row_nan = out.isnan().all(-1)
+            assert torch.equal(row_nan, out.isnan().any(-1)) and torch.equal(out[~row_nan], clean[~row_nan])
+            held.append(int((~row_nan).sum()))
+    finally:
+        _cabi.lib().mpt_test_attention_wait_runs_out(-1)
+    assert held[0] == 0 and held[0] <= held[1] <= held[2]
+    assert torch.equal(q.mx_attention(qry, cache, pages, ln, starts), clean)
