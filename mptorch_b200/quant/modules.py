@@ -225,6 +225,15 @@ class QPackedLinear(nn.Module):
     def from_linear(cls, linear: nn.Linear, fmt: str = "mxfp4") -> "QPackedLinear":
         return cls(linear.weight, linear.bias, fmt)
 
+    def _apply(self, fn, recurse=True):
+        """Conversions of a model (``half``, ``bfloat16``, ``to``) change its dense tensors' type; the tensor scale belongs to the packed
+        weight and stays the float32 value that it is."""
+        scale = self.global_scale
+        super()._apply(fn, recurse)
+        if scale is not None and self.global_scale.dtype != scale.dtype:
+            self.global_scale = scale.to(self.global_scale.device)
+        return self
+
     def extra_repr(self) -> str:
         return "in_features=%d, out_features=%d, bias=%s, fmt=%s" % (self.in_features, self.out_features, self.bias is not None, self.fmt)
 

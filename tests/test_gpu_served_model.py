@@ -104,3 +104,25 @@ def test_generate_and_packed_layer(model):
         q.QPackedLinear(torch.zeros(4, 40, device="cuda"))
     with pytest.raises(ValueError, match="fmt"):
         q.QPackedLinear(torch.zeros(4, 64, device="cuda"), fmt="fp8")
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("convert", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.to(torch.bfloat16), lambda m: m.to("cpu", torch.half).cuda(),
+                                     lambda m: m.half().float()])
+def test_packed_layer_after_conversions(fmt, convert):
+    """A model's dense tensors change their type; what a packed weight stands for does not."""
+    torch.manual_seed(2)
+    lin = torch.nn.Linear(96, 40).cuda()
+    plain = q.QPackedLinear.from_linear(lin, fmt)
+    model = torch.nn.Sequential(q.QPackedLinear.from_linear(lin, fmt))
+    assert convert(model) is model
+    layer = model[0]
+    x = torch.randn(5, 96, device="cuda")
+    for dtype in (torch.float32, torch.bfloat16, torch.half):
+        want = plain(x.to(dtype)) - plain.bias.to(dtype) + layer.bias.to(dtype)    # the bias is a dense tensor
+        got = model(x.to(dtype))
+        # three roundings to the type against one of a sum that cancels
+        assert got.dtype == dtype and ((got.double() - want.double()).abs() <= 4 * torch.finfo(dtype).eps * (plain(x.to(dtype)).double().abs() + plain.bias.double().abs())).all()
+    if fmt == "nvfp4":
+        assert layer.global_scale.dtype == torch.float32 and torch.equal(layer.global_scale, plain.global_scale)
+    assert torch.equal(layer.codes, plain.codes) and torch.equal(layer.scales, plain.scales)
