@@ -765,6 +765,8 @@ def _dense_type(who, x):
 def _no_gradient(who, *tensors):
     if any(t.requires_grad for t in tensors) and torch.is_grad_enabled():
         raise RuntimeError("%s: has no backward pass; call it under torch.no_grad()" % who)
+    if any(torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("%s: has no forward-mode derivative" % who)
 
 
 def _whole(who, what, t, dtype, shape):
@@ -800,7 +802,7 @@ def _block_linear(who, x, codes, scales, global_scale, bias, fmt):
         raise RuntimeError("%s: bias must be [%d] of x's type" % (who, n_out))
     if global_scale is not None and (global_scale.dtype != torch.float32 or global_scale.numel() != 1):
         raise RuntimeError("%s: global_scale must be one float32 value" % who)
-    _no_gradient(who, x, *([bias] if bias is not None else []))
+    _no_gradient(who, *(t for t in (x, bias, global_scale) if t is not None))
     _on_device(who, x, codes=codes, scales=scales, bias=bias, global_scale=global_scale)
     with torch.cuda.device(x.device):
         x, bias = x.contiguous(), None if bias is None else bias.contiguous()

@@ -3,7 +3,8 @@ MX format, and attention over it.
 
 These are the operators that read the codes which ``mx_quantize`` and ``nvfp4_quantize`` hand out.  Dense tensors are float32,
 bfloat16 or float16; sums, softmax statistics and scales are held in 32 bits and a result is rounded to its type once.  They
-answer with a model and do not train it: an input that needs a gradient is refused while gradients are recorded.
+answer with a model and do not train it: an input that needs a gradient is refused while gradients are recorded, and so is one
+that carries a forward-mode tangent.
 
 The tokens of a batch.  ``pages`` [sequences, width] names for each sequence the pages that hold its tokens, in order (an entry
 outside the cache holds none: -1 behind the last page); ``lens`` [sequences] counts a sequence's tokens with the new ones.  New

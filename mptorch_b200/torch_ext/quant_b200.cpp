@@ -425,6 +425,7 @@ int dense_type(const char* who, const at::Tensor& x) {
 }
 void no_gradient(const char* who, const at::Tensor& x) {
     TORCH_CHECK(!(x.requires_grad() && at::GradMode::is_enabled()), who, ": has no backward pass; call it under torch.no_grad()");
+    TORCH_CHECK(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && x._fw_grad(0).defined()), who, ": has no forward-mode derivative");
 }
 void bytes_tensor(const char* who, const char* what, const at::Tensor& t, int64_t dim) {
     TORCH_CHECK(t.scalar_type() == at::kByte && t.dim() == dim && t.is_contiguous(), who, ": ", what, " must be a contiguous uint8 tensor with ", dim,
@@ -453,6 +454,7 @@ at::Tensor block_linear(const std::string& who_s, const at::Tensor& x_in, const 
     if (global_scale) TORCH_CHECK(global_scale->scalar_type() == at::kFloat && global_scale->numel() == 1, who, ": global_scale must be one float32 value");
     no_gradient(who, x_in);
     if (bias) no_gradient(who, *bias);
+    if (global_scale) no_gradient(who, *global_scale);
     TORCH_CHECK(x_in.is_cuda(), who, ": x must be a CUDA tensor");
     same_device(who, "codes", codes, x_in);
     same_device(who, "scales", scales, x_in);

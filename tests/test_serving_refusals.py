@@ -140,3 +140,25 @@ def test_c_abi_refuses_before_any_launch():
     assert "null pointer" in err("mpt_mx_cache_write", cache(), rows(), None, one, 0, strides, strides, None)
     assert "null pointer" in err("mpt_mx_cache_read", cache(), rows(), one, None, 0, None)
     assert "data type" in err("mpt_mx_cache_read", cache(), rows(), one, one, 5, None)
+
+
+def test_derivatives_are_not_dropped_in_silence():
+    """Every dense input: one that needs a gradient, and a dual tensor, whose tangent no_grad does not stop."""
+    import torch.autograd.forward_ad as fwd
+
+    c, s = weights()
+    nc, ns = weights(group=16)
+    cache = q.MXCache.empty(4, 2, 64, 16, device="cpu")
+    p, n, _ = batch()
+    k, x, b, one = torch.zeros(2, 1, 2, 64), torch.zeros(3, 64), torch.zeros(8), torch.ones(1)
+    calls = [(lambda t: q.mx_linear(t, c, s), x), (lambda t: q.mx_linear(x, c, s, t), b), (lambda t: q.nvfp4_linear(t, nc, ns, one), x),
+             (lambda t: q.nvfp4_linear(x, nc, ns, t), one), (lambda t: q.nvfp4_linear(x, nc, ns, one, t), b),
+             (lambda t: q.mx_cache_write(t, k, cache, p, n), k), (lambda t: q.mx_cache_write(k, t, cache, p, n), k),
+             (lambda t: q.mx_attention(t, cache, p, n), k), (lambda t: q.mx_attention(k, cache, p, n, out=t), k.clone())]
+    for call, t in calls:
+        refused("backward", call, t.clone().requires_grad_())
+        with torch.no_grad():
+            refused("CUDA", call, t.clone().requires_grad_())
+            with fwd.dual_level():
+                refused("forward-mode", call, fwd.make_dual(t.clone(), torch.ones_like(t)))
+            refused("CUDA", call, t)
