@@ -403,7 +403,8 @@ MPT_API int mpt_mx_cache_read(const mpt_mx_cache *cache, const mpt_mx_batch *bat
 
 /* Attention of the new rows over their sequences' tokens in the cache: out = softmax(scale * q K^T) V over the tokens t
  * at most at the row's position p with window == 0, t > p - window or t < sinks.  Query head h reads kv head
- * h / (q_heads / heads).  q: [rows, q_heads, dim] with strides as above; out: contiguous.  A row that sees nothing
+ * h / (q_heads / heads).  q: [rows, q_heads, dim] with strides as above; out: contiguous; it is q, with the
+ * same strides, or shares no memory with it.  A row that sees nothing
  * gives zeros; rows behind the last sequence are zeroed where `zero_tail` is set and left as they were otherwise.
  * `workspace`: mpt_mx_attention_workspace_bytes() bytes at a multiple of 256, of this call alone until it is done. */
 MPT_API size_t mpt_mx_attention_workspace_bytes(const mpt_mx_cache *cache, const mpt_mx_batch *batch, int q_heads, int dtype,

@@ -873,6 +873,14 @@ def _row_strides(t):
     return (ctypes.c_int64 * 3)(t.stride(0) if t.dim() == 4 else 0, t.stride(t.dim() - 3), t.stride(t.dim() - 2))
 
 
+def _shares_memory(t, out):
+    """Whether ``t`` may share memory with the contiguous tensor ``out`` and is not the same tensor."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    a, b = t.data_ptr(), out.data_ptr()
+    apart = a + (last + 1) * t.element_size() <= b or b + out.numel() * out.element_size() <= a
+    return not apart and not (a == b and t.is_contiguous())
+
+
 def mx_cache_write(k, v, cache, pages, lens, starts=None):
     """Quantizes the new rows of K and V into the pages of an MX cache."""
     if _ext is not None:
@@ -935,6 +943,8 @@ def mx_attention(q, cache, pages, lens, starts=None, scale=1.0, window=0, sinks=
         q = q if q.stride(-1) == 1 else q.contiguous()
         o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
         if o.numel():
+            if out is not None and _shares_memory(q, out):
+                q = q.clone()
             need = _cabi.lib().mpt_mx_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(b), heads, dtype, window, sinks)
             ws = _workspace(need, q.device)
             call("mpt_mx_attention", ctypes.byref(c), ctypes.byref(b), ptr(q), dtype, _row_strides(q), heads, scale, window, sinks, ptr(o),

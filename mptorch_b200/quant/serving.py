@@ -84,8 +84,8 @@ def mx_attention(q: torch.Tensor, cache, pages: torch.Tensor, lens: torch.Tensor
 
     q [sequences, new, heads, head_dim], or [rows, heads, head_dim] with ``starts``; query head h reads kv head
     ``h // (heads / kv_heads)``; ``scale`` is 1 / sqrt(head_dim) unless given.  With ``window`` a token sees the last ``window``
-    positions, its own among them, and the first ``sinks`` ones.  A row that sees nothing gives zeros.  ``out`` takes the result;
-    its rows behind the last sequence are left as they were."""
+    positions, its own among them, and the first ``sinks`` ones.  A row that sees nothing gives zeros.  ``out`` takes the result
+    and may be q itself or share memory with it; its rows behind the last sequence are left as they were."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.shape[-1] else 1.0
     return _be.mx_attention(q, cache, pages, lens, starts, float(scale), window, sinks, out)

@@ -528,6 +528,14 @@ std::array<int64_t, 3> row_strides(const at::Tensor& t) {
     const int64_t d = t.dim();
     return {d == 4 ? t.stride(0) : 0, t.stride(d - 3), t.stride(d - 2)};
 }
+// whether `t` may share memory with the contiguous tensor `out` and is not the same tensor: rows would be written before they are read
+bool shares_memory(const at::Tensor& t, const at::Tensor& out) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    const char *a = static_cast<const char*>(t.data_ptr()), *b = static_cast<const char*>(out.data_ptr());
+    const bool apart = a + (last + 1) * t.element_size() <= b || b + out.numel() * out.element_size() <= a;
+    return !apart && !(a == b && t.is_contiguous());
+}
 at::Tensor dense_last(const at::Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 
 void mx_cache_write(at::Tensor k_in, at::Tensor v_in, std::vector<at::Tensor> cache, at::Tensor pages, at::Tensor lens, std::optional<at::Tensor> starts) {
@@ -582,9 +590,10 @@ at::Tensor mx_attention(at::Tensor q_in, std::vector<at::Tensor> cache, at::Tens
     if (out_in) same_device(who, "out", *out_in, q_in);
     serving_devices(who, q_in, cache, pages, lens, starts);
     c10::cuda::CUDAGuard guard(q_in.device());
-    const at::Tensor q = dense_last(q_in);
+    at::Tensor q = dense_last(q_in);
     at::Tensor out = out_in ? *out_in : at::empty(q.sizes(), q.options());
     if (out.numel() == 0) return out;
+    if (out_in && shares_memory(q, out)) q = q.clone();
     const auto qs = row_strides(q);
     const size_t need = mpt_mx_attention_workspace_bytes(&s.cache, &s.batch, (int)heads, dtype, (int)window, (int)sinks);
     const at::Tensor ws = workspace(need, q);

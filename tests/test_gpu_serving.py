@@ -881,3 +881,29 @@ def test_attention_chunks_after_a_wait_that_ran_out(q, dtype, dim, group):
         _cabi.lib().mpt_test_attention_wait_runs_out(-1)
     assert held[0] == 0 and held[0] <= held[1] <= held[2]
     assert torch.equal(q.mx_attention(qry, cache, pages, ln, starts), clean)
+
+
+@pytest.mark.parametrize("route", ["ext", "ctypes"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("new", [1, 20, 300])
+def test_attention_into_the_memory_of_q(q, dtype, new, route, monkeypatch):
+    """out is q, begins some rows before or behind it, or has its heads in another order."""
+    from mptorch_b200 import backend as be
+
+    if route == "ctypes":
+        monkeypatch.setattr(be, "_ext", None)
+    lens = [new + 300, new + 40, new]
+    qry, cache, pages, ln, _ = setup(q, lens, [new] * 3, 2, 4, 64, 16, "e4m3", dtype, 7, uniform=True)
+    want = q.mx_attention(qry, cache, pages, ln)
+    mine = qry.clone()
+    assert q.mx_attention(mine, cache, pages, ln, out=mine) is not None and torch.equal(mine, want)
+    for shift in (-3, -1, 1, 2):
+        room = torch.zeros(qry.numel() + 6 * 64, device="cuda", dtype=dtype)
+        there = room[3 * 64:3 * 64 + qry.numel()].view_as(qry).copy_(qry)
+        out = room[(3 + shift) * 64:(3 + shift) * 64 + qry.numel()].view_as(qry)
+        q.mx_attention(there, cache, pages, ln, out=out)
+        assert torch.equal(out, want)
+    turned = qry.transpose(1, 2).contiguous()                       # [sequences, heads, new, dim]
+    out = turned.view(qry.shape)
+    q.mx_attention(turned.transpose(1, 2), cache, pages, ln, out=out)
+    assert torch.equal(out, want)
