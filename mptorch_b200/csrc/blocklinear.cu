@@ -126,17 +126,18 @@ __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const 
     if (threadIdx.x < 16) tops[threadIdx.x] = 0u;
     __syncthreads();
     const int per_row = p.n_in >> 3, padded = chunks * (kChunk >> 3);
+    float row_top = 0.f;                      // of a single row
     for (int i = threadIdx.x; i < p.rows * per_row; i += 32 * kWarps) {
         float v[8], top = 0.f;
         read8(p.x, p.dtype, p.x_vec, (int64_t)i * 8, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) { const float a = fabsf(v[e]); if (a < INFINITY) top = fmaxf(top, a); }
-        if (p.rows == 1) {
-            const uint32_t all = __reduce_max_sync(__activemask(), __float_as_uint(top));
-            if (lane == 0) atomicMax(&tops[0], all);
-        } else {
-            atomicMax(&tops[i / per_row], __float_as_uint(top));
-        }
+        if (p.rows == 1) row_top = fmaxf(row_top, top);
+        else atomicMax(&tops[i / per_row], __float_as_uint(top));
+    }
+    if (p.rows == 1) {
+        const uint32_t all = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(row_top));
+        if (lane == 0) atomicMax(&tops[0], all);
     }
     __syncthreads();
     if (threadIdx.x < p.rows) exponent[threadIdx.x] = row_exponent(tops[threadIdx.x]);

@@ -907,3 +907,19 @@ def test_attention_into_the_memory_of_q(q, dtype, new, route, monkeypatch):
     out = turned.view(qry.shape)
     q.mx_attention(turned.transpose(1, 2), cache, pages, ln, out=out)
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("k", [32, 96, 1120, 4128, 8224])
+def test_linear_one_row_finds_its_largest_value_anywhere(q, fmt, dtype, k):
+    """A row is scaled by its largest magnitude, wherever it stands: a power of two beside zeros comes back exactly times the weight."""
+    g = gen(k)
+    codes, scales, glob, w = pack(24, k, fmt, g)
+    for at in {0, 7, 8, 31, k // 2, k - 32, k - 9, k - 1}:
+        x = torch.zeros(1, k, device="cuda", dtype=dtype)
+        x[0, at] = 2.0 ** 60
+        x[0, (at + 11) % k] = 2.0 ** 45
+        want = x.double() @ w.t()
+        got = linear(q, x, codes, scales, glob).double()
+        assert ((got - want).abs() <= (2.0 ** -22 + half_ulp(dtype)) * want.abs() + 2.0 ** -22 * (x.double().abs() @ w.abs().t())).all()
