@@ -162,3 +162,32 @@ def test_derivatives_are_not_dropped_in_silence():
             with fwd.dual_level():
                 refused("forward-mode", call, fwd.make_dual(t.clone(), torch.ones_like(t)))
             refused("CUDA", call, t)
+
+
+def test_calls_in_the_readme_take_their_arguments_in_order():
+    """Each call of this package in a code line of README.md fits the function, and a name that is a parameter's stands in its place."""
+    import ast
+    import inspect
+    import os
+
+    text = open(os.path.join(os.path.dirname(__file__), "..", "README.md")).read()
+    seen = set()
+    for line in text.splitlines():
+        if not line.startswith("    ") or "q." not in line:
+            continue
+        try:
+            tree = ast.parse(line.strip())
+        except SyntaxError:
+            continue
+        for call in (n for n in ast.walk(tree) if isinstance(n, ast.Call) and isinstance(n.func, ast.Attribute)):
+            fn = getattr(q, call.func.attr, None) if isinstance(call.func.value, ast.Name) and call.func.value.id == "q" else None
+            if fn is None:
+                continue
+            seen.add(call.func.attr)
+            sig = inspect.signature(fn)
+            sig.bind(*call.args, **{k.arg: k.value for k in call.keywords})
+            names = list(sig.parameters)
+            for i, a in enumerate(call.args):
+                if isinstance(a, ast.Name) and a.id in names:
+                    assert names[i] == a.id, line
+    assert {"mx_linear", "mx_cache_write", "mx_attention", "float_quantize", "float_mm"} <= seen
