@@ -923,3 +923,39 @@ def test_linear_one_row_finds_its_largest_value_anywhere(q, fmt, dtype, k):
         want = x.double() @ w.t()
         got = linear(q, x, codes, scales, glob).double()
         assert ((got - want).abs() <= (2.0 ** -22 + half_ulp(dtype)) * want.abs() + 2.0 ** -22 * (x.double().abs() @ w.abs().t())).all()
+
+
+@pytest.mark.parametrize("fmt,fold,rows,n,k", [("nvfp4", 1536, 24, 4000, 9632), ("nvfp4", 1536, 130, 300, 9632), ("nvfp4", 1536, 300, 1000, 16384),
+                                               ("mxfp4", 4096, 24, 300, 32768), ("mxfp4", 4096, 130, 260, 32768)])
+def test_linear_many_rows_sums_of_one_sign(q, fmt, fold, rows, n, k):
+    """float32 rows: sums of the tile kernel are added up in memory after 1536 (NVFP4) or 4096 (MXFP4) products.  Sums that run through lose
+    half of the bound for each product on average, K 2^-28: 3.6e-5 for 9632 and 1.2e-4 for 32768, against 1.2e-5 and 3.2e-5 allowed."""
+    g = gen(rows + n)
+    codes, scales, glob, _ = pack(n, k, fmt, g)
+    codes &= 0x77
+    w = torch.stack([field_value(codes & 15, 2, 1), field_value(codes >> 4, 2, 1)], -1).flatten(-2)
+    w = w * (e8m0_value(scales).repeat_interleave(32, -1) if glob is None else e4m3_value(scales).repeat_interleave(16, -1) * glob.double())
+    x = torch.randn(rows, k, device="cuda", generator=g).abs()
+    want = x.double() @ w.t()
+    assert ((linear(q, x, codes, scales, glob).double() - want).norm() / want.norm()).item() <= cut_off_bound(fold, k)
+
+
+@pytest.mark.parametrize("dim,group", [(32, 1), (64, 1), (96, 2), (128, 1)])
+def test_attention_chunks_over_long_contexts_of_one_sign(q, dim, group):
+    """float32 chunks: sums are added up in registers after 512 tokens: 4.7e-6 is allowed, and 6000 tokens in one sum lose 2.2e-5 on average."""
+    lens, new = [6000, 5000], [130, 200]
+    qry, cache, pages, ln, starts = setup(q, lens, new, 4, group, dim, 64, "e4m3", torch.float32, dim)
+    cache.v_codes.bitwise_and_(127)
+    got, at, off, norm = q.mx_attention(qry, cache, pages, ln, starts, scale=0.02), 0, 0.0, 0.0
+    for s, n in enumerate(new):
+        t = torch.arange(lens[s], device="cuda")
+        slot = pages[s].long()[t // 64]
+        hidden = t > lens[s] - n + torch.arange(n, device="cuda")[:, None]
+        for h in range(4):
+            k, v = (values(cache[i][slot, h, t % 64], cache[i + 1][slot, h, t % 64], dim) for i in (0, 2))
+            for j in range(h * group, (h + 1) * group):
+                o = torch.softmax(((qry[at:at + n, j].double() @ k.t()) * 0.02).masked_fill(hidden, -math.inf), -1) @ v
+                off += (got[at:at + n, j].double() - o).square().sum().item()
+                norm += o.square().sum().item()
+        at += n
+    assert math.sqrt(off / norm) <= cut_off_bound(512, max(lens))
