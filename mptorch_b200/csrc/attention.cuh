@@ -196,16 +196,6 @@ __device__ __forceinline__ void zero_outside(const AttentionParams& p) {
     }
 }
 
-__device__ __forceinline__ float load_value(const void* p, int dtype, int64_t i) {
-    return dtype == MPT_DTYPE_F32 ? static_cast<const float*>(p)[i]
-         : dtype == MPT_DTYPE_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : __half2float(static_cast<const __half*>(p)[i]);
-}
-__device__ __forceinline__ void store_value(void* p, int dtype, int64_t i, float v) {
-    if (dtype == MPT_DTYPE_F32) static_cast<float*>(p)[i] = v;
-    else if (dtype == MPT_DTYPE_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(p)[i] = __float2half_rn(v);
-}
-
 __device__ __forceinline__ float exp2_fast(float x) {       // relative error 2^-22; exact at integers; results below 2^-126 are zero
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

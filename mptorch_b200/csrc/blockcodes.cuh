@@ -80,6 +80,26 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {   // p: a mu
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<uint4*>(t)[i];
 }
 
+__device__ __forceinline__ float load_value(const void* p, int dtype, int64_t i) {
+    return dtype == MPT_DTYPE_F32 ? static_cast<const float*>(p)[i]
+         : dtype == MPT_DTYPE_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : __half2float(static_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void store_value(void* p, int dtype, int64_t i, float v) {
+    if (dtype == MPT_DTYPE_F32) static_cast<float*>(p)[i] = v;
+    else if (dtype == MPT_DTYPE_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// fp32 sums of binary16 products, 16 x 8 by 16 at a time: added to c, or begun
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // A paged MX cache and a batch of sequences in it, as kernels take them.
 struct CacheView {
     uint8_t *k_codes, *k_scales, *v_codes, *v_scales;

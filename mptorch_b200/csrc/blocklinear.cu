@@ -32,14 +32,6 @@ template <int N>
 __device__ __forceinline__ void cp_small(uint32_t dst, const void* src, int bytes) {   // 4 or 8
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(dst), "l"(src), "n"(N), "r"(bytes));
 }
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
 __device__ __forceinline__ uint32_t times(uint32_t a, __half2 s) {
     const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), s);
     return *reinterpret_cast<const uint32_t*>(&r);
@@ -192,8 +184,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const 
                     e2m1x8_to_half(*reinterpret_cast<const uint32_t*>(w + g * kPitch + b * 16 + tig * 4), a);
                     e2m1x8_to_half(*reinterpret_cast<const uint32_t*>(w + (g + 8) * kPitch + b * 16 + tig * 4), d);
                     const bool here = mine && b == my_block;
-                    mma(c, a[0], d[0], a[1], d[1], here ? xv.x : 0u, here ? xv.y : 0u);
-                    mma(c, a[2], d[2], a[3], d[3], here ? xv.z : 0u, here ? xv.w : 0u);
+                    mma16816(c, a[0], d[0], a[1], d[1], here ? xv.x : 0u, here ? xv.y : 0u);
+                    mma16816(c, a[2], d[2], a[3], d[3], here ? xv.z : 0u, here ? xv.w : 0u);
                 }
                 // sums of row g (and g + 8) in this lane: groups 2 tig and 2 tig + 1 (MXFP4: modulo four)
                 const int at = NV ? 2 * tig : 2 * (tig & 1);
@@ -269,9 +261,9 @@ __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const 
                         }
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            if (b == 0) mma_first(part[n], a[0], d[0], a[1], d[1], x[n].x, x[n].y);
-                            else mma(part[n], a[0], d[0], a[1], d[1], x[n].x, x[n].y);
-                            mma(part[n], a[2], d[2], a[3], d[3], x[n].z, x[n].w);
+                            if (b == 0) mma16816_first(part[n], a[0], d[0], a[1], d[1], x[n].x, x[n].y);
+                            else mma16816(part[n], a[0], d[0], a[1], d[1], x[n].x, x[n].y);
+                            mma16816(part[n], a[2], d[2], a[3], d[3], x[n].z, x[n].w);
                         }
                     } else {
                         const int e0 = (s0.x >> (8 * b)) & 255u, e1 = (s1.x >> (8 * b)) & 255u;
@@ -280,8 +272,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const 
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             float c[4];
-                            mma_first(c, a[0], d[0], a[1], d[1], x[n].x, x[n].y);
-                            mma(c, a[2], d[2], a[3], d[3], x[n].z, x[n].w);
+                            mma16816_first(c, a[0], d[0], a[1], d[1], x[n].x, x[n].y);
+                            mma16816(c, a[2], d[2], a[3], d[3], x[n].z, x[n].w);
                             acc[n][0] = fmaf(c[0], f0, acc[n][0]);
                             acc[n][1] = fmaf(c[1], f0, acc[n][1]);
                             acc[n][2] = fmaf(c[2], f1, acc[n][2]);
@@ -341,8 +333,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1) block_linear_few_kernel(const 
             if (PIECES == 2) v = fmaf(v2, 0x1p-11f, v);
             if (n < p.n_out) {
                 v = scale_by_power(v, (NV ? 0 : ref - 127) - exponent[m]) * glob;
-                if (p.bias != nullptr) v += read_value(p.bias, p.dtype, n);
-                write_value(p.y, p.dtype, (int64_t)m * p.n_out + n, v);
+                if (p.bias != nullptr) v += load_value(p.bias, p.dtype, n);
+                store_value(p.y, p.dtype, (int64_t)m * p.n_out + n, v);
             }
         }
         team_sync();

@@ -24,15 +24,6 @@ __device__ __forceinline__ float scale_by_power(float v, int e) {
 // The power of two that brings a row of x with the largest finite magnitude of these bits to [2^14, 2^15)
 __device__ __forceinline__ int row_exponent(uint32_t top_bits) { return top_bits ? min(max(127 + 14 - (int)(top_bits >> 23), -126), 126) : 0; }
 
-__device__ __forceinline__ float read_value(const void* p, int dtype, int64_t i) {
-    return dtype == MPT_DTYPE_F32 ? static_cast<const float*>(p)[i]
-         : dtype == MPT_DTYPE_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : __half2float(static_cast<const __half*>(p)[i]);
-}
-__device__ __forceinline__ void write_value(void* p, int dtype, int64_t i, float v) {
-    if (dtype == MPT_DTYPE_F32) static_cast<float*>(p)[i] = v;
-    else if (dtype == MPT_DTYPE_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(p)[i] = __float2half_rn(v);
-}
 __device__ __forceinline__ void read8(const void* p, int dtype, bool vec, int64_t i, float (&v)[8]) {
     if (dtype == MPT_DTYPE_F32) load8(static_cast<const float*>(p) + i, vec, v);
     else if (dtype == MPT_DTYPE_BF16) load8(static_cast<const __nv_bfloat16*>(p) + i, vec, v);

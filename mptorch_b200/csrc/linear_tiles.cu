@@ -157,7 +157,7 @@ __device__ __noinline__ void tile_end(const TilesParams& p, uint32_t tmem, const
     tmem_fence_after();
     const int rw = (warp & 3) * 32 + lane, n = rt * kRowsW + rw;
     const float glob = NV && l.global_scale != nullptr ? __ldg(l.global_scale) : 1.f;
-    const float bias = whole && l.bias != nullptr && n < l.n_out ? read_value(l.bias, l.dtype, n) : 0.f;
+    const float bias = whole && l.bias != nullptr && n < l.n_out ? load_value(l.bias, l.dtype, n) : 0.f;
     const int we = NV ? 0 : top_e[rw] - 140;
     const bool near = we >= -60 && we <= 60;                       // no product leaves fp32's range on the way
     const float wpow = __uint_as_float((uint32_t)(127 + (near ? we : 0)) << 23);
@@ -185,7 +185,7 @@ __device__ __noinline__ void tile_end(const TilesParams& p, uint32_t tmem, const
                 if (!ok) y = __uint_as_float(0x7FC00000u);
                 if (more) kept[(c0 + k) * kRowsW] = y;
                 else if (!whole) part[(c0 + k) * kRowsW] = y;
-                else if (n < l.n_out) write_value(l.y, l.dtype, (int64_t)m * l.n_out + n, y + bias);
+                else if (n < l.n_out) store_value(l.y, l.dtype, (int64_t)m * l.n_out + n, y + bias);
             }
         }
         __syncwarp();
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(256) linear_far_kernel(const TilesParams p) {
         const int m0 = ((int)(item % each) * 8 + (threadIdx.x >> 5)) * kFarCols;
         if (m0 >= l.rows) continue;
         const uint8_t *codes = l.codes + n * (l.n_in >> 1), *scales = l.scales + n * groups;
-        const float bias = l.bias != nullptr ? read_value(l.bias, l.dtype, n) : 0.f;
+        const float bias = l.bias != nullptr ? load_value(l.bias, l.dtype, n) : 0.f;
         float sum[kFarCols] = {};
         for (int k = lane; k < l.n_in / 8; k += 32) {
             float w[8], x[kFarCols][8];
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(256) linear_far_kernel(const TilesParams p) {
         for (int j = 0; j < kFarCols; ++j) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum[j] += __shfl_xor_sync(0xFFFFFFFFu, sum[j], o);
-            if (lane == 0 && m0 + j < l.rows) write_value(l.y, l.dtype, (m0 + j) * (int64_t)l.n_out + n, sum[j] + bias);
+            if (lane == 0 && m0 + j < l.rows) store_value(l.y, l.dtype, (m0 + j) * (int64_t)l.n_out + n, sum[j] + bias);
         }
     }
 }
@@ -521,8 +521,8 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const TilesParams p) {
         float y = 0.f;
         for (int k = blockIdx.x; k <= last; ++k)
             y += p.partial[(2 * (int64_t)k + (k == (int)blockIdx.x && k * p.per < p0 ? 1 : 0)) * p.cols * kRowsW + i];
-        if (l.bias != nullptr) y += read_value(l.bias, l.dtype, n);
-        write_value(l.y, l.dtype, (int64_t)m * l.n_out + n, y);
+        if (l.bias != nullptr) y += load_value(l.bias, l.dtype, n);
+        store_value(l.y, l.dtype, (int64_t)m * l.n_out + n, y);
     }
 }
 
