@@ -949,4 +949,6 @@ def mx_attention(q, cache, pages, lens, starts=None, scale=1.0, window=0, sinks=
             ws = _workspace(need, q.device)
             call("mpt_mx_attention", ctypes.byref(c), ctypes.byref(b), ptr(q), dtype, _row_strides(q), heads, scale, window, sinks, ptr(o),
                  int(out is None), ptr(ws), need, stream_ptr(q.device))
+            if out is not None and not out.is_inference():
+                torch.autograd.graph.increment_version(out)
     return o

@@ -599,6 +599,7 @@ at::Tensor mx_attention(at::Tensor q_in, std::vector<at::Tensor> cache, at::Tens
     const at::Tensor ws = workspace(need, q);
     check(mpt_mx_attention(&s.cache, &s.batch, q.data_ptr(), dtype, qs.data(), (int)heads, (float)scale, (int)window, (int)sinks, out.data_ptr(),
                            out_in ? 0 : 1, need ? ws.data_ptr() : nullptr, need, stream()));
+    if (out_in && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();      // written in place
     return out;
 }
 

@@ -903,6 +903,9 @@ def test_attention_into_the_memory_of_q(q, dtype, new, route, monkeypatch):
         out = room[(3 + shift) * 64:(3 + shift) * 64 + qry.numel()].view_as(qry)
         q.mx_attention(there, cache, pages, ln, out=out)
         assert torch.equal(out, want)
+    version = out._version
+    q.mx_attention(qry, cache, pages, ln, out=out)
+    assert out._version > version                                   # autograd learns of it
     turned = qry.transpose(1, 2).contiguous()                       # [sequences, heads, new, dim]
     out = turned.view(qry.shape)
     q.mx_attention(turned.transpose(1, 2), cache, pages, ln, out=out)
@@ -959,3 +962,60 @@ def test_attention_chunks_over_long_contexts_of_one_sign(q, dim, group):
                 norm += o.square().sum().item()
         at += n
     assert math.sqrt(off / norm) <= cut_off_bound(512, max(lens))
+
+
+@pytest.mark.parametrize("rows", [3, 24, 300])
+def test_mxfp4_products_in_graphs_and_on_streams(q, rows):
+    """Weights with and without far blocks: two captured graphs replayed in turn with new inputs, and calls on several streams at once."""
+    g = gen(rows)
+    sets = []
+    for i in range(2):
+        codes, scales, _, _ = pack(3000, 1056, "mxfp4", g)
+        if i:
+            scales[::7, 3] = 30
+        sets.append([torch.randn(rows, 1056, device="cuda", generator=g), codes, scales])
+    eager = [[q.mx_linear(x, c, s) for x in (sets[0][0], sets[1][0])] for _, c, s in sets]
+    static = [[t.clone() for t in a] for a in sets]
+    graphs, outs = [], []
+    for a in static:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(q.mx_linear(*a))
+        graphs.append(gr)
+    for turn in range(3):
+        for i, gr in enumerate(graphs):
+            static[i][0].copy_(sets[turn % 2][0])
+            gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, e[turn % 2]) for o, e in zip(outs, eager))
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = [[] for _ in streams]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(q.mx_linear(sets[i & 1][0], *sets[i >> 1][1:]))
+    torch.cuda.synchronize()
+    for i, results in enumerate(got):
+        assert all(torch.equal(r, eager[i >> 1][i & 1]) for r in results)
+
+
+@pytest.mark.parametrize("new", [1, 20])
+def test_attention_of_blocks_of_zeros_and_single_large_values(q, new):
+    """V with blocks of zeros (whose scale is the smallest) and with one token far above the others, each row against 64 bits."""
+    dim, length = 96, new + 150
+    for dtype in TYPES:
+        qry, cache, pages, ln, starts = setup(q, [length], [new], 2, 2, dim, 16, "e4m3", dtype, 31)
+        g = gen(new)
+        zero = torch.rand(cache.v_scales.shape, device="cuda", generator=g) < 0.4
+        cache.v_scales.masked_fill_(zero, 0)
+        cache.v_codes.masked_fill_(zero.repeat_interleave(32, -1), 0)
+        want, tol = reference(qry, cache, pages, [length], [new], dim, 1 / math.sqrt(dim))
+        check_attention(q.mx_attention(qry, cache, pages, ln, starts), want, tol)
+        for t, scale in ((3, 200), (90, 160), (91, 90)):
+            cache.v_scales[pages[0, t // 16], 1, t % 16, 1] = scale
+        got = q.mx_attention(qry, cache, pages, ln, starts)
+        want, tol = reference(qry, cache, pages, [length], [new], dim, 1 / math.sqrt(dim))
+        if dtype == torch.float16:                                  # (a result beyond its range is an infinity)
+            got, want = got.float().clamp(-65504, 65504), want.clamp(-65504, 65504)
+        check_attention(got, want, tol)
