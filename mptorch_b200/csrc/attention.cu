@@ -18,8 +18,8 @@
 // 3.8e-7 and 1.4e-7.
 //
 // Measured on a B200 (the bytes at the measured bandwidth in brackets): one token each over 16 contexts up to 32768, 32 heads on 8 of
-// 128, E4M3, bfloat16 139 us (97.9: issue slots 54 % busy, DRAM 60 %; twelve warps an SM do not cover the latency of conversions and products);
-// over a window of 1024 with 4 sinks, 96 sequences, 24 heads on 8 of 96, E2M1, float16 60 us (11.8: an element is half a byte, and
+// 128, E4M3, bfloat16 136 us (97.9: issue slots 57 % busy, DRAM 58 %; twelve warps an SM do not cover the latency of conversions and products);
+// over a window of 1024 with 4 sinks, 96 sequences, 24 heads on 8 of 96, E2M1, float16 62 us (11.8: an element is half a byte, and
 // the conversions are twice as many a byte); four sequences up to 1024, 12 heads of 64, float32 18.4 us (0.6: host time, two launches).
 #define MPT_DEFINE_JOIN
 #include "attention.cuh"

@@ -9,12 +9,14 @@
 // m is moved, and O multiplied, only when a row's maximum has grown by more than 2^8 over it; p is at most 2^8 then.
 //
 // Accuracy.  bfloat16 queries are one operand; float16 and float32 ones are the sum of two and three bfloat16 pieces (16 and 24
-// bits), and so are their weights p; sums are fp32 throughout, and short ones where three pieces are worth it (kFold).
+// bits), and so are their weights p; sums are fp32 throughout, and short ones where three pieces are worth it (kFold).  With
+// bfloat16 weights the 1024-token chunks below are 2.2e-3 off, where fp32 arithmetic that is rounded to bfloat16 once is 1.7e-3 off; a
+// second piece of the weights would be half as many products again.
 //
-// Measured on a B200: 1024-token chunks of two sequences over 8192, 32 heads on 8 of 128, E4M3, bfloat16 310 us (115.5 for the
-// products at the measured rate of bfloat16; 610 TFLOP/s).  The expansion takes 20 us of it and the join of cut tiles some 10; what bounds
+// Measured on a B200: 1024-token chunks of two sequences over 8192, 32 heads on 8 of 128, E4M3, bfloat16 312 us (115.5 for the
+// products at the measured rate of bfloat16; 605 TFLOP/s).  The expansion takes 18 us of it and the join of cut tiles some 10; what bounds
 // the rest is the chain of a tile, product, softmax, product, two CTAs on an SM hiding each other's.  Six ragged chunks up to 300 over
-// 2000, 12 heads of 64, float32: 84 us (2.9), three pieces of q and of p each, and runs of a few tiles.
+// 2000, 12 heads of 64, float32: 85 us (2.9), three pieces of q and of p each, and runs of a few tiles.
 #include "attention.cuh"
 #include "attention_chunk.cuh"
 #include "tcgen05.cuh"

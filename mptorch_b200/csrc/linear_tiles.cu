@@ -10,15 +10,17 @@
 //      64 at a time (a warp then reads 128 bytes of each of four rows), two pieces ahead in registers: one conversion and one
 //      multiplication for two weights.  NVFP4: a code times its E4M3 scale is exact (six bits).  MXFP4: a code times
 //      2^(13 + e - E), E the row's largest exponent, is exact down to e = E - 36; rows with smaller blocks that are not all zeros are
-//      found here and computed by a kernel at the end, in fp32 (rare, and slow: 1024 x 4096 by 4096 takes 120 us without, 197 with 40 such rows, 6.6 ms with nothing else).
+//      found here and computed by a kernel at the end, in fp32 (rare, and slow: 1024 x 4096 by 4096 takes 123 us without, 200 with 40 such
+//      rows, 6.6 ms with nothing else).
 //      Sums are fp32 in tensor memory, those of float32's second pieces apart, and the powers of two are put back at the end.
 //   3. A tile that a run ends in is left in parts, which are added up in order.
 //
 // Measured on a B200 (bf16 products at the measured rate and bytes at the measured bandwidth in brackets): 37 x 4096 by 11008 NVFP4
-// weights, float16, 36.8 us (4.1 of bytes: x's tiles, the parts of cut tiles and three kernels' starts are most of it); 1024 x 4096 by
-// 4096 MXFP4 weights, float32, 120 us (42 of products, two pieces each); 1024 x 4096 by 11008 NVFP4, bfloat16, 176 us (56).  What bounds
-// it is the warps that turn codes into weights, again for every 256 columns of x (128 rows of float32): they wait for places in the
-// ring and for codes on the way, with the issue slots 35 % busy and the tensor cores 37 % in the second of these.
+// weights, float16, 37.1 us (4.1 of bytes: the tile kernel alone takes 30, x's tiles 6 and the join 12, which overlap); 1024 x 4096 by
+// 4096 MXFP4 weights, float32, 123 us (42 of products, two pieces each; 3 for the look at far blocks); 1024 x 4096 by 11008 NVFP4,
+// bfloat16, 174 us (56).  What bounds it is the warps that turn codes into weights, again for every 256 columns of x (128 rows of
+// float32): they wait for places in the ring and for codes on the way, with the issue slots 35 % busy and the tensor cores 36 % in the
+// second of these.
 #include <type_traits>
 
 #include "blocklinear.cuh"
@@ -35,7 +37,8 @@ constexpr int kRowsW = 128, kBlock = 64, kSuper = 4, kWorkers = 512, kThreads = 
 // x 4096 by 4096: 3.3e-6 of the result without, 1.7e-6 with 8, 1.1e-6 with 6, 8.1e-7 with 4 (fp32 arithmetic as torch has it 1.1e-6), in
 // 110, 128, 145 and 155 us.  MXFP4 loses less: 33 x 4096 by 18889 1.7e-6 without, 9152 4.4e-6 without and 1.5e-6 with 16 (torch's 1.1e-6
 // and 1.6e-6), the last in 151 us; it pays more for it, since that kernel has no registers left (1024 x 4096 by 4096: 120 us without,
-// 177 with 8).  bfloat16 and float16 round the result far more coarsely.
+// 177 with 8; 4352 by 4096, the first size with 16, 182).  Those are weights of normal values; where all codes are as frequent the errors are
+// twice as large (4096: 3e-6), and 1.1e-5 where all products have one sign.  bfloat16 and float16 round the result far more coarsely.
 constexpr int kFoldNv = 6, kFoldMx = 16;
 constexpr int kPartW = kRowsW * 128;                               // bytes of a tile of W: 128 rows of 64 weights
 

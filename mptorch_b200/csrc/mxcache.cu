@@ -7,7 +7,7 @@
 // elements of K or of V of one token, all heads after one another, so that the token's sequence and page are looked up once; a lane has
 // four pieces under way at a time, and four lanes share a block and find its maximum with two shuffles.  K and V go in one launch.
 //
-// Measured on a B200: seven prompts of up to 4096 tokens, 8 heads of 128, bfloat16 to and from E2M1: 70 us for both calls (25.7 for
+// Measured on a B200: seven prompts of up to 4096 tokens, 8 heads of 128, bfloat16 to and from E2M1: 71 us for both calls (25.7 for
 // the bytes at the measured bandwidth); instruction issue bounds the writes (45 us) and memory latency the
 // reads (23 us).  With a warp for each 32 pieces, which looks up its token each time, both took 99 us.  One token each of 32 sequences
 // (12 heads of 64, float32): 26 us for both, host time.

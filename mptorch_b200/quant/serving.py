@@ -2,7 +2,10 @@
 MX format, and attention over it.
 
 These are the operators that read the codes which ``mx_quantize`` and ``nvfp4_quantize`` hand out.  Dense tensors are float32,
-bfloat16 or float16; sums, softmax statistics and scales are held in 32 bits and a result is rounded to its type once.  They
+bfloat16 or float16; sums, softmax statistics and scales are held in 32 bits and a result is rounded to its type once.  The
+operands of the products have 16 bits: rows of x and q in bfloat16 and float16 are held exactly down to 2^-29 of their largest
+magnitude and to 2^-39 of it below, float32 ones to 22 bits and 2^-50; the weights of a softmax to 11 bits (chunks of 32 rows and
+more: 8 in bfloat16, 16 in float16, 24 in float32; fewer rows in float32: 22), and at least to 2^-26 of the row's largest.  They
 answer with a model and do not train it: an input that needs a gradient is refused while gradients are recorded, and so is one
 that carries a forward-mode tangent.
 
