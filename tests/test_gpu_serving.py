@@ -1019,3 +1019,30 @@ def test_attention_of_blocks_of_zeros_and_single_large_values(q, new):
         if dtype == torch.float16:                                  # (a result beyond its range is an infinity)
             got, want = got.float().clamp(-65504, 65504), want.clamp(-65504, 65504)
         check_attention(got, want, tol)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("rows,n,k", [(70000, 48, 32768), (70000, 32800, 64), (1, 300000, 32768), (20, 300000, 32768)])
+def test_linear_offsets_past_32_bits(q, fmt, rows, n, k):
+    """x, y, and packed weights of more than 2^31 elements or 2^32 bytes: places at the far end and in between."""
+    g = gen(rows + n)
+    codes, scales = torch.empty(n, k // 2, device="cuda", dtype=torch.uint8), torch.empty(n, k // (32 if fmt == "mxfp4" else 16), device="cuda", dtype=torch.uint8)
+    for i in range(0, n, 20000):
+        codes[i:i + 20000].random_(0, 256, generator=g)
+        scales[i:i + 20000].random_(112, 126, generator=g) if fmt == "mxfp4" else scales[i:i + 20000].random_(0, 127, generator=g)
+    if fmt == "mxfp4":
+        scales[-1, 0] = 20                                          # a block of its own kernel, at the far end
+    glob = None if fmt == "mxfp4" else torch.tensor([0.5], device="cuda")
+    x = torch.empty(rows, k, device="cuda", dtype=torch.bfloat16)
+    for i in range(0, rows, 10000):
+        x[i:i + 10000].normal_(generator=g)
+    y = linear(q, x, codes, scales, glob)
+    at_m = torch.unique(torch.tensor([0, 1, rows // 3, rows - 2, rows - 1], device="cuda").clamp(0, rows - 1))
+    at_n = torch.unique(torch.tensor([0, 17, n // 2, n - 3, n - 1], device="cuda"))
+    c, s = codes[at_n], scales[at_n]
+    v = torch.stack([field_value(c & 15, 2, 1), field_value(c >> 4, 2, 1)], -1).flatten(-2)
+    w = v * (e8m0_value(s).repeat_interleave(32, -1) if glob is None else e4m3_value(s).repeat_interleave(16, -1) * glob.double())
+    check_linear(y[at_m][:, at_n], x[at_m], w)
+    # and that nothing is zero or left out on a larger part
+    mean = y[-min(rows, 50):, -min(n, 1000):].float().abs().mean().item()
+    assert 0.5 < mean / y[:min(rows, 50), :min(n, 1000)].float().abs().mean().item() < 2
